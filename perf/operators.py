@@ -197,7 +197,7 @@ def _plain_quantize(s):
         x = x[s["rows"].long()]
     most = x.abs().amax(dim=1).clamp_min(LEAST)
     top = MOST8[s["q"]]
-    return {"q": (x / most[:, None] * top).clamp(-top, top).to(F8[s["q"]]), "scale": (most / top).float()}
+    return {"q": (x * top / most[:, None]).clamp(-top, top).to(F8[s["q"]]), "scale": (most / top).float()}
 
 
 def _in_groups(x, ends, most):
