@@ -189,6 +189,81 @@ int b200fp8_spmv_bell_f32(int m, int k, const void* ell_values, int a_dtype, lon
                           void* stream);
 
 /*
+ * The products of a layer of experts (a mixture layer): every group of rows has a weight matrix of its own.  No
+ * counterpart in the reference, whose operator has one matrix; layouts and FP8 formats are the operator's.
+ *
+ *   b200fp8_gemm_grouped        D[r][n] = ep(sum_k A[r][k] B[e][n][k])     A [rows][K]  B [experts][N][K]  D [rows][N]
+ *   b200fp8_gemm_grouped_dgrad  D[r][k] = ep(sum_n A[r][n] B[e][n][k])     A [rows][N]  B [experts][N][K]  D [rows][K]
+ *   b200fp8_gemm_grouped_wgrad  D[e][n][k] = ep(sum_{r in e} A[r][n] B[r][k])
+ *                                                                          A [rows][N]  B [rows][K]        D [experts][N][K]
+ *
+ * dgrad and wgrad are the two products of the backward pass (A is then the gradient of the output, in either FP8 format);
+ * they read the operands as the forward pass stored them, without transposed copies.
+ *
+ * ends: DEVICE, int32, one per expert: group e holds the rows [ends[e-1], ends[e]) (the first starts at 0).  It is read by
+ * the kernel, so that a router on the same stream may write it just before; the sizes need not be known on the host, and
+ * a group may be empty.  The kernel clamps every end to [0, rows] and to the largest end before it.  Rows of no group are
+ * left as they were in D.  An empty group's gradient in wgrad is beta * D (zero for beta = 0).
+ *
+ * ep is the epilogue of b200fp8_gemm_rowcol_epilogue (NULL: D = convert(sum)), with b_row_scale and bias holding one value
+ * per expert and column of D ([experts][columns of D]) and a_row_scale one per row; amax_d is taken over the rows of groups.
+ * wgrad sums over the rows: it takes alpha, beta, a_scale, b_scale, d_scale and amax_d only (operands with one scale each).
+ *
+ * ld*: row pitches; stride_b / stride_d: pitch from one expert's matrix to the next (elements; not read for one expert).
+ * Requirements: A and B 16-byte aligned; K, lda, ldb, stride_b and, in dgrad and wgrad, N multiples of 16; D aligned to its
+ * element (16 bytes, and rows of a multiple of 16 bytes, for the fast store path).  options: kernel (AUTO, PAIR_N256,
+ * CTA1_N256 or CTA1_N128) and max_ctas; depth and split_k must be 0.  Results do not depend on the kernel's schedule.
+ */
+int b200fp8_gemm_grouped(int experts, int rows, int k, int n, const int* ends, const void* a, int a_dtype, long long lda,
+                         const void* b, int b_dtype, long long ldb, long long stride_b, void* d, int d_dtype, long long ldd,
+                         const b200fp8_epilogue* epilogue, const b200fp8_options* options, void* stream);
+int b200fp8_gemm_grouped_dgrad(int experts, int rows, int k, int n, const int* ends, const void* a, int a_dtype, long long lda,
+                               const void* b, int b_dtype, long long ldb, long long stride_b, void* d, int d_dtype,
+                               long long ldd, const b200fp8_epilogue* epilogue, const b200fp8_options* options, void* stream);
+int b200fp8_gemm_grouped_wgrad(int experts, int rows, int k, int n, const int* ends, const void* a, int a_dtype, long long lda,
+                               const void* b, int b_dtype, long long ldb, void* d, int d_dtype, long long ldd, long long stride_d,
+                               const b200fp8_epilogue* epilogue, const b200fp8_options* options, void* stream);
+
+/*
+ * Rows of 16-bit floats (x_dtype B200FP8_OUT_BF16 or _F16) to rows of 8-bit floats with one FP32 scale each, the operands
+ * of the row-scaled products (a_row_scale, b_row_scale):
+ *
+ *     m = max(2^-80, largest finite |x[i][k]|),  scale[r] = m / top,  q[r][k] = nearest(x[i][k] / m * top)
+ *
+ * with i = index[r] (r itself for index = NULL) and top = 448 (E4M3) or 57344 (E5M2); nearest is round-to-nearest-even of
+ * the exact quotient.  Infinities become +-top, a NaN stays a NaN.  index (DEVICE, int32) copies rows into the experts'
+ * order on the way; an index outside [0, source_rows) makes a row of zeros.  Any K and any pitch; 16-byte aligned rows
+ * of x and 8-byte aligned rows of q take the fast path.  q and scale must not overlap x.
+ */
+int b200fp8_quantize_rows(int source_rows, int rows, int k, const void* x, int x_dtype, long long ldx, const int* index,
+                          void* q, int q_dtype, long long ldq, float* scale, void* stream);
+
+/*
+ * Products of a matrix of 4-bit weights with a few vectors (the GEMV of weight-only quantised layers):
+ *
+ *     y[m][n] = sum over groups g of scales[n][g] * sum_{k in g} (codes[n][k] - zeros[n][g]) * x[m][k]
+ *
+ * codes: N rows of K/2 bytes, two codes 0..15 to a byte, the even k in the low half; code_ld is the row pitch in BYTES, a
+ * multiple of 16.  scales: N rows of K/group values of scale_dtype (B200FP8_OUT_F32, _BF16 or _F16); zeros: N rows of
+ * K/group bytes (their low four bits), or NULL for 8 throughout.  group is 32, 64 or 128 and divides K.  x: BF16 or FP16,
+ * 16-byte aligned, ldx a multiple of 8; y: x's type or FP32.  Sums are FP32, the products before them exact.  Made for
+ * few vectors: weights are read once per sixteen of them.
+ *
+ * b200fp8_gemv_w4_experts: row r of y takes the weights of expert[r] (DEVICE, int32) and row r / (rows / tokens) of x --
+ * `rows` is a multiple of `tokens`, at most 4096; experts at most 4096.  A row whose expert lies outside [0, experts) is
+ * left as it was.  Strides from one expert's matrix to the next: code_stride in bytes (a multiple of 16), scale_stride
+ * and zero_stride in elements.  Each expert that occurs is read once per eight of its rows.
+ */
+int b200fp8_gemv_w4(int m, int k, int n, int group, const void* codes, long long code_ld, const void* scales, int scale_dtype,
+                    long long scale_ld, const unsigned char* zeros, long long zero_ld, const void* x, int x_dtype, long long ldx,
+                    void* y, int y_dtype, long long ldy, void* stream);
+int b200fp8_gemv_w4_experts(int tokens, int rows, int experts, int k, int n, int group, const void* codes, long long code_ld,
+                            long long code_stride, const void* scales, int scale_dtype, long long scale_ld,
+                            long long scale_stride, const unsigned char* zeros, long long zero_ld, long long zero_stride,
+                            const int* expert, const void* x, int x_dtype, long long ldx, void* y, int y_dtype, long long ldy,
+                            void* stream);
+
+/*
  * N-sharded multi-GPU GEMM with the all-gather of C fused into the kernel's
  * epilogue (no counterpart in the reference, which is single-GPU; it follows
  * the operator above).  Rank `rank` of `world` (<= 8, one process per GPU)

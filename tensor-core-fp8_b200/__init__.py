@@ -5,8 +5,9 @@ The directory name is not an identifier; import it through ``load_package()`` in
 
     from tcfp8_b200 import gemm        # GEMM / GEMM4: the reference's operator surface
     from tcfp8_b200 import shard       # N-sharded multi-GPU plan
+    from tcfp8_b200 import experts     # products grouped by expert, their gradients, 4-bit weights (also names of gemm)
 """
 from . import _cabi  # noqa: F401
-from . import gemm, shard  # noqa: F401
+from . import experts, gemm, shard  # noqa: F401
 
-__all__ = ["gemm", "shard", "_cabi"]
+__all__ = ["gemm", "shard", "experts", "_cabi"]

@@ -35,6 +35,12 @@ DECLARED_SYMBOLS = (
     "b200fp8_gemv_f32",
     "b200fp8_spmm_bell_rowcol_f32",
     "b200fp8_spmv_bell_f32",
+    "b200fp8_gemm_grouped",
+    "b200fp8_gemm_grouped_dgrad",
+    "b200fp8_gemm_grouped_wgrad",
+    "b200fp8_quantize_rows",
+    "b200fp8_gemv_w4",
+    "b200fp8_gemv_w4_experts",
     "b200fp8_gemm_rowcol_f32_allgather",
     "b200fp8_gemm_rowcol_f32_host",
     "b200fp8_host_release",
@@ -116,6 +122,14 @@ def lib() -> ctypes.CDLL:
         L.b200fp8_spmm_bell_rowcol_f32.argtypes = [ci, ci, ci, vp, ci, ll, vp, ci, vp, ci, ll, vp, ll,
                                                    ctypes.POINTER(Options), vp]
         L.b200fp8_spmv_bell_f32.argtypes = [ci, ci, vp, ci, ll, vp, ci, vp, ci, vp, ctypes.POINTER(Options), vp]
+        grouped = [ci, ci, ci, ci, vp, vp, ci, ll, vp, ci, ll]
+        L.b200fp8_gemm_grouped.argtypes = grouped + [ll, vp, ci, ll, ctypes.POINTER(EpilogueDesc), ctypes.POINTER(Options), vp]
+        L.b200fp8_gemm_grouped_dgrad.argtypes = L.b200fp8_gemm_grouped.argtypes
+        L.b200fp8_gemm_grouped_wgrad.argtypes = grouped + [vp, ci, ll, ll, ctypes.POINTER(EpilogueDesc), ctypes.POINTER(Options), vp]
+        L.b200fp8_quantize_rows.argtypes = [ci, ci, ci, vp, ci, ll, vp, vp, ci, ll, vp, vp]
+        L.b200fp8_gemv_w4.argtypes = [ci, ci, ci, ci, vp, ll, vp, ci, ll, vp, ll, vp, ci, ll, vp, ci, ll, vp]
+        L.b200fp8_gemv_w4_experts.argtypes = [ci, ci, ci, ci, ci, ci, vp, ll, ll, vp, ci, ll, ll, vp, ll, ll, vp, vp, ci, ll, vp,
+                                              ci, ll, vp]
         L.b200fp8_gemm_rowcol_f32_host.argtypes = [ci, ci, ci, vp, ci, vp, ci, vp, ci]
         L.b200fp8_gemm_rowcol_f32_noalloc.argtypes = [ci, ci, ci, vp, ci, vp, ci, vp, vp, vp]
         L.b200fp8_fill_normal.argtypes = [vp, ll, ci, ctypes.c_float, ull, ull, vp]

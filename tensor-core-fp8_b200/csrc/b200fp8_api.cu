@@ -16,6 +16,7 @@
 #include "gemm_skinny_streamk_sm100.cuh"
 #include "fill_fp8.cuh"
 #include "l2_sides.cuh"
+#include "host_sm100.h"
 
 namespace b200fp8 {
 namespace {
@@ -496,6 +497,20 @@ cudaError_t ensure(void** p, size_t* have, size_t want) {
 }
 
 }  // namespace
+
+// host_sm100.h: what the library's other translation units share with this one
+cudaError_t host_device(HostDevice* out) {
+    DeviceCtx* ctx = nullptr;
+    const cudaError_t e = get_ctx(&ctx);
+    if (e != cudaSuccess) return e;
+    out->sm_count = ctx->sm_count;
+    out->status = ctx->status;
+    out->encode = g_encode;
+    out->pdl = tune().pdl != 0;
+    return cudaSuccess;
+}
+void count_launch() { ++t_launches; }
+
 }  // namespace b200fp8
 
 using namespace b200fp8;

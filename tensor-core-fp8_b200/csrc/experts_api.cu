@@ -1,0 +1,362 @@
+// Host side of the expert-layer entry points of include/b200fp8.h: argument checks, tensor maps, kernel choice, launch.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <atomic>
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <cstdlib>
+
+#include "../../include/b200fp8.h"
+#include "host_sm100.h"
+#include "gemm_grouped_sm100.cuh"
+#include "gemv_w4_sm100.cuh"
+#include "quantize_rows_sm100.cuh"
+
+namespace b200fp8 {
+namespace {
+
+constexpr int kDevices = 64;
+constexpr int kMaxRows = 1 << 30;
+constexpr int kMaxExperts = 1 << 16;
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+bool fp8(int d) { return d == B200FP8_E4M3 || d == B200FP8_E5M2; }
+
+// dynamic shared memory above the default has to be asked for once per kernel and device
+template <auto kKernel>
+cudaError_t allow_smem(int bytes) {
+    static std::atomic<bool> done[kDevices] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= kDevices) return cudaErrorInvalidDevice;
+    if (done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done[dev].store(true, std::memory_order_relaxed);
+    return e;
+}
+
+template <class... Params, class... Args>
+cudaError_t launch(void (*kernel)(Params...), bool pdl, dim3 grid, int threads, int smem, int cluster, cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = static_cast<unsigned>(cluster);
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
+    if (pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // see griddep_wait in the kernels
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = static_cast<unsigned>(n);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Args&&>(args)...);
+    if (e == cudaSuccess) count_launch();
+    return e;
+}
+
+// A tensor map over `count` matrices of rows x cols elements, row pitch ld, matrix pitch `stride` (elements); the box is
+// one matrix deep.  A map is a pure function of these numbers, so each host thread keeps the last ones it encoded.
+cudaError_t encode_3d(const HostDevice& dev, CUtensorMap* map, CUtensorMapDataType type, int elem, const void* base, uint64_t cols,
+                      uint64_t rows, uint64_t count, uint64_t ld, uint64_t stride, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+    struct Key {
+        const void* base; uint64_t cols, rows, count, ld, stride; uint32_t box_cols, box_rows; int type, swizzle;
+        bool operator==(const Key& o) const {
+            return base == o.base && cols == o.cols && rows == o.rows && count == o.count && ld == o.ld && stride == o.stride &&
+                   box_cols == o.box_cols && box_rows == o.box_rows && type == o.type && swizzle == o.swizzle;
+        }
+    };
+    constexpr int kSlots = 64;
+    struct Cache { Key key[kSlots]; CUtensorMap map[kSlots]; bool used[kSlots]; };
+    static thread_local Cache cache = {};
+    const Key key{base, cols, rows, count, ld, stride, box_cols, box_rows, static_cast<int>(type), static_cast<int>(swizzle)};
+    const uint64_t h = ((reinterpret_cast<uintptr_t>(base) >> 8) + cols * 31 + rows * 131 + box_rows * 7 + box_cols) * 0x9E3779B97F4A7C15ull;
+    const int slot = static_cast<int>(h >> 58);
+    if (cache.used[slot] && cache.key[slot] == key) { *map = cache.map[slot]; return cudaSuccess; }
+    const cuuint64_t dims[3] = {cols, rows, count};
+    const cuuint64_t strides[2] = {ld * elem, stride * elem};
+    const cuuint32_t box[3] = {box_cols, box_rows, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    if (dev.encode(map, type, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return cudaErrorInvalidValue;
+    cache.key[slot] = key; cache.map[slot] = *map; cache.used[slot] = true;
+    return cudaSuccess;
+}
+
+struct GroupedCall {
+    int experts, rows, k, n;
+    const int* ends;
+    const void* a; int a_dtype; long long lda;
+    const void* b; int b_dtype; long long ldb, stride_b;
+    void* d; int d_dtype; long long ldd, stride_d;
+    int max_ctas;
+    Epilogue epi;
+};
+
+template <int MODE, int BN, int STAGES, int CTAS>
+cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStream_t stream) {
+    using L = GroupedSmem<BN, STAGES, CTAS>;
+    cudaError_t e = allow_smem<gemm_fp8_grouped_kernel<MODE, BN, STAGES, CTAS>>(L::kDynamicBytes);
+    if (e != cudaSuccess) return e;
+    constexpr int kTile = kTileM * CTAS;
+    GroupedArgs args{};
+    args.experts = c.experts;
+    args.rows = c.rows;
+    args.cols = MODE == kGroupedForward ? c.n : c.k;
+    args.depth = MODE == kGroupedForward ? c.k : c.n;
+    args.tile_rows_all = c.n;
+    args.ends = c.ends;
+    args.m_tiles = (c.n + kTile - 1) / kTile;                     // wgrad
+    args.n_tiles = (args.cols + BN - 1) / BN;
+    args.group_m = 16;
+    args.idesc = make_idesc_f8(c.a_dtype, c.b_dtype, kTile, BN) | (MODE == kGroupedWgrad ? 1u << 15 : 0u) | (MODE != kGroupedForward ? 1u << 16 : 0u);
+    args.d = c.d; args.ldd = c.ldd; args.stride_d = c.stride_d;
+    args.a = static_cast<const uint8_t*>(c.a); args.lda = c.lda;
+    args.b = static_cast<const uint8_t*>(c.b); args.ldb = c.ldb;
+    args.a_cols = c.n;                                            // wgrad
+    args.status = dev.status;
+    args.epi = c.epi;
+    const int out_bytes = out_dtype_bytes(c.d_dtype);
+    args.tma_store = (c.ldd * out_bytes) % 16 == 0 && (static_cast<long long>(args.cols) * out_bytes) % 16 == 0 &&
+                     (MODE != kGroupedWgrad || (c.stride_d * out_bytes) % 16 == 0) && aligned(c.d, 16);
+
+    GroupedMaps maps;
+    const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const CUtensorMapSwizzle s128 = CU_TENSOR_MAP_SWIZZLE_128B;
+    const uint64_t a_cols = MODE == kGroupedForward ? c.k : c.n;
+    const uint64_t rows = static_cast<uint64_t>(std::max(1, c.rows));
+    for (int i = 0; i < 4; ++i) {
+        if (i < 3 && (MODE == kGroupedWgrad ? i != 1 : CTAS == 2)) { continue; }
+        const uint32_t box = MODE == kGroupedWgrad && i == 1 ? 32 : 16u << i;
+        if ((e = encode_3d(dev, &maps.a[i], u8, 1, c.a, a_cols, rows, 1, c.lda, c.lda * rows, kBlockK, box, s128)) != cudaSuccess) return e;
+    }
+    if (MODE == kGroupedWgrad) {
+        const uint64_t whole = c.ldb * rows;
+        if ((e = encode_3d(dev, &maps.b, u8, 1, c.b, c.k, rows, 1, c.ldb, whole, kBlockK, 128, s128)) != cudaSuccess) return e;
+        if ((e = encode_3d(dev, &maps.b32, u8, 1, c.b, c.k, rows, 1, c.ldb, whole, kBlockK, 32, s128)) != cudaSuccess) return e;
+    } else if ((e = encode_3d(dev, &maps.b, u8, 1, c.b, c.k, c.n, c.experts, c.ldb, c.stride_b, kBlockK, MODE == kGroupedForward ? L::kBRows : 128, s128)) != cudaSuccess) {
+        return e;
+    }
+    for (int i = 0; i < 3; ++i)
+        if (MODE == kGroupedWgrad ? i != 1 : CTAS == 2) maps.a[i] = maps.a[3];    // not used by this kernel
+    if (MODE != kGroupedWgrad) maps.b32 = maps.b;
+    maps.d = maps.b;
+    if (args.tma_store) {
+        const CUtensorMapDataType type = out_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : out_bytes == 1 ? u8
+                                         : c.d_dtype == B200FP8_OUT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+        const CUtensorMapSwizzle sw = out_bytes == 4 ? s128 : out_bytes == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE;
+        const bool wg = MODE == kGroupedWgrad;
+        if ((e = encode_3d(dev, &maps.d, type, out_bytes, c.d, args.cols, wg ? c.n : rows, wg ? c.experts : 1, c.ldd,
+                           wg ? c.stride_d : c.ldd * rows, 32, 32, sw)) != cudaSuccess)
+            return e;
+    }
+    // no more CTAs than there can be tiles: the sizes of the groups are known on the device only
+    const long long groups = MODE == kGroupedWgrad ? c.experts : std::min(c.experts, c.rows);
+    const long long tiles = (MODE == kGroupedWgrad ? groups * args.m_tiles : groups + c.rows / kTile) * args.n_tiles;
+    if (tiles > (1LL << 30)) return cudaErrorInvalidValue;
+    int units = dev.sm_count / CTAS;
+    if (c.max_ctas > 0) units = std::max(1, std::min(units, c.max_ctas / CTAS));
+    units = static_cast<int>(std::min<long long>(units, tiles));
+    return launch(gemm_fp8_grouped_kernel<MODE, BN, STAGES, CTAS>, dev.pdl, dim3(static_cast<unsigned>(units * CTAS), 1, 1), kGemmThreads, L::kDynamicBytes, CTAS, stream, maps, args);
+}
+
+template <int MODE>
+cudaError_t dispatch_grouped(const HostDevice& dev, const GroupedCall& c, int kernel, cudaStream_t stream) {
+    if (kernel == B200FP8_KERNEL_AUTO) {
+        const long long rows = MODE == kGroupedWgrad ? c.n : c.rows / std::max(1, c.experts);   // rows of D per group
+        const long long cols = MODE == kGroupedForward ? c.n : c.k;
+        const long long tiles = static_cast<long long>(c.experts) * ((rows + 127) / 128) * ((cols + 255) / 256);
+        kernel = rows >= 192 && cols > 128 && tiles >= 2LL * dev.sm_count ? B200FP8_KERNEL_PAIR_N256
+                 : tiles >= dev.sm_count && rows > 64                     ? B200FP8_KERNEL_CTA1_N256
+                                                                          : B200FP8_KERNEL_CTA1_N128;
+    }
+    switch (kernel) {
+        case B200FP8_KERNEL_PAIR_N256: return launch_grouped<MODE, 256, 6, 2>(dev, c, stream);
+        case B200FP8_KERNEL_CTA1_N256: return launch_grouped<MODE, 256, 4, 1>(dev, c, stream);
+        case B200FP8_KERNEL_CTA1_N128: return launch_grouped<MODE, 128, 6, 1>(dev, c, stream);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+// What the three products check alike.  `a_cols` / `d_cols`: extents along the contiguous index of A and D.
+cudaError_t grouped(int mode, int experts, int rows, int k, int n, const int* ends, const void* a, int a_dtype, long long lda, const void* b,
+                    int b_dtype, long long ldb, long long stride_b, void* d, int d_dtype, long long ldd, long long stride_d,
+                    const b200fp8_epilogue* ep, const b200fp8_options* options, cudaStream_t stream) {
+    if (options && options->struct_bytes != static_cast<int>(sizeof(b200fp8_options))) return cudaErrorInvalidValue;
+    if (options && (options->depth != 0 || options->split_k != 0 || options->max_ctas < 0)) return cudaErrorInvalidValue;
+    if (ep && ep->struct_bytes != static_cast<int>(sizeof(b200fp8_epilogue)) && ep->struct_bytes != B200FP8_EPILOGUE_V1_BYTES) return cudaErrorInvalidValue;
+    const bool extended = ep && ep->struct_bytes == static_cast<int>(sizeof(b200fp8_epilogue));
+    if (extended && (ep->activation < B200FP8_ACT_NONE || ep->activation > B200FP8_ACT_GELU_TANH)) return cudaErrorInvalidValue;
+    if (experts < 0 || rows < 0 || k <= 0 || n <= 0 || experts > kMaxExperts || rows > kMaxRows || !fp8(a_dtype) || !fp8(b_dtype)) return cudaErrorInvalidValue;
+    if (d_dtype < B200FP8_OUT_F32 || d_dtype > B200FP8_OUT_E5M2) return cudaErrorInvalidValue;
+    const bool wgrad = mode == kGroupedWgrad;
+    if (ep && ep->bias && (ep->bias_dtype < B200FP8_OUT_F32 || ep->bias_dtype > B200FP8_OUT_F16 || !aligned(ep->bias, out_dtype_bytes(ep->bias_dtype)))) return cudaErrorInvalidValue;
+    if (ep && !aligned(ep->amax_d, 4)) return cudaErrorInvalidValue;
+    // a bias, an activation or a scale of one row has no place in a sum over the rows
+    if (wgrad && ep && (ep->bias || (extended && (ep->activation || ep->a_row_scale || ep->b_row_scale)))) return cudaErrorInvalidValue;
+    const long long a_cols = mode == kGroupedForward ? k : n, d_cols = mode == kGroupedForward ? n : k;
+    // the contiguous extents that TMA and the tensor core walk: whole 16-byte pieces
+    if (k % 16 || (mode != kGroupedForward && n % 16) || lda % 16 || ldb % 16) return cudaErrorInvalidValue;
+    if (lda < a_cols || ldb < k || ldd < d_cols) return cudaErrorInvalidValue;
+    constexpr long long kMostStride = 1LL << 39;                  // a tensor map's strides are below 2^40 bytes
+    if (lda > kMostStride || ldb > kMostStride || ldd > kMostStride / 4) return cudaErrorInvalidValue;
+    if (!wgrad && (stride_b % 16 || (experts > 1 && stride_b < static_cast<long long>(n - 1) * ldb + k) || stride_b > kMostStride)) return cudaErrorInvalidValue;
+    if (wgrad && ((experts > 1 && stride_d < static_cast<long long>(n - 1) * ldd + k) || stride_d > kMostStride / 4)) return cudaErrorInvalidValue;
+    const int out_bytes = out_dtype_bytes(d_dtype);
+    const bool nothing = experts == 0 || (rows == 0 && !wgrad);
+    if (!nothing) {
+        if (!ends || !aligned(ends, 4) || !d || !aligned(d, out_bytes)) return cudaErrorInvalidValue;
+        if ((rows > 0 && !a) || ((!wgrad || rows > 0) && !b) || !aligned(a, 16) || !aligned(b, 16)) return cudaErrorInvalidValue;
+        // a matrix of all rows has to be addressable as one tensor map
+        if (static_cast<double>(rows) * static_cast<double>(lda) > 5e11 || static_cast<double>(rows) * static_cast<double>(wgrad ? ldb : ldd) * out_bytes > 1e12) return cudaErrorInvalidValue;
+    }
+    const int kernel = options ? options->kernel : B200FP8_KERNEL_AUTO;
+    if (kernel != B200FP8_KERNEL_AUTO && kernel != B200FP8_KERNEL_PAIR_N256 && kernel != B200FP8_KERNEL_CTA1_N256 && kernel != B200FP8_KERNEL_CTA1_N128)
+        return cudaErrorInvalidValue;
+    HostDevice dev;
+    cudaError_t e = host_device(&dev);
+    if (e != cudaSuccess) return e;
+    if (ep && ep->amax_d && (e = cudaMemsetAsync(ep->amax_d, 0, sizeof(float), stream)) != cudaSuccess) return e;
+    if (nothing) return cudaSuccess;
+
+    GroupedCall c{};
+    c.experts = experts; c.rows = rows; c.k = k; c.n = n; c.ends = ends;
+    c.a = a; c.a_dtype = a_dtype; c.lda = lda;
+    c.b = b; c.b_dtype = b_dtype; c.ldb = ldb; c.stride_b = experts > 1 ? stride_b : static_cast<long long>(n) * ldb;
+    c.d = d; c.d_dtype = d_dtype; c.ldd = ldd; c.stride_d = experts > 1 ? stride_d : static_cast<long long>(n) * ldd;
+    if (rows == 0) {
+        // wgrad without any row: every group is empty and nothing of A or B is read; the maps need some valid base
+        c.a = c.b = reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(d) & ~static_cast<uintptr_t>(15));
+    }
+    c.max_ctas = options ? options->max_ctas : 0;
+    c.epi.active = 1;
+    c.epi.out_dtype = d_dtype;
+    c.epi.alpha = 1.0f;
+    if (ep) {
+        c.epi.alpha = ep->alpha; c.epi.beta = ep->beta;
+        c.epi.a_scale = ep->a_scale; c.epi.b_scale = ep->b_scale; c.epi.d_scale = ep->d_scale;
+        c.epi.amax = ep->amax_d;
+        c.epi.bias = ep->bias; c.epi.bias_dtype = ep->bias_dtype;
+        if (extended) { c.epi.activation = ep->activation; c.epi.a_row_scale = ep->a_row_scale; c.epi.b_row_scale = ep->b_row_scale; }
+    }
+    switch (mode) {
+        case kGroupedForward: return dispatch_grouped<kGroupedForward>(dev, c, kernel, stream);
+        case kGroupedDgrad: return dispatch_grouped<kGroupedDgrad>(dev, c, kernel, stream);
+        default: return dispatch_grouped<kGroupedWgrad>(dev, c, kernel, stream);
+    }
+}
+
+cudaError_t w4(const W4Args& args, int x_dtype, cudaStream_t stream) {
+    const bool by_expert = args.expert != nullptr;
+    if (args.n < 0 || args.k < 0 || args.m < 0) return cudaErrorInvalidValue;
+    if (x_dtype != B200FP8_OUT_BF16 && x_dtype != B200FP8_OUT_F16) return cudaErrorInvalidValue;
+    if (args.y_dtype != x_dtype && args.y_dtype != B200FP8_OUT_F32) return cudaErrorInvalidValue;
+    if (args.scale_dtype < B200FP8_OUT_F32 || args.scale_dtype > B200FP8_OUT_F16) return cudaErrorInvalidValue;
+    if ((args.group != 32 && args.group != 64 && args.group != 128) || args.k % args.group) return cudaErrorInvalidValue;
+    if (args.code_ld < args.k / 2 || args.code_ld % 16 || args.scale_ld < args.k / args.group || args.ldx < args.k || args.ldx % 8 || args.ldy < args.n)
+        return cudaErrorInvalidValue;
+    if (args.zeros && args.zero_ld < args.k / args.group) return cudaErrorInvalidValue;
+    if (args.m == 0 || args.n == 0) return cudaSuccess;
+    const int y_bytes = out_dtype_bytes(args.y_dtype);
+    if (!args.y || !aligned(args.y, y_bytes)) return cudaErrorInvalidValue;
+    if (args.k > 0 && (!args.codes || !args.scales || !args.x || !aligned(args.codes, 16) || !aligned(args.x, 16) ||
+                       !aligned(args.scales, out_dtype_bytes(args.scale_dtype))))
+        return cudaErrorInvalidValue;
+    HostDevice dev;
+    const cudaError_t e = host_device(&dev);
+    if (e != cudaSuccess) return e;
+    const long long blocks = (args.n + 16LL * kW4SimpleWarps - 1) / (16 * kW4SimpleWarps);
+    const dim3 grid(static_cast<unsigned>(blocks), by_expert ? 1u : static_cast<unsigned>(std::min((args.m + 7) / 8, 65535)),
+                    by_expert ? static_cast<unsigned>(std::min(args.experts, args.m)) : 1u);
+    auto kernel = x_dtype == B200FP8_OUT_BF16 ? gemv_w4_simple_kernel<true> : gemv_w4_simple_kernel<false>;
+    return launch(kernel, dev.pdl, grid, 32 * kW4SimpleWarps, 0, 1, stream, args);
+}
+
+}  // namespace
+}  // namespace b200fp8
+
+using namespace b200fp8;
+
+extern "C" {
+
+int b200fp8_gemm_grouped(int experts, int rows, int k, int n, const int* ends, const void* a, int a_dtype, long long lda, const void* b,
+                         int b_dtype, long long ldb, long long stride_b, void* d, int d_dtype, long long ldd, const b200fp8_epilogue* epilogue,
+                         const b200fp8_options* options, void* stream) {
+    return grouped(kGroupedForward, experts, rows, k, n, ends, a, a_dtype, lda, b, b_dtype, ldb, stride_b, d, d_dtype, ldd, 0, epilogue, options,
+                   static_cast<cudaStream_t>(stream));
+}
+
+int b200fp8_gemm_grouped_dgrad(int experts, int rows, int k, int n, const int* ends, const void* a, int a_dtype, long long lda, const void* b,
+                               int b_dtype, long long ldb, long long stride_b, void* d, int d_dtype, long long ldd,
+                               const b200fp8_epilogue* epilogue, const b200fp8_options* options, void* stream) {
+    return grouped(kGroupedDgrad, experts, rows, k, n, ends, a, a_dtype, lda, b, b_dtype, ldb, stride_b, d, d_dtype, ldd, 0, epilogue, options,
+                   static_cast<cudaStream_t>(stream));
+}
+
+int b200fp8_gemm_grouped_wgrad(int experts, int rows, int k, int n, const int* ends, const void* a, int a_dtype, long long lda, const void* b,
+                               int b_dtype, long long ldb, void* d, int d_dtype, long long ldd, long long stride_d,
+                               const b200fp8_epilogue* epilogue, const b200fp8_options* options, void* stream) {
+    return grouped(kGroupedWgrad, experts, rows, k, n, ends, a, a_dtype, lda, b, b_dtype, ldb, 0, d, d_dtype, ldd, stride_d, epilogue, options,
+                   static_cast<cudaStream_t>(stream));
+}
+
+int b200fp8_quantize_rows(int source_rows, int rows, int k, const void* x, int x_dtype, long long ldx, const int* index, void* q, int q_dtype,
+                          long long ldq, float* scale, void* stream) {
+    if (source_rows < 0 || rows < 0 || k < 0 || !fp8(q_dtype) || (x_dtype != B200FP8_OUT_BF16 && x_dtype != B200FP8_OUT_F16)) return cudaErrorInvalidValue;
+    if (ldx < k || ldq < k || (!index && rows > source_rows)) return cudaErrorInvalidValue;
+    if (rows == 0) return cudaSuccess;
+    if (!scale || !aligned(scale, 4) || !aligned(index, 4) || !aligned(x, 2)) return cudaErrorInvalidValue;
+    if (k > 0 && (!q || (!x && source_rows > 0))) return cudaErrorInvalidValue;
+    HostDevice dev;
+    const cudaError_t e = host_device(&dev);
+    if (e != cudaSuccess) return e;
+    QuantizeArgs args{static_cast<const uint16_t*>(x), ldx, source_rows, index, rows, k, static_cast<uint8_t*>(q), ldq, scale, q_dtype};
+    auto kernel = x_dtype == B200FP8_OUT_BF16 ? quantize_rows_any_kernel<true> : quantize_rows_any_kernel<false>;
+    return launch(kernel, dev.pdl, dim3(static_cast<unsigned>(rows), 1, 1), 256, 0, 1, static_cast<cudaStream_t>(stream), args);
+}
+
+int b200fp8_gemv_w4(int m, int k, int n, int group, const void* codes, long long code_ld, const void* scales, int scale_dtype,
+                    long long scale_ld, const unsigned char* zeros, long long zero_ld, const void* x, int x_dtype, long long ldx, void* y,
+                    int y_dtype, long long ldy, void* stream) {
+    W4Args args{};
+    args.codes = static_cast<const uint8_t*>(codes); args.code_ld = code_ld;
+    args.scales = scales; args.scale_dtype = scale_dtype; args.scale_ld = scale_ld;
+    args.zeros = zeros; args.zero_ld = zero_ld;
+    args.x = static_cast<const uint16_t*>(x); args.ldx = ldx;
+    args.y = y; args.y_dtype = y_dtype; args.ldy = ldy;
+    args.m = m; args.n = n; args.k = k; args.group = group;
+    return w4(args, x_dtype, static_cast<cudaStream_t>(stream));
+}
+
+int b200fp8_gemv_w4_experts(int tokens, int rows, int experts, int k, int n, int group, const void* codes, long long code_ld,
+                            long long code_stride, const void* scales, int scale_dtype, long long scale_ld, long long scale_stride,
+                            const unsigned char* zeros, long long zero_ld, long long zero_stride, const int* expert, const void* x,
+                            int x_dtype, long long ldx, void* y, int y_dtype, long long ldy, void* stream) {
+    if (tokens < 0 || rows < 0 || experts < 0 || rows > kW4MostRows || experts > kW4MostExperts) return cudaErrorInvalidValue;
+    if (rows > 0 && (tokens == 0 || rows % tokens || !expert || !aligned(expert, 4))) return cudaErrorInvalidValue;
+    if (experts > 1 && k > 0 && n > 0 &&
+        (code_stride % 16 || code_stride < (n - 1) * code_ld + k / 2 || scale_stride < (n - 1) * scale_ld + k / std::max(group, 1) ||
+         (zeros && zero_stride < (n - 1) * zero_ld + k / std::max(group, 1))))
+        return cudaErrorInvalidValue;
+    W4Args args{};
+    args.codes = static_cast<const uint8_t*>(codes); args.code_ld = code_ld; args.code_stride = code_stride;
+    args.scales = scales; args.scale_dtype = scale_dtype; args.scale_ld = scale_ld; args.scale_stride = scale_stride;
+    args.zeros = zeros; args.zero_ld = zero_ld; args.zero_stride = zero_stride;
+    args.x = static_cast<const uint16_t*>(x); args.ldx = ldx;
+    args.y = y; args.y_dtype = y_dtype; args.ldy = ldy;
+    args.m = experts == 0 ? 0 : rows; args.n = n; args.k = k; args.group = group;
+    args.expert = expert; args.experts = experts;
+    args.rows_per_x = tokens > 0 ? std::max(1, rows / tokens) : 1;
+    return w4(args, x_dtype, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
