@@ -123,9 +123,9 @@ def lib() -> ctypes.CDLL:
                                                    ctypes.POINTER(Options), vp]
         L.b200fp8_spmv_bell_f32.argtypes = [ci, ci, vp, ci, ll, vp, ci, vp, ci, vp, ctypes.POINTER(Options), vp]
         grouped = [ci, ci, ci, ci, vp, vp, ci, ll, vp, ci, ll]
-        L.b200fp8_gemm_grouped.argtypes = grouped + [ll, vp, ci, ll, ctypes.POINTER(EpilogueDesc), ctypes.POINTER(Options), vp]
+        L.b200fp8_gemm_grouped.argtypes = grouped + [ll, vp, ci, ll, vp, ctypes.POINTER(Options), vp]      # the epilogue as packed bytes
         L.b200fp8_gemm_grouped_dgrad.argtypes = L.b200fp8_gemm_grouped.argtypes
-        L.b200fp8_gemm_grouped_wgrad.argtypes = grouped + [vp, ci, ll, ll, ctypes.POINTER(EpilogueDesc), ctypes.POINTER(Options), vp]
+        L.b200fp8_gemm_grouped_wgrad.argtypes = grouped + [vp, ci, ll, ll, vp, ctypes.POINTER(Options), vp]
         L.b200fp8_quantize_rows.argtypes = [ci, ci, ci, vp, ci, ll, vp, vp, ci, ll, vp, vp]
         L.b200fp8_gemv_w4.argtypes = [ci, ci, ci, ci, vp, ll, vp, ci, ll, vp, ll, vp, ci, ll, vp, ci, ll, vp]
         L.b200fp8_gemv_w4_experts.argtypes = [ci, ci, ci, ci, ci, ci, vp, ll, ll, vp, ci, ll, ll, vp, ll, ll, vp, vp, ci, ll, vp,

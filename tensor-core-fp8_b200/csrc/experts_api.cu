@@ -5,7 +5,6 @@
 #include <algorithm>
 #include <climits>
 #include <cstdint>
-#include <cstdlib>
 
 #include "../../include/b200fp8.h"
 #include "host_sm100.h"
@@ -255,9 +254,61 @@ cudaError_t grouped(int mode, int experts, int rows, int k, int n, const int* en
     }
 }
 
+template <bool BF16, int G, int NT, bool WIDE>
+cudaError_t launch_w4(const HostDevice& dev, W4Args args, cudaStream_t stream) {
+    using L = W4Smem<NT>;
+    const int list_bytes = args.expert ? 4 * args.m : 0;
+    const int bytes = L::kFixedBytes + list_bytes;
+    cudaError_t e = allow_smem<gemv_w4_kernel<BF16, G, NT, WIDE>>(L::kFixedBytes + 4 * kW4MostRows);
+    if (e != cudaSuccess) return e;
+    const int slots = args.expert ? std::min(args.experts, args.m) : 1;
+    const int tiles = (args.n + kW4TileRows - 1) / kW4TileRows;
+    if (tiles > 65535) return cudaErrorInvalidValue;             // N beyond 8 million
+    args.k_blocks = (args.k + kW4BoxK - 1) / kW4BoxK;
+    args.status = dev.status;
+    args.k_unit = G == 128 ? 2 : 1;
+    const int units = (args.k_blocks + args.k_unit - 1) / args.k_unit;
+    const int scale_bytes = out_dtype_bytes(args.scale_dtype);
+    args.vector_scales = args.scale_ld % 4 == 0 && args.scale_stride % 4 == 0 && aligned(args.scales, 4 * scale_bytes);
+    args.vector_zeros = args.zero_ld % 4 == 0 && args.zero_stride % 4 == 0 && aligned(args.zeros, 4);
+    // K is parted until three CTAs share two SMs: every part costs its CTA a start and a meeting with the others (about 5 us in
+    // all), so more of them lose (8192 x 8192, one vector: 25.3 / 16.5 / 15.0 / 21.9 us in 1 / 2 / 4 / 8 parts; 28672 x 8192, eight
+    // vectors: 47 / 53 / 55 / 74)
+    int splits = 1;
+    while (splits < 8 && 2 * splits <= units && static_cast<long long>(slots) * tiles * splits < (dev.sm_count * 3) / 2) splits *= 2;
+    args.splits = splits;
+    CUtensorMap map;
+    const uint64_t experts = args.expert ? args.experts : 1;
+    if ((e = encode_3d(dev, &map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, args.codes, args.k / 2, args.n, experts, args.code_ld,
+                       experts > 1 ? args.code_stride : args.code_ld * static_cast<long long>(args.n), kW4BoxBytes, 16,
+                       CU_TENSOR_MAP_SWIZZLE_128B)) != cudaSuccess)
+        return e;
+    return launch(gemv_w4_kernel<BF16, G, NT, WIDE>, dev.pdl, dim3(splits, static_cast<unsigned>(tiles), static_cast<unsigned>(slots)), kW4Threads, bytes, splits,
+                  stream, map, args);
+}
+
+template <bool BF16, int G>
+cudaError_t launch_w4_group(const HostDevice& dev, const W4Args& args, cudaStream_t stream) {
+    // by expert most experts have at most eight rows (a decode step); where they have more on average, and for more than
+    // eight dense vectors, sixteen share a pass over the weights
+    const bool two = args.expert ? args.m > 8 * args.experts : args.m > 8;
+    const bool wide = args.scale_dtype == B200FP8_OUT_F32;
+    if (two) return wide ? launch_w4<BF16, G, 2, true>(dev, args, stream) : launch_w4<BF16, G, 2, false>(dev, args, stream);
+    return wide ? launch_w4<BF16, G, 1, true>(dev, args, stream) : launch_w4<BF16, G, 1, false>(dev, args, stream);
+}
+
+template <bool BF16>
+cudaError_t launch_w4_type(const HostDevice& dev, const W4Args& args, cudaStream_t stream) {
+    switch (args.group) {
+        case 32: return launch_w4_group<BF16, 32>(dev, args, stream);
+        case 64: return launch_w4_group<BF16, 64>(dev, args, stream);
+        default: return launch_w4_group<BF16, 128>(dev, args, stream);
+    }
+}
+
 cudaError_t w4(const W4Args& args, int x_dtype, cudaStream_t stream) {
     const bool by_expert = args.expert != nullptr;
-    if (args.n < 0 || args.k < 0 || args.m < 0) return cudaErrorInvalidValue;
+    if (args.n < 0 || args.k <= 0 || args.m < 0 || args.code_ld > (1LL << 39) || args.code_stride > (1LL << 39)) return cudaErrorInvalidValue;
     if (x_dtype != B200FP8_OUT_BF16 && x_dtype != B200FP8_OUT_F16) return cudaErrorInvalidValue;
     if (args.y_dtype != x_dtype && args.y_dtype != B200FP8_OUT_F32) return cudaErrorInvalidValue;
     if (args.scale_dtype < B200FP8_OUT_F32 || args.scale_dtype > B200FP8_OUT_F16) return cudaErrorInvalidValue;
@@ -274,11 +325,8 @@ cudaError_t w4(const W4Args& args, int x_dtype, cudaStream_t stream) {
     HostDevice dev;
     const cudaError_t e = host_device(&dev);
     if (e != cudaSuccess) return e;
-    const long long blocks = (args.n + 16LL * kW4SimpleWarps - 1) / (16 * kW4SimpleWarps);
-    const dim3 grid(static_cast<unsigned>(blocks), by_expert ? 1u : static_cast<unsigned>(std::min((args.m + 7) / 8, 65535)),
-                    by_expert ? static_cast<unsigned>(std::min(args.experts, args.m)) : 1u);
-    auto kernel = x_dtype == B200FP8_OUT_BF16 ? gemv_w4_simple_kernel<true> : gemv_w4_simple_kernel<false>;
-    return launch(kernel, dev.pdl, grid, 32 * kW4SimpleWarps, 0, 1, stream, args);
+    if (x_dtype == B200FP8_OUT_BF16) return launch_w4_type<true>(dev, args, stream);
+    return launch_w4_type<false>(dev, args, stream);
 }
 
 }  // namespace

@@ -5,14 +5,31 @@
 // c: codes 0..15, two to a byte, the even k in the low half; one scale (and, optionally, one zero point; 8 without) per row
 // and group of 32, 64 or 128 k.  x is BF16 or FP16; y has its type or FP32.
 //
-// The arithmetic is exact up to the FP32 sums: c - z is a whole number of at most 15 and so exact in either 16-bit type,
-// the tensor core (m16n8k16) multiplies exactly and adds in FP32, and the scale multiplies a group's FP32 sum, not the
-// rounded weight.  Rows of the weights are the M index of the instruction and the vectors its N index, so up to eight
-// vectors cost what one costs; the order of k inside an instruction is free, and is chosen so that a lane's eight codes
-// are one aligned 32-bit word: (k, k + 4) share a 16-bit pair, which is what a mask and a shift take out of the word.
+// The arithmetic is exact up to the FP32 sums: c - z is a whole number of at most 15 and so exact in FP16 (over 1024), the tensor core
+// (m16n8k16) multiplies exactly and adds in FP32, and the scale multiplies a group's FP32 sum, not the rounded weight.
+// BF16 vectors are brought to FP16 by a power of two per vector and 256 of K, so that the largest of these lies in
+// [2^14, 2^15): eight significant bits fit eleven, and what falls below FP16's smallest step is less than 2^-39 of the
+// largest, far below the FP32 sums' rounding.  (FP16 takes one shift per eight codes where BF16 takes three.)
+// Rows of the weights are the M index of the instruction and the vectors its N index, so up to eight vectors cost what
+// one costs; the order of k inside an instruction is free, and is chosen so that a lane's eight codes are one aligned
+// 32-bit word: (k, k + 4) share a 16-bit pair, which is what a mask takes out of the word.
 //
-// By expert: row r of y takes the weights of expert[r] and row r / (rows / tokens) of x.  A block finds the experts that
-// occur by itself (a bit set over `expert`), so each of them is read once whatever the routing, with no second launch.
+// Bound by the weights' bytes from HBM: 13 weights per nanosecond at the measured rate, 47 per SM and clock, of which the
+// instructions above take 9 per eight (a shift, four masks, four subtractions) plus the tensor core's one.  So the
+// kernel is about bytes in flight and few instructions:
+//
+//   * a CTA owns 128 rows of weights, 16 for each of eight warps, and a part of K; every warp streams the codes of its rows
+//     by TMA through a ring of its own ([16 rows][128 bytes] boxes under the 128-byte swizzle) and refills a slot as soon as
+//     it has read it: no producer warp and no waiting for other warps; two CTAs per SM;
+//   * its part of x lies in shared memory, in the order in which the lanes want it;
+//   * the parts of K of one 128-row tile form a thread-block cluster and add their FP32 sums through distributed shared
+//     memory in the order of K: no scratch in HBM, no atomics, one launch.
+//
+// By expert: row r of y takes the weights of expert[r] and row r / (rows / tokens) of x.  A block finds its rows by itself
+// in one pass over `expert`: with fewer rows than experts block z stands for row z and works if that row is the
+// first of its expert, else block z stands for expert z.  Each expert's weights are read once per eight of its rows.
+//
+// Waits on mbarriers are bounded as in the other kernels: a wait that runs out sets the status word and ends the kernel.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -33,127 +50,441 @@ struct W4Args {
     int m, n, k, group;
     const int* expert;     // by expert: the expert of each row of y, else nullptr
     int experts, rows_per_x;
+    int k_blocks;          // ceil(k / 256)
+    int k_unit;            // parts of K begin at multiples of this many blocks
+    int vector_scales, vector_zeros;   // four scales (zero points) of a row can be loaded at once
+    int splits;            // parts of K = CTAs of a cluster
+    int* status;
 };
 
 constexpr int kW4MostRows = 4096;        // rows of y of one call by expert: their list is held in shared memory
 constexpr int kW4MostExperts = 4096;
+constexpr int kW4TileRows = 128;
+constexpr int kW4Warps = 8;
+constexpr int kW4Threads = 32 * kW4Warps;
+constexpr int kW4Stages = 4;
+constexpr int kW4BoxBytes = 128;         // of codes per row and ring slot: 256 of K
+constexpr int kW4BoxK = 2 * kW4BoxBytes;
+constexpr int kW4SlotBytes = 16 * kW4BoxBytes;
+constexpr int kStatusW4Timeout = 106;
 
-template <bool BF16>
+// c = a b (FIRST) or c += a b
+template <bool FIRST>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (BF16)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if constexpr (FIRST)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
     else
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Codes j and j + 4 of a word as a pair of 16-bit floats minus the zero point, exactly.  A code placed in the low bits of
-// the number 128 (BF16: eight significant bits) or 1024 (FP16: eleven) adds itself to that number.
+// A row's zero point z as what its codes lose: -z / 1024 in both halves (FP16).  `zeros` holds four zero points, one to a byte.
+__device__ __forceinline__ __half2 w4_minus(uint32_t zeros, uint32_t place) {
+    const uint32_t z = __byte_perm(zeros, 0u, 0x4040u + place * 0x0101u);     // z * 2^-24: a subnormal number's bits count upwards
+    return __hmul2(*reinterpret_cast<const __half2*>(&z), __half2half2(__ushort_as_half(0xF400)));   // * -2^14
+}
+// The eight codes of a word as four pairs (j, j + 4) of FP16 numbers (c - z) / 1024, exactly.  A code in the four lowest bits
+// of a half is the subnormal number c * 2^-24, one in the next four bits c * 2^-20, so that a mask alone makes it a
+// number and one fused multiply-add scales it and takes the zero point off.
+__device__ __forceinline__ void w4_unpack(uint32_t word, __half2 minus, uint32_t (&a)[4]) {
+    const uint32_t next = word >> 8;
+    const uint32_t v[4] = {word & 0x000F000Fu, word & 0x00F000F0u, next & 0x000F000Fu, next & 0x00F000F0u};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&v[i]), __half2half2(__ushort_as_half(i & 1 ? 0x6400 : 0x7400)), minus);
+        a[i] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+
+// Eight consecutive x of one vector as FP16 pairs (0, 4), (1, 5), (2, 6), (3, 7).  BF16: a whole warp calls it with the
+// pieces of 256 consecutive k and gets the power of two `back` that undoes the scaling.
 template <bool BF16>
-__device__ __forceinline__ uint32_t w4_pair(uint32_t word, int j, uint32_t minus) {
-    const uint32_t v = ((word >> (4 * j)) & 0x000F000Fu) | (BF16 ? 0x43004300u : 0x64006400u);
-    if constexpr (BF16) {
-        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&minus));
-        return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ uint4 w4_vector_piece(uint4 v, float& back) {
+    if constexpr (!BF16) {
+        back = 1.0f;
+        return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
     } else {
-        const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&minus));
-        return *reinterpret_cast<const uint32_t*>(&r);
-    }
-}
-// the number 128 + z (1024 + z) in both halves
-template <bool BF16>
-__device__ __forceinline__ uint32_t w4_minus(uint32_t z) { return ((z & 15u) | (BF16 ? 0x4300u : 0x6400u)) * 0x00010001u; }
-
-__device__ __forceinline__ float w4_scale(const W4Args& args, long long at) { return load_out(args.scales, at, args.scale_dtype); }
-
-// Rows of y that this block computes together: the `slot`-th expert that occurs, in ascending order, and its rows.
-// Returns the expert, or -1 when fewer experts occur.  All threads of the block call it.
-__device__ __forceinline__ int w4_find_rows(const W4Args& args, int slot, uint32_t* bits, int* list, int* count) {
-    for (int i = threadIdx.x; i < (args.experts + 31) / 32; i += blockDim.x) bits[i] = 0u;
-    __syncthreads();
-    for (int r = threadIdx.x; r < args.m; r += blockDim.x) {
-        const int e = args.expert[r];
-        if (e >= 0 && e < args.experts) atomicOr(bits + (e >> 5), 1u << (e & 31));
-    }
-    __syncthreads();
-    int found = -1, left = slot;
-    for (int i = 0; i < (args.experts + 31) / 32; ++i) {
-        const int here = __popc(bits[i]);
-        if (left < here) { found = 32 * i + static_cast<int>(__fns(bits[i], 0, left + 1)); break; }
-        left -= here;
-    }
-    if (found < 0) return -1;
-    if (threadIdx.x < 32) {                                    // one warp keeps the list in ascending order
-        int n = 0;
-        for (int r0 = 0; r0 < args.m; r0 += 32) {
-            const int r = r0 + static_cast<int>(threadIdx.x);
-            const bool mine = r < args.m && args.expert[r] == found;
-            const uint32_t who = __ballot_sync(0xffffffffu, mine);
-            if (mine) list[n + __popc(who & ((1u << threadIdx.x) - 1u))] = r;
-            n += __popc(who);
-        }
-        if (threadIdx.x == 0) *count = n;
-    }
-    __syncthreads();
-    return found;
-}
-
-constexpr int kW4SimpleWarps = 4;
-
-// The simple form: a warp per 16 rows of the weights and eight vectors, straight from global memory.
-template <bool BF16>
-__global__ void __launch_bounds__(32 * kW4SimpleWarps) gemv_w4_simple_kernel(const W4Args args) {
-    __shared__ uint32_t bits[kW4MostExperts / 32];
-    __shared__ int list[kW4MostRows];
-    __shared__ int count;
-    ptx::griddep_wait();
-    ptx::griddep_launch_dependents();
-    int e = 0, have = args.m;
-    if (args.expert) {
-        e = w4_find_rows(args, blockIdx.z, bits, list, &count);
-        if (e < 0) return;
-        have = count;
-    }
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int n0 = (blockIdx.x * kW4SimpleWarps + (threadIdx.x >> 5)) * 16;
-    if (n0 >= args.n) return;
-    const int lo = min(n0 + g, args.n - 1), hi = min(n0 + g + 8, args.n - 1);
-    const uint8_t* codes = args.codes + e * args.code_stride;
-    const uint8_t *clo = codes + lo * args.code_ld, *chi = codes + hi * args.code_ld;
-    const long long slo = e * args.scale_stride + lo * args.scale_ld, shi = e * args.scale_stride + hi * args.scale_ld;
-    const long long zlo = e * args.zero_stride + lo * args.zero_ld, zhi = e * args.zero_stride + hi * args.zero_ld;
-    for (int m0 = blockIdx.y * 8; m0 < have; m0 += 8 * gridDim.y) {
-        const int col = m0 + g;
-        const int row = col < have ? (args.expert ? list[col] / args.rows_per_x : col) : -1;
-        const uint16_t* x = args.x + (row < 0 ? 0 : row) * args.ldx;
-        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k0 = 0; k0 < args.k; k0 += args.group) {
-            const int at = k0 / args.group;
-            uint32_t mlo = w4_minus<BF16>(8), mhi = mlo;
-            if (args.zeros) { mlo = w4_minus<BF16>(args.zeros[zlo + at]); mhi = w4_minus<BF16>(args.zeros[zhi + at]); }
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int k = k0 + t * 8; k < k0 + args.group; k += 32) {
-                const uint32_t wlo = *reinterpret_cast<const uint32_t*>(clo + k / 2), whi = *reinterpret_cast<const uint32_t*>(chi + k / 2);
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (row >= 0) v = *reinterpret_cast<const uint4*>(x + k);
-                const uint32_t b0 = __byte_perm(v.x, v.z, 0x5410), b1 = __byte_perm(v.x, v.z, 0x7632);
-                const uint32_t b2 = __byte_perm(v.y, v.w, 0x5410), b3 = __byte_perm(v.y, v.w, 0x7632);
-                mma_16816<BF16>(c, w4_pair<BF16>(wlo, 0, mlo), w4_pair<BF16>(whi, 0, mhi), w4_pair<BF16>(wlo, 1, mlo), w4_pair<BF16>(whi, 1, mhi), b0, b1);
-                mma_16816<BF16>(c, w4_pair<BF16>(wlo, 2, mlo), w4_pair<BF16>(whi, 2, mhi), w4_pair<BF16>(wlo, 3, mlo), w4_pair<BF16>(whi, 3, mhi), b2, b3);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t most = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = max(most, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (most >= 0x7F80u) {                                   // an infinity or a NaN: the largest finite number counts
+            most = 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t a = w[i] & 0x7FFFu, b = (w[i] >> 16) & 0x7FFFu;
+                most = max(most, max(a < 0x7F80u ? a : 0u, b < 0x7F80u ? b : 0u));
             }
-            const float sl = w4_scale(args, slo + at), sh = w4_scale(args, shi + at);
-            y[0] = fmaf(sl, c[0], y[0]);
-            y[1] = fmaf(sl, c[1], y[1]);
-            y[2] = fmaf(sh, c[2], y[2]);
-            y[3] = fmaf(sh, c[3], y[3]);
+            most = __reduce_max_sync(0xffffffffu, most);
         }
+        const int up = min(126, 141 - static_cast<int>(most >> 7));          // 14 - (exponent - 127)
+        const float forth = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+        back = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+        uint32_t r[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int c = m0 + 2 * t + (i & 1), n = n0 + g + (i >> 1) * 8;
-            if (c < have && n < args.n) store_out(args.y, static_cast<long long>(args.expert ? list[c] : c) * args.ldy + n, y[i], args.y_dtype);
+            const uint32_t lo = w[i >> 1], hi = w[2 + (i >> 1)];             // numbers i and i + 4
+            const float a = __uint_as_float(i & 1 ? lo & 0xFFFF0000u : lo << 16), b = __uint_as_float(i & 1 ? hi & 0xFFFF0000u : hi << 16);
+            const __half2 h = __floats2half2_rn(a * forth, b * forth);
+            r[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        return make_uint4(r[0], r[1], r[2], r[3]);
+    }
+}
+
+// Four scales in a row from group `at` on (a multiple of four) as they are stored: FP32, or 16-bit ones two to a word.
+template <bool WIDE> struct W4Scales;
+template <> struct W4Scales<true> {
+    uint4 v;
+    __device__ __forceinline__ void load(const W4Args& args, long long row, int at, int groups) {
+        const uint32_t* p = static_cast<const uint32_t*>(args.scales) + row + at;
+        if (args.vector_scales && at + 4 <= groups) { v = __ldg(reinterpret_cast<const uint4*>(p)); return; }
+        v = make_uint4(0u, 0u, 0u, 0u);
+        if (at < groups) v.x = __ldg(p);
+        if (at + 1 < groups) v.y = __ldg(p + 1);
+        if (at + 2 < groups) v.z = __ldg(p + 2);
+        if (at + 3 < groups) v.w = __ldg(p + 3);
+    }
+    // scales 2 pair and 2 pair + 1 of lane `from`
+    __device__ __forceinline__ float2 pair(int p, int from, int) const {
+        return make_float2(__uint_as_float(__shfl_sync(0xffffffffu, p ? v.z : v.x, from)), __uint_as_float(__shfl_sync(0xffffffffu, p ? v.w : v.y, from)));
+    }
+};
+template <> struct W4Scales<false> {
+    uint2 v;
+    __device__ __forceinline__ void load(const W4Args& args, long long row, int at, int groups) {
+        const uint16_t* p = static_cast<const uint16_t*>(args.scales) + row + at;
+        if (args.vector_scales && at + 4 <= groups) { v = __ldg(reinterpret_cast<const uint2*>(p)); return; }
+        v = make_uint2(0u, 0u);
+        if (at < groups) v.x = __ldg(p);
+        if (at + 1 < groups) v.x |= static_cast<uint32_t>(__ldg(p + 1)) << 16;
+        if (at + 2 < groups) v.y = __ldg(p + 2);
+        if (at + 3 < groups) v.y |= static_cast<uint32_t>(__ldg(p + 3)) << 16;
+    }
+    __device__ __forceinline__ float2 pair(int p, int from, int dtype) const {
+        const uint32_t w = __shfl_sync(0xffffffffu, p ? v.y : v.x, from);
+        return dtype == 1 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&w));
+    }
+};
+// Four zero points in a row, one to a byte.
+__device__ __forceinline__ uint32_t w4_zeros(const W4Args& args, const uint8_t* row, int at, int groups) {
+    if (args.vector_zeros && at + 4 <= groups) return __ldg(reinterpret_cast<const uint32_t*>(row + at));
+    uint32_t v = 0u;
+    if (at < groups) v = __ldg(row + at);
+    if (at + 1 < groups) v |= static_cast<uint32_t>(__ldg(row + at + 1)) << 8;
+    if (at + 2 < groups) v |= static_cast<uint32_t>(__ldg(row + at + 2)) << 16;
+    if (at + 3 < groups) v |= static_cast<uint32_t>(__ldg(row + at + 3)) << 24;
+    return v;
+}
+
+template <int NT>
+struct W4Smem {
+    static constexpr int kXK = 2048 / NT;                        // of K whose x is staged at a time
+    static constexpr int kXPitch = kXK * 2 + 64;                 // bytes; two vectors' lanes meet different banks
+    static constexpr int kPartPitch = kW4TileRows + 4;           // floats
+    static constexpr int kXOff = kW4Warps * kW4Stages * kW4SlotBytes;
+    static constexpr int kBackOff = kXOff + 8 * NT * kXPitch;     // powers of two [blocks][vectors]
+    static constexpr int kPartOff = kBackOff + kXK / kW4BoxK * 8 * NT * 4;
+    static constexpr int kBarOff = kPartOff + 8 * NT * kPartPitch * 4;   // full[warp][stage], ready, done
+    static constexpr int kMiscOff = kBarOff + 8 * (kW4Warps * kW4Stages + 2);   // abort flag
+    static constexpr int kListOff = kMiscOff + 16;                       // by expert: rows of y (the call's row count)
+    static constexpr int kFixedBytes = kListOff + 1024;                  // with the slack for 1024-byte alignment
+};
+
+// Rows of y for this block by expert, in ascending order into `list` (written by warp 0; every warp learns expert and
+// count).  Returns the expert, -1 when the block has none.
+__device__ __forceinline__ int w4_find_rows(const W4Args& args, int slot, int* list, bool write, int& count) {
+    const int lane = threadIdx.x & 31;
+    const bool by_row = args.m < args.experts;
+    const int e = by_row ? __ldg(args.expert + slot) : slot;
+    count = 0;
+    constexpr int kAtOnce = 8;                                   // loads in flight: one round trip for up to 256 rows
+    for (int r0 = 0; r0 < args.m; r0 += 32 * kAtOnce) {
+        int id[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) id[i] = r0 + 32 * i + lane < args.m ? __ldg(args.expert + r0 + 32 * i + lane) : -1;
+        if (e < 0 || e >= args.experts) return -1;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const uint32_t who = __ballot_sync(0xffffffffu, id[i] == e);
+            if (by_row && count == 0 && who != 0 && r0 + 32 * i + __ffs(who) - 1 < slot) return -1;   // an earlier row stands for it
+            if (write && id[i] == e) list[count + __popc(who & ((1u << lane) - 1u))] = r0 + 32 * i + lane;
+            count += __popc(who);
         }
     }
+    return count > 0 ? e : -1;
+}
+
+template <bool BF16, int G, int NT, bool WIDE>                     // WIDE: FP32 scales
+__global__ void __launch_bounds__(kW4Threads, 2)
+gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)      // codes [experts][N][K/2], box 128 bytes x 16 rows
+{
+    using L = W4Smem<NT>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
+    uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_addr(smem_raw));
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+    const int lane = threadIdx.x & 31;
+    const uint32_t bar_full = smem_base + L::kBarOff + warp * 8 * kW4Stages;     // this warp's
+    const uint32_t bar_ready = smem_base + L::kBarOff + 8 * kW4Warps * kW4Stages, bar_done = bar_ready + 8;
+    const uint32_t ring = smem_base + warp * kW4Stages * kW4SlotBytes;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + L::kMiscOff);
+    int* list = reinterpret_cast<int*>(smem_gen + L::kListOff);
+    const bool clustered = args.splits > 1;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < kW4Warps * kW4Stages; ++s) ptx::mbar_init(smem_base + L::kBarOff + 8 * s, 1);
+        ptx::mbar_init(bar_ready, args.splits);
+        ptx::mbar_init(bar_done, args.splits);
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&tmap);
+    }
+    __syncthreads();
+    if (clustered) ptx::cluster_arrive();                        // the wait comes before the first remote arrival
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+
+    int e = 0, have = args.m;
+    if (args.expert) e = w4_find_rows(args, blockIdx.z, list, warp == 0, have);
+    if (e < 0) {                                                 // the same for all CTAs of the cluster
+        if (clustered) ptx::cluster_wait();
+        return;
+    }
+    const int n0 = blockIdx.y * kW4TileRows;
+    const int split = blockIdx.x;
+    const int units = (args.k_blocks + args.k_unit - 1) / args.k_unit;
+    const int kb0 = static_cast<int>(static_cast<long long>(units) * split / args.splits) * args.k_unit;
+    const int kb1 = min(args.k_blocks, static_cast<int>(static_cast<long long>(units) * (split + 1) / args.splits) * args.k_unit);
+    const int batches = (have + 8 * NT - 1) / (8 * NT);
+    int to_fill = batches * (kb1 - kb0);                         // blocks of this warp's rows still to be asked for
+    int fill_kb = kb0;
+    // one lane: the next block into slot s
+    auto fill = [&](int s) {
+        if (ptx::elect_one()) {
+            ptx::mbar_arrive_expect_tx(bar_full + 8 * s, kW4SlotBytes);
+            ptx::tma_load_3d(ring + s * kW4SlotBytes, &tmap, fill_kb * kW4BoxBytes, n0 + warp * 16, e, bar_full + 8 * s);
+        }
+        --to_fill;
+        if (++fill_kb == kb1) fill_kb = kb0;
+    };
+    for (int s = 0; s < kW4Stages && to_fill > 0; ++s) fill(s);
+
+    constexpr int kGroups = kW4BoxK / G;                         // groups per ring slot: 2, 4 or 8
+    constexpr int kWords = 8 / kGroups;                          // 32-bit words of codes per lane, row and group
+    const int g = lane >> 2, t = lane & 3;
+    // Which of the warp's rows stands at place g of the instruction is free; these orders keep the reads of codes free of
+    // bank conflicts: the rows that one pass of a shared-memory read takes (two of 64 bytes, four of 32, eight of 16)
+    // differ in the bits of the swizzle that the bytes of one row do not.
+    const int row_of = G == 128 ? (g >> 1) | ((g & 1) << 2) : G == 64 ? (2 * g) % 8 + g / 4 : g;
+    const int r_lo = warp * 16 + row_of, r_hi = r_lo + 8;        // this lane's two rows of the tile
+    // 16-byte chunk ^ row mod 8, the same for both rows: the bits that depend on the lane; the others are xor'ed in
+    const uint32_t lane_at = row_of * kW4BoxBytes + ((G == 128 ? t ^ row_of : G == 64 ? (t >> 1) ^ row_of : row_of) << 4) + (G == 64 ? (t & 1) * 8 : G == 32 ? t * 4 : 0);
+    const uint32_t x_lane = smem_base + L::kXOff + g * L::kXPitch + t * 16;
+    const int groups = args.k / G;
+    const long long n_lo = min(n0 + r_lo, args.n - 1), n_hi = min(n0 + r_hi, args.n - 1);
+    const long long s_lo = e * args.scale_stride + n_lo * args.scale_ld, s_hi = e * args.scale_stride + n_hi * args.scale_ld;
+    const uint8_t* z_lo = args.zeros ? args.zeros + e * args.zero_stride + n_lo * args.zero_ld : nullptr;
+    const uint8_t* z_hi = args.zeros ? args.zeros + e * args.zero_stride + n_hi * args.zero_ld : nullptr;
+    // Scales and zero points: the four lanes of a row hold those of 16 groups in a row, four each (a whole sector of
+    // 16-bit scales), fetched 16 groups ahead and handed round by shuffles.  Fetched one by one, just before their use,
+    // they bound the kernel: every load missed to HBM and kept the load unit busy with eight rows' lines.
+    W4Scales<WIDE> s_now[2], s_next[2];
+    uint32_t z_now[2], z_next[2] = {0x08080808u, 0x08080808u};
+    const int g_first = kb0 * kGroups;
+    auto fetch = [&](int window) {
+        const int at = g_first + 16 * window + 4 * t;
+        s_next[0].load(args, s_lo, at, groups);
+        s_next[1].load(args, s_hi, at, groups);
+        if (z_lo) { z_next[0] = w4_zeros(args, z_lo, at, groups) & 0x0F0F0F0Fu; z_next[1] = w4_zeros(args, z_hi, at, groups) & 0x0F0F0F0Fu; }
+    };
+    int s = 0;
+    uint32_t ph = 0, round = 0;
+    bool ok = true;                                              // after a wait that ran out: no more waits, no more copies, and on to the end
+    for (int b = 0; b < batches; ++b) {
+        const int m0 = b * 8 * NT, cols = min(8 * NT, have - m0);
+        float y[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) y[j][0] = y[j][1] = y[j][2] = y[j][3] = 0.0f;
+        fetch(0);
+        for (int kc = kb0; kc < kb1; kc += L::kXK / kW4BoxK) {
+            const int kend = min(kb1, kc + L::kXK / kW4BoxK);
+            // x of these k-blocks: a warp takes one block, a lane eight of its k, for every vector (four loads in flight), and
+            // places them so that the four lanes of a row of fragments read 64 bytes.  Vectors that are not there are zeros,
+            // written once per batch.
+            __syncthreads();
+            constexpr int kBlocks = L::kXK / kW4BoxK;             // a chunk's: eight, or four
+            const int block = warp % kBlocks;
+            const int limit = kc == kb0 ? 8 * NT : cols;
+            if (kc + block < kend || kc == kb0) {
+                const int k = (kc + block) * kW4BoxK + lane * 8;
+                const int rest = lane % (4 * kWords), pos = lane - rest + rest % kWords * 4 + rest / kWords;   // within the group
+                const uint32_t to = smem_base + L::kXOff + (block * (kW4BoxK / 8) + pos) * 16;
+                for (int c0 = warp / kBlocks * 4; c0 < limit; c0 += 4 * NT) {
+                    uint4 v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v[i] = make_uint4(0u, 0u, 0u, 0u);
+                        if (c0 + i < cols && k < args.k && kc + block < kend) {
+                            const int row = args.expert ? list[m0 + c0 + i] / args.rows_per_x : m0 + c0 + i;
+                            v[i] = __ldg(reinterpret_cast<const uint4*>(args.x + row * args.ldx + k));
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (c0 + i >= limit) break;
+                        float back;
+                        const uint4 h = w4_vector_piece<BF16>(v[i], back);
+                        ptx::st_shared_v4(to + (c0 + i) * L::kXPitch, h.x, h.y, h.z, h.w);
+                        if (BF16 && lane == 0) reinterpret_cast<float*>(smem_gen + L::kBackOff)[block * 8 * NT + c0 + i] = back;
+                    }
+                }
+            }
+            __syncthreads();
+            for (int kb = kc; kb < kend; ++kb) {
+                const int rel = (kb - kb0) * kGroups & 15;        // first group of the slot within its 16
+                if (rel == 0) {
+                    s_now[0] = s_next[0]; s_now[1] = s_next[1];
+                    z_now[0] = z_next[0]; z_now[1] = z_next[1];
+                    if (kb + 16 / kGroups < kb1) fetch(((kb - kb0) * kGroups >> 4) + 1);
+                }
+                if (ok && !wait_bounded(bar_full + 8 * s, ph, abort_flag, false)) {
+                    record_failure(args.status, abort_flag, kStatusW4Timeout);
+                    ok = false;
+                }
+                __syncwarp();
+                const uint32_t at = ring + s * kW4SlotBytes + lane_at;
+                uint32_t lo[8], hi[8];
+                if constexpr (G == 128) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint4 a = ptx::ld_shared_v4(at ^ (i << 6)), c = ptx::ld_shared_v4((at ^ (i << 6)) + 8 * kW4BoxBytes);
+                        lo[4 * i] = a.x; lo[4 * i + 1] = a.y; lo[4 * i + 2] = a.z; lo[4 * i + 3] = a.w;
+                        hi[4 * i] = c.x; hi[4 * i + 1] = c.y; hi[4 * i + 2] = c.z; hi[4 * i + 3] = c.w;
+                    }
+                } else if constexpr (G == 64) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(lo[2 * i]), "=r"(lo[2 * i + 1]) : "r"(at ^ (i << 5)) : "memory");
+                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2+1024];" : "=r"(hi[2 * i]), "=r"(hi[2 * i + 1]) : "r"(at ^ (i << 5)) : "memory");
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        lo[i] = ptx::ld_shared_u32(at ^ (i << 4));
+                        hi[i] = ptx::ld_shared_u32((at ^ (i << 4)) + 8 * kW4BoxBytes);
+                    }
+                }
+                // The slot may be refilled once these reads are done.  The refill is a write of another proxy (TMA), and nothing
+                // but a proxy fence orders it behind them: without it a warp read codes of the ring's next turn.
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (ok && to_fill > 0) fill(s);
+                __syncwarp();
+                if (++s == kW4Stages) { s = 0; ph ^= 1u; }
+                const uint32_t x_at = x_lane + (kb - kc) * (2 * kW4BoxK);
+                float2 two_lo, two_hi;
+                uint32_t zl = 0x08080808u, zh = 0x08080808u;
+                float ys[NT][4];                                  // this slot's sums, in the scaling of its x
+#pragma unroll
+                for (int j = 0; j < NT; ++j) ys[j][0] = ys[j][1] = ys[j][2] = ys[j][3] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kGroups; ++i) {
+                    // group rel + i of the 16: lane (rel + i) / 4 of the row holds it, at place (rel + i) % 4
+                    const int from = (lane & ~3) | ((rel + i) >> 2);
+                    if ((i & 1) == 0) {
+                        const int p = ((kGroups == 2 ? rel : i) >> 1) & 1;
+                        two_lo = s_now[0].pair(p, from, args.scale_dtype);
+                        two_hi = s_now[1].pair(p, from, args.scale_dtype);
+                    }
+                    const float cs_lo = i & 1 ? two_lo.y : two_lo.x, cs_hi = i & 1 ? two_hi.y : two_hi.x;
+                    if (z_lo && (i & 3) == 0) {                  // four groups' zero points of this lane's rows
+                        zl = __shfl_sync(0xffffffffu, z_now[0], from);
+                        zh = __shfl_sync(0xffffffffu, z_now[1], from);
+                    }
+                    const uint32_t place = kGroups == 2 ? (rel + i) & 3 : i & 3;
+                    const __half2 m_lo = w4_minus(zl, place), m_hi = w4_minus(zh, place);
+                    float c[NT][4];
+#pragma unroll
+                    for (int w = i * kWords; w < (i + 1) * kWords; ++w) {
+                        uint32_t a[4], b[4];
+                        w4_unpack(lo[w], m_lo, a);
+                        w4_unpack(hi[w], m_hi, b);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            const uint4 v = ptx::ld_shared_v4(x_at + 8 * j * L::kXPitch + w * 64);
+                            if (w == i * kWords) mma_16816<true>(c[j], a[0], b[0], a[1], b[1], v.x, v.y);
+                            else mma_16816<false>(c[j], a[0], b[0], a[1], b[1], v.x, v.y);
+                            mma_16816<false>(c[j], a[2], b[2], a[3], b[3], v.z, v.w);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        float* sum = BF16 ? ys[j] : y[j];
+                        sum[0] = fmaf(cs_lo, c[j][0], sum[0]);
+                        sum[1] = fmaf(cs_lo, c[j][1], sum[1]);
+                        sum[2] = fmaf(cs_hi, c[j][2], sum[2]);
+                        sum[3] = fmaf(cs_hi, c[j][3], sum[3]);
+                    }
+                }
+                if (BF16) {
+                    const float* back = reinterpret_cast<const float*>(smem_gen + L::kBackOff) + (kb - kc) * 8 * NT + 2 * t;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const float2 p = *reinterpret_cast<const float2*>(back + 8 * j);
+                        y[j][0] = fmaf(p.x, ys[j][0], y[j][0]);
+                        y[j][1] = fmaf(p.y, ys[j][1], y[j][1]);
+                        y[j][2] = fmaf(p.x, ys[j][2], y[j][2]);
+                        y[j][3] = fmaf(p.y, ys[j][3], y[j][3]);
+                    }
+                }
+            }
+        }
+        // the parts of K meet: every CTA lays its sums out in its shared memory and adds a share of the rows
+        float* part = reinterpret_cast<float*>(smem_gen + L::kPartOff);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[(8 * j + 2 * t + (i & 1)) * L::kPartPitch + (i >> 1 ? r_hi : r_lo)] = 1024.0f * y[j][i];   // see w4_unpack
+        if (clustered) {
+            if (b == 0) ptx::cluster_wait();                     // every CTA of the cluster has its barriers
+            __syncthreads();
+            if (threadIdx.x < args.splits) ptx::mbar_arrive_cluster(ptx::mapa(bar_ready, threadIdx.x));
+            if (ok && !wait_bounded(bar_ready, round & 1u, abort_flag, true)) { record_failure(args.status, abort_flag, kStatusW4Timeout); ok = false; }
+        } else {
+            __syncthreads();
+        }
+        const int share = kW4TileRows / args.splits;
+        const uint32_t part_addr = smem_base + L::kPartOff;
+        for (int i = threadIdx.x; i < cols * share && ok; i += 32 * kW4Warps) {
+            const int c = i / share, r = split * share + i - c * share;
+            float sum = 0.0f;
+            if (clustered) {
+                const uint32_t at = part_addr + (c * L::kPartPitch + r) * 4;
+                for (int p = 0; p < args.splits; ++p) sum += __uint_as_float(ptx::ld_shared_cluster_u32(ptx::mapa(at, p)));
+            } else {
+                sum = part[c * L::kPartPitch + r];
+            }
+            if (n0 + r < args.n) store_out(args.y, static_cast<long long>(args.expert ? list[m0 + c] : m0 + c) * args.ldy + n0 + r, sum, args.y_dtype);
+        }
+        __syncthreads();
+        if (clustered && b + 1 < batches) {                      // the next batch may overwrite the sums once all have read them
+            if (threadIdx.x < args.splits) ptx::mbar_arrive_cluster(ptx::mapa(bar_done, threadIdx.x));
+            if (ok && !wait_bounded(bar_done, round & 1u, abort_flag, true)) { record_failure(args.status, abort_flag, kStatusW4Timeout); ok = false; }
+        }
+        ++round;
+    }
+    if (!ok && lane == 0) {                                       // leave no copy in flight into this CTA's shared memory
+        for (int i = 0; i < kW4Stages; ++i) {
+            const uint64_t t0 = ptx::globaltimer_ns();
+            while (!ptx::mbar_try_wait(bar_full + 8 * s, ph) && ptx::globaltimer_ns() - t0 < kWaitLimitNs / 8) {}
+            if (++s == kW4Stages) { s = 0; ph ^= 1u; }
+        }
+    }
+    __syncwarp();
+    if (clustered) { ptx::cluster_arrive(); ptx::cluster_wait(); }   // no CTA leaves while another reads its shared memory
 }
 
 }  // namespace b200fp8

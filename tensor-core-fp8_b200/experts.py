@@ -5,10 +5,14 @@ Layouts and formats are those of the dense operator (GEMM/include/gemm.cuh:12-55
 the contraction index.  The reference has one weight matrix per product and no weights below eight bits, so these
 operators have no counterpart there.  Everything is checked here before the call (the C ABI sees only pointers); calls
 are enqueued on the current stream of the tensors' device.  Outputs must not share memory with inputs.
+
+A decode step's kernels run for a few microseconds, so the checks are written to cost little: each asks a tensor once for
+what it needs and looks closer only where that is not the plain contiguous case.
 """
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -19,57 +23,64 @@ F8 = {torch.float8_e4m3fn: E4M3, torch.float8_e5m2: E5M2}
 OUT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3, torch.float8_e5m2: 4}
 HALF = {torch.bfloat16: 1, torch.float16: 2}
 WIDE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-F32, INT32, U8 = (torch.float32,), (torch.int32,), (torch.uint8,)
-_EPILOGUE_BYTES, _OPTIONS_BYTES = ctypes.sizeof(_cabi.EpilogueDesc), ctypes.sizeof(Options)
+F32, INT32, U8 = {torch.float32: 0}, {torch.int32: 0}, {torch.uint8: 0}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3}
 
+_EPILOGUE = struct.Struct("@iffPPPPPiiPP")          # b200fp8_epilogue of include/b200fp8.h
+_EPILOGUE_BYTES = ctypes.sizeof(_cabi.EpilogueDesc)
+assert _EPILOGUE.size == _EPILOGUE_BYTES
+_functions: dict = {}
 
-def _matrix(name: str, t: torch.Tensor, dtypes, shape) -> int:
-    """Checks type, shape and layout of a matrix (or of one per expert) and returns its row pitch in elements."""
+
+def _pitch(name: str, t: torch.Tensor, dtypes, cols: int) -> int:
+    """Type and layout of a matrix of `cols` columns (or of one per expert); returns its row pitch in elements."""
+    if t.dtype in dtypes and t.is_contiguous():
+        return cols
     if t.dtype not in dtypes:
         raise TypeError(f"{name} has type {t.dtype}, expected one of {', '.join(str(d) for d in dtypes)}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    cols, rows = shape[-1], shape[-2]
-    if t.is_contiguous():
-        return cols
+    rows = t.shape[-2]
     if cols > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name}: the last dimension must be contiguous, got strides {t.stride()}")
     pitch = t.stride(-2) if rows > 1 else cols
     if pitch < cols:
         raise ValueError(f"{name}: rows overlap (pitch {pitch}, {cols} columns)")
-    if len(shape) == 3 and shape[0] > 1 and t.stride(0) < (rows - 1) * pitch + cols:
+    if t.dim() == 3 and t.shape[0] > 1 and t.stride(0) < (rows - 1) * pitch + cols:
         raise ValueError(f"{name}: matrices overlap (pitch {t.stride(0)})")
     return pitch
 
 
-def _stride(t: torch.Tensor, pitch: int) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * pitch
+def _stride(t: torch.Tensor, matrices: int, rows: int, pitch: int) -> int:
+    """Pitch from one expert's matrix to the next."""
+    return t.stride()[0] if matrices > 1 else rows * pitch
 
 
-def _vector(name: str, t: torch.Tensor, dtypes, shape) -> None:
+def _vector(name: str, t: torch.Tensor, dtypes, *shape: int) -> int:
+    """Checks a contiguous tensor of this shape and returns its address."""
     if t.dtype not in dtypes or t.shape != shape or not t.is_contiguous():
         raise TypeError(f"{name} must be contiguous {list(shape)} of {', '.join(str(d) for d in dtypes)}, got {t.dtype} {list(t.shape)}")
+    return t.data_ptr()
 
 
-def _device(first: torch.Tensor, *others) -> torch.device:
-    device = first.device
-    if device.type != "cuda":
+def _device(first: torch.Tensor, *others) -> int:
+    device = first.get_device()
+    if device < 0:
         raise ValueError("the operators take CUDA tensors (device pointers)")
     for t in others:
-        if t is not None and t.device != device:
-            raise ValueError(f"all tensors must live on one device, got {device} and {t.device}")
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"all tensors must live on one device, got {first.device} and {t.device}")
     return device
 
 
-def _call(device: torch.device, what: str, function, *args) -> None:
+def _call(device: int, what: str, *args) -> None:
     """Enqueues the call on the device's current stream, with that device current."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        code = function(*args, stream)
+    function = _functions.get(what)
+    if function is None:
+        function = _functions[what] = getattr(_cabi.lib(), "b200fp8_" + what)
+    if torch.cuda.current_device() == device:
+        code = function(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            code = function(*args, stream)
+            code = function(*args, torch._C._cuda_getCurrentRawStream(device))
     if code:
         _cabi.check(code, what)
 
@@ -83,59 +94,58 @@ def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, *, rows
     """
     if x.dim() != 2 or q.dim() != 2:
         raise ValueError("x and q are matrices")
-    count, k = q.shape
-    if x.shape[1] != k or (rows is None and count != x.shape[0]):
+    source, k = x.shape
+    count, columns = q.shape
+    if columns != k or (rows is None and count != source):
         raise ValueError(f"q must have x's rows and columns (rows as `rows` says), got {list(q.shape)} for {list(x.shape)}")
-    ldx = _matrix("x", x, HALF, x.shape)
-    ldq = _matrix("q", q, F8, q.shape)
-    _vector("scale", scale, F32, (count,))
-    if rows is not None:
-        _vector("rows", rows, INT32, (count,))
-    device = _device(q, x, scale, rows)
-    _call(device, "quantize_rows", _cabi.lib().b200fp8_quantize_rows, x.shape[0], count, k, x.data_ptr(), HALF[x.dtype], ldx,
-          None if rows is None else rows.data_ptr(), q.data_ptr(), F8[q.dtype], ldq, scale.data_ptr())
+    ldx, ldq = _pitch("x", x, HALF, k), _pitch("q", q, F8, k)
+    at = _vector("scale", scale, F32, count)
+    index = None if rows is None else _vector("rows", rows, INT32, count)
+    _call(_device(q, x, scale, rows), "quantize_rows", source, count, k, x.data_ptr(), HALF[x.dtype], ldx, index, q.data_ptr(),
+          F8[q.dtype], ldq, at)
     return q, scale
 
 
-def _grouped(what, a, b, d, ends, cols, *, alpha, beta, a_scale, b_scale, d_scale, amax_d, bias=None, a_row_scale=None,
-             b_row_scale=None, activation=0, kernel=KERNEL_AUTO, max_ctas=0):
+def _one(name: str, t) -> int:
+    """Address of an optional one-element float32 tensor."""
+    if t is None:
+        return 0
+    if t.dtype != torch.float32 or t.numel() != 1:
+        raise TypeError(f"{name} is a one-element float32 tensor")
+    return t.data_ptr()
+
+
+def _grouped(what, a, b, d, ends, experts, rows, n, k, a_cols, cols, alpha, beta, a_scale, b_scale, d_scale, amax_d, bias, a_row_scale, b_row_scale,
+             activation, kernel, max_ctas):
     """The part of the three products that comes behind their shape checks: epilogue, options, call."""
-    experts = ends.shape[0]
-    _vector("ends", ends, INT32, (experts,))
-    for name, t in (("a_scale", a_scale), ("b_scale", b_scale), ("d_scale", d_scale), ("amax_d", amax_d)):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != 1):
-            raise TypeError(f"{name} is a one-element float32 tensor")
-    if bias is not None:
-        _vector("bias", bias, WIDE, (experts, cols))
-    if a_row_scale is not None:
-        _vector("a_row_scale", a_row_scale, F32, (a.shape[0],))
-    if b_row_scale is not None:
-        _vector("b_row_scale", b_row_scale, F32, (experts, cols))
-    if isinstance(activation, str):
+    first_row = _vector("ends", ends, INT32, experts)
+    if activation.__class__ is str:
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation is one of {sorted(ACTIVATIONS)}")
         activation = ACTIVATIONS[activation]
-    elif activation not in ACTIVATIONS.values():
+    elif activation not in (0, 1, 2, 3):
         raise ValueError("unknown activation")
+    ep = _EPILOGUE.pack(_EPILOGUE_BYTES, alpha, beta, _one("a_scale", a_scale), _one("b_scale", b_scale), _one("d_scale", d_scale),
+                        _one("amax_d", amax_d), 0 if bias is None else _vector("bias", bias, WIDE, experts, cols),
+                        0 if bias is None else WIDE[bias.dtype], activation,
+                        0 if a_row_scale is None else _vector("a_row_scale", a_row_scale, F32, rows),
+                        0 if b_row_scale is None else _vector("b_row_scale", b_row_scale, F32, experts, cols))
+    opt = None if kernel == KERNEL_AUTO and not max_ctas else ctypes.byref(Options(ctypes.sizeof(Options), 0, kernel, 0, max_ctas))
+    lda, ldb, ldd = _pitch("a", a, F8, a_cols), _pitch("b", b, F8, k), _pitch("d", d, OUT, cols)
     device = _device(d, a, b, ends, a_scale, b_scale, d_scale, amax_d, bias, a_row_scale, b_row_scale)
-    ptr = lambda t: None if t is None else t.data_ptr()
-    ep = _cabi.EpilogueDesc(_EPILOGUE_BYTES, alpha, beta, ptr(a_scale), ptr(b_scale), ptr(d_scale), ptr(amax_d), ptr(bias),
-                            0 if bias is None else WIDE[bias.dtype], activation, ptr(a_row_scale), ptr(b_row_scale))
-    opt = None if kernel == KERNEL_AUTO and not max_ctas else ctypes.byref(Options(_OPTIONS_BYTES, 0, kernel, 0, max_ctas))
-    lda = _matrix("a", a, F8, a.shape)
-    ldb = _matrix("b", b, F8, b.shape)
-    ldd = _matrix("d", d, OUT, d.shape)
-    if what == "gemm_grouped_wgrad":
-        tail = (ldb, d.data_ptr(), OUT[d.dtype], ldd, _stride(d, ldd))
-        n, k = d.shape[1:]
-    else:
-        tail = (ldb, _stride(b, ldb), d.data_ptr(), OUT[d.dtype], ldd)
-        n, k = b.shape[1:]
     if experts == 0 or n == 0 or k == 0:
         return d
-    _call(device, what, getattr(_cabi.lib(), "b200fp8_" + what), experts, a.shape[0], k, n, ends.data_ptr(), a.data_ptr(), F8[a.dtype], lda,
-          b.data_ptr(), F8[b.dtype], *tail, ctypes.byref(ep), opt)
+    if what == "gemm_grouped_wgrad":
+        _call(device, what, experts, rows, k, n, first_row, a.data_ptr(), F8[a.dtype], lda, b.data_ptr(), F8[b.dtype], ldb, d.data_ptr(),
+              OUT[d.dtype], ldd, _stride(d, experts, n, ldd), ep, opt)
+    else:
+        _call(device, what, experts, rows, k, n, first_row, a.data_ptr(), F8[a.dtype], lda, b.data_ptr(), F8[b.dtype], ldb,
+              _stride(b, experts, n, ldb), d.data_ptr(), OUT[d.dtype], ldd, ep, opt)
     return d
+
+
+def _shapes(a, b, d, ends, wanted):
+    raise ValueError(f"{wanted}, ends [experts]: got {list(a.shape)}, {list(b.shape)}, {list(d.shape)}, {list(ends.shape)}")
 
 
 def gemm_grouped(a: torch.Tensor, b: torch.Tensor, d: torch.Tensor, ends: torch.Tensor, *, alpha: float = 1.0, beta: float = 0.0,
@@ -149,13 +159,14 @@ def gemm_grouped(a: torch.Tensor, b: torch.Tensor, d: torch.Tensor, ends: torch.
     act(alpha * a_scale * b_scale * a_row_scale[r] * b_row_scale[e][n] * sum + beta * d + bias[e][n]), times d_scale.
     K must be a multiple of 16.  Returns d.
     """
-    if a.dim() != 2 or b.dim() != 3 or d.dim() != 2 or ends.dim() != 1 or b.shape[0] != ends.shape[0] or b.shape[2] != a.shape[1] \
-            or d.shape != (a.shape[0], b.shape[1]):
-        raise ValueError(f"a [rows][K], b [experts][N][K], d [rows][N], ends [experts]: got {list(a.shape)}, {list(b.shape)}, "
-                         f"{list(d.shape)}, {list(ends.shape)}")
-    return _grouped("gemm_grouped", a, b, d, ends, b.shape[1], alpha=alpha, beta=beta, a_scale=a_scale, b_scale=b_scale, d_scale=d_scale,
-                    amax_d=amax_d, bias=bias, a_row_scale=a_row_scale, b_row_scale=b_row_scale, activation=activation, kernel=kernel,
-                    max_ctas=max_ctas)
+    if a.dim() != 2 or b.dim() != 3 or d.dim() != 2 or ends.dim() != 1:
+        _shapes(a, b, d, ends, "a [rows][K], b [experts][N][K], d [rows][N]")
+    rows, k = a.shape
+    experts, n, depth = b.shape
+    if depth != k or d.shape != (rows, n) or ends.shape[0] != experts:
+        _shapes(a, b, d, ends, "a [rows][K], b [experts][N][K], d [rows][N]")
+    return _grouped("gemm_grouped", a, b, d, ends, experts, rows, n, k, k, n, alpha, beta, a_scale, b_scale, d_scale, amax_d, bias, a_row_scale,
+                    b_row_scale, activation, kernel, max_ctas)
 
 
 def gemm_grouped_dgrad(a: torch.Tensor, b: torch.Tensor, d: torch.Tensor, ends: torch.Tensor, *, alpha: float = 1.0, beta: float = 0.0,
@@ -164,13 +175,14 @@ def gemm_grouped_dgrad(a: torch.Tensor, b: torch.Tensor, d: torch.Tensor, ends: 
     """The gradient of ``gemm_grouped`` by its rows: d[r] = ep(b[e]^T a[r]), with a [rows][N] the gradient of the output, the
     weights b [experts][N][K] as the forward pass has them, and d [rows][K].  Epilogue as there, vectors of [experts][K].
     N and K must be multiples of 16."""
-    if a.dim() != 2 or b.dim() != 3 or d.dim() != 2 or ends.dim() != 1 or b.shape[0] != ends.shape[0] or b.shape[1] != a.shape[1] \
-            or d.shape != (a.shape[0], b.shape[2]):
-        raise ValueError(f"a [rows][N], b [experts][N][K], d [rows][K], ends [experts]: got {list(a.shape)}, {list(b.shape)}, "
-                         f"{list(d.shape)}, {list(ends.shape)}")
-    return _grouped("gemm_grouped_dgrad", a, b, d, ends, b.shape[2], alpha=alpha, beta=beta, a_scale=a_scale, b_scale=b_scale, d_scale=d_scale,
-                    amax_d=amax_d, bias=bias, a_row_scale=a_row_scale, b_row_scale=b_row_scale, activation=activation, kernel=kernel,
-                    max_ctas=max_ctas)
+    if a.dim() != 2 or b.dim() != 3 or d.dim() != 2 or ends.dim() != 1:
+        _shapes(a, b, d, ends, "a [rows][N], b [experts][N][K], d [rows][K]")
+    rows, n = a.shape
+    experts, depth, k = b.shape
+    if depth != n or d.shape != (rows, k) or ends.shape[0] != experts:
+        _shapes(a, b, d, ends, "a [rows][N], b [experts][N][K], d [rows][K]")
+    return _grouped("gemm_grouped_dgrad", a, b, d, ends, experts, rows, n, k, n, k, alpha, beta, a_scale, b_scale, d_scale, amax_d, bias, a_row_scale,
+                    b_row_scale, activation, kernel, max_ctas)
 
 
 def gemm_grouped_wgrad(a: torch.Tensor, b: torch.Tensor, d: torch.Tensor, ends: torch.Tensor, *, alpha: float = 1.0, beta: float = 0.0,
@@ -178,24 +190,22 @@ def gemm_grouped_wgrad(a: torch.Tensor, b: torch.Tensor, d: torch.Tensor, ends: 
     """The gradient of ``gemm_grouped`` by its weights: d[e] = alpha * a_scale * b_scale * sum over the rows r of group e of
     a[r]^T b[r], plus beta * d[e]; a [rows][N] is the gradient of the output, b [rows][K] the forward pass's input, d
     [experts][N][K].  An empty group gives beta * d[e] (zeros for beta = 0).  N and K must be multiples of 16."""
-    if a.dim() != 2 or b.dim() != 2 or d.dim() != 3 or ends.dim() != 1 or a.shape[0] != b.shape[0] \
-            or d.shape != (ends.shape[0], a.shape[1], b.shape[1]):
-        raise ValueError(f"a [rows][N], b [rows][K], d [experts][N][K], ends [experts]: got {list(a.shape)}, {list(b.shape)}, "
-                         f"{list(d.shape)}, {list(ends.shape)}")
-    return _grouped("gemm_grouped_wgrad", a, b, d, ends, b.shape[1], alpha=alpha, beta=beta, a_scale=a_scale, b_scale=b_scale, d_scale=d_scale,
-                    amax_d=amax_d, kernel=kernel, max_ctas=max_ctas)
+    if a.dim() != 2 or b.dim() != 2 or d.dim() != 3 or ends.dim() != 1:
+        _shapes(a, b, d, ends, "a [rows][N], b [rows][K], d [experts][N][K]")
+    experts, n, k = d.shape
+    rows, a_cols = a.shape
+    if b.shape != (rows, k) or a_cols != n or ends.shape[0] != experts:
+        _shapes(a, b, d, ends, "a [rows][N], b [rows][K], d [experts][N][K]")
+    return _grouped("gemm_grouped_wgrad", a, b, d, ends, experts, rows, n, k, n, k, alpha, beta, a_scale, b_scale, d_scale, amax_d, None, None, None, 0,
+                    kernel, max_ctas)
 
 
-def _w4(codes, scales, x, y, zeros, lead):
-    """Shapes and layouts that both 4-bit products check; returns (n, k, group, pitches)."""
-    n, half = codes.shape[-2:]
-    k, groups = 2 * half, scales.shape[-1]
-    if groups == 0 or k % groups or k // groups not in (32, 64, 128):
-        raise ValueError(f"scales has one value per row and group of 32, 64 or 128: got {groups} for K = {k}")
-    pitch = (_matrix("codes", codes, U8, (*lead, n, half)), _matrix("scales", scales, WIDE, (*lead, n, groups)),
-             0 if zeros is None else _matrix("zeros", zeros, U8, (*lead, n, groups)),
-             _matrix("x", x, HALF, (x.shape[0], k)), _matrix("y", y, (x.dtype, torch.float32), (y.shape[0], n)))
-    return n, k, k // groups, pitch
+def _w4_group(k: int, groups: int) -> int:
+    """The group size that the number of scales of a row says."""
+    for group in (128, 64, 32):
+        if group * groups == k and groups:
+            return group
+    raise ValueError(f"scales (and zeros) have one value per row and group of 32, 64 or 128 of K: got {groups} groups for K = {k}")
 
 
 def gemv_w4(codes: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, y: torch.Tensor, *, zeros: torch.Tensor | None = None):
@@ -205,13 +215,25 @@ def gemv_w4(codes: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, y: torch
     float16 and says the group size (32, 64 or 128); zeros is uint8 of the same shape, or None for 8.  x [M][K] is bfloat16 or
     float16, y [M][N] has its type or float32.  Made for a few vectors.  Returns y.
     """
-    if codes.dim() != 2 or scales.dim() != 2 or x.dim() != 2 or y.dim() != 2 or x.shape[0] != y.shape[0]:
+    if codes.dim() != 2 or scales.dim() != 2 or x.dim() != 2 or y.dim() != 2:
         raise ValueError("codes [N][K/2], scales [N][K/group], x [M][K], y [M][N]")
-    n, k, group, ld = _w4(codes, scales, x, y, zeros, ())
+    n, half = codes.shape
+    m, k = x.shape
+    lines, groups = scales.shape
+    if k != 2 * half or lines != n or y.shape != (m, n) or (zeros is not None and zeros.shape != (n, groups)):
+        raise ValueError(f"codes [N][K/2], scales and zeros [N][K/group], x [M][K], y [M][N]: got {list(codes.shape)}, {list(scales.shape)}, "
+                         f"{list(x.shape)}, {list(y.shape)}")
+    group = _w4_group(k, groups)
+    ldc, lds, ldx, ldy = _pitch("codes", codes, U8, half), _pitch("scales", scales, WIDE, groups), _pitch("x", x, HALF, k), _pitch("y", y, WIDE, n)
+    if y.dtype != x.dtype and y.dtype != torch.float32:
+        raise TypeError(f"y has x's type or float32, got {y.dtype} and {x.dtype}")
     device = _device(y, codes, scales, x, zeros)
-    _call(device, "gemv_w4", _cabi.lib().b200fp8_gemv_w4, x.shape[0], k, n, group, codes.data_ptr(), ld[0], scales.data_ptr(),
-          WIDE[scales.dtype], ld[1], None if zeros is None else zeros.data_ptr(), ld[2], x.data_ptr(), HALF[x.dtype], ld[3],
-          y.data_ptr(), WIDE[y.dtype], ld[4])
+    if zeros is None:
+        z, ldz = None, 0
+    else:
+        ldz, z = _pitch("zeros", zeros, U8, groups), zeros.data_ptr()
+    _call(device, "gemv_w4", m, k, n, group, codes.data_ptr(), ldc, scales.data_ptr(), WIDE[scales.dtype], lds, z, ldz, x.data_ptr(),
+          HALF[x.dtype], ldx, y.data_ptr(), WIDE[y.dtype], ldy)
     return y
 
 
@@ -225,14 +247,26 @@ def gemv_w4_experts(codes: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, 
     """
     if codes.dim() != 3 or scales.dim() != 3 or x.dim() != 2 or y.dim() != 2:
         raise ValueError("codes [experts][N][K/2], scales [experts][N][K/group], x [tokens][K], y [rows][N]")
-    tokens, rows, experts = x.shape[0], y.shape[0], codes.shape[0]
-    if (rows % tokens if tokens else rows):
-        raise ValueError(f"y's rows ({rows}) must be a multiple of x's ({tokens})")
-    _vector("expert", expert, INT32, (rows,))
-    n, k, group, ld = _w4(codes, scales, x, y, zeros, (experts,))
+    experts, n, half = codes.shape
+    tokens, k = x.shape
+    rows, columns = y.shape
+    matrices, lines, groups = scales.shape
+    if k != 2 * half or columns != n or matrices != experts or lines != n or (rows % tokens if tokens else rows) or \
+            (zeros is not None and zeros.shape != (experts, n, groups)):
+        raise ValueError(f"codes [experts][N][K/2], scales and zeros [experts][N][K/group], x [tokens][K], y [rows][N], rows a multiple of "
+                         f"tokens: got {list(codes.shape)}, {list(scales.shape)}, {list(x.shape)}, {list(y.shape)}")
+    group = _w4_group(k, groups)
+    ids = _vector("expert", expert, INT32, rows)
+    ldc, lds, ldx, ldy = _pitch("codes", codes, U8, half), _pitch("scales", scales, WIDE, groups), _pitch("x", x, HALF, k), _pitch("y", y, WIDE, n)
+    if y.dtype != x.dtype and y.dtype != torch.float32:
+        raise TypeError(f"y has x's type or float32, got {y.dtype} and {x.dtype}")
     device = _device(y, codes, scales, x, expert, zeros)
-    _call(device, "gemv_w4_experts", _cabi.lib().b200fp8_gemv_w4_experts, tokens, rows, experts, k, n, group, codes.data_ptr(), ld[0],
-          _stride(codes, ld[0]), scales.data_ptr(), WIDE[scales.dtype], ld[1], _stride(scales, ld[1]),
-          None if zeros is None else zeros.data_ptr(), ld[2], 0 if zeros is None else _stride(zeros, ld[2]), expert.data_ptr(),
-          x.data_ptr(), HALF[x.dtype], ld[3], y.data_ptr(), WIDE[y.dtype], ld[4])
+    if zeros is None:
+        z, ldz, stride_z = None, 0, 0
+    else:
+        ldz, z = _pitch("zeros", zeros, U8, groups), zeros.data_ptr()
+        stride_z = _stride(zeros, experts, n, ldz)
+    _call(device, "gemv_w4_experts", tokens, rows, experts, k, n, group, codes.data_ptr(), ldc, _stride(codes, experts, n, ldc), scales.data_ptr(),
+          WIDE[scales.dtype], lds, _stride(scales, experts, n, lds), z, ldz, stride_z, ids, x.data_ptr(), HALF[x.dtype], ldx, y.data_ptr(),
+          WIDE[y.dtype], ldy)
     return y

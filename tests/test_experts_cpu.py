@@ -164,8 +164,9 @@ def test_python_layer_proves_shapes_and_types_first(pkg):
 
 
 def test_python_layer_refuses_rows_and_matrices_that_overlap(pkg):
-    e = pkg.experts
+    e, one = pkg.experts, {torch.float32: 0}
     with pytest.raises(ValueError):
-        e._matrix("t", torch.empty(4, 8).as_strided((4, 8), (4, 1)), (torch.float32,), (4, 8))       # rows that overlap
+        e._pitch("t", torch.empty(4, 8).as_strided((4, 8), (4, 1)), one, 8)            # rows that overlap
     with pytest.raises(ValueError):
-        e._matrix("t", torch.empty(100).as_strided((2, 4, 8), (24, 8, 1)), (torch.float32,), (2, 4, 8))   # matrices that overlap
+        e._pitch("t", torch.empty(100).as_strided((2, 4, 8), (24, 8, 1)), one, 8)      # matrices that overlap
+    assert e._pitch("t", torch.empty(4, 16)[:, :8], one, 8) == 16 and e._pitch("t", torch.empty(1, 16)[:, :8], one, 8) == 8
