@@ -254,6 +254,19 @@ cudaError_t grouped(int mode, int experts, int rows, int k, int n, const int* en
     }
 }
 
+template <bool BF16, int Q>
+cudaError_t launch_quantize(const HostDevice& dev, const QuantizeArgs& args, cudaStream_t stream) {
+    const unsigned rows = static_cast<unsigned>(args.rows);
+    const bool pieces = args.k % 8 == 0 && args.ldx % 8 == 0 && args.ldq % 8 == 0 && aligned(args.x, 16) && aligned(args.q, 8);
+    if (!pieces || args.k > 8 * kQuantizePieces * kQuantizeMostThreads)
+        return launch(quantize_rows_any_kernel<BF16>, dev.pdl, dim3(rows, 1, 1), 256, 0, 1, stream, args);
+    const int threads = (args.k + 8 * kQuantizePieces - 1) / (8 * kQuantizePieces);
+    if (threads <= 32) return launch(quantize_rows_kernel<BF16, Q, 32>, dev.pdl, dim3((rows + 3) / 4, 1, 1), 128, 0, 1, stream, args);
+    if (threads <= 128) return launch(quantize_rows_kernel<BF16, Q, 128>, dev.pdl, dim3(rows, 1, 1), 128, 0, 1, stream, args);
+    if (threads <= 256) return launch(quantize_rows_kernel<BF16, Q, 256>, dev.pdl, dim3(rows, 1, 1), 256, 0, 1, stream, args);
+    return launch(quantize_rows_kernel<BF16, Q, 512>, dev.pdl, dim3(rows, 1, 1), 512, 0, 1, stream, args);
+}
+
 template <bool BF16, int G, int NT, bool WIDE>
 cudaError_t launch_w4(const HostDevice& dev, W4Args args, cudaStream_t stream) {
     using L = W4Smem<NT>;
@@ -368,8 +381,9 @@ int b200fp8_quantize_rows(int source_rows, int rows, int k, const void* x, int x
     const cudaError_t e = host_device(&dev);
     if (e != cudaSuccess) return e;
     QuantizeArgs args{static_cast<const uint16_t*>(x), ldx, source_rows, index, rows, k, static_cast<uint8_t*>(q), ldq, scale, q_dtype};
-    auto kernel = x_dtype == B200FP8_OUT_BF16 ? quantize_rows_any_kernel<true> : quantize_rows_any_kernel<false>;
-    return launch(kernel, dev.pdl, dim3(static_cast<unsigned>(rows), 1, 1), 256, 0, 1, static_cast<cudaStream_t>(stream), args);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (x_dtype == B200FP8_OUT_BF16) return q_dtype == B200FP8_E4M3 ? launch_quantize<true, 0>(dev, args, st) : launch_quantize<true, 1>(dev, args, st);
+    return q_dtype == B200FP8_E4M3 ? launch_quantize<false, 0>(dev, args, st) : launch_quantize<false, 1>(dev, args, st);
 }
 
 int b200fp8_gemv_w4(int m, int k, int n, int group, const void* codes, long long code_ld, const void* scales, int scale_dtype,

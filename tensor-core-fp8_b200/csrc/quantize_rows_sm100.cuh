@@ -9,7 +9,9 @@
 // reciprocal normal numbers for rows of zeros.
 //
 // Bound by HBM: 2 bytes read and 1 written per element.  A row stays in registers between the maximum and the
-// conversion, so it is read once.
+// conversion, so it is read once: 32, 128, 256 or 512 threads hold it, four 16-byte pieces each, all loads in flight at
+// once (rows of up to 1024, 4096, 8192 and 16384 elements; a row of up to 1024 is one warp's, without a barrier).  Longer
+// rows and rows that are not 16-byte aligned take the two-pass form at the end.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -34,6 +36,9 @@ struct QuantizeArgs {
 
 constexpr float kQuantizeLeast = 8.271806125530277e-25f;    // 2^-80
 
+constexpr int kQuantizePieces = 4;       // of eight elements per thread
+constexpr int kQuantizeMostThreads = 512;
+
 template <bool BF16>
 __device__ __forceinline__ float2 unpack16(uint32_t w) {
     if constexpr (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
@@ -53,11 +58,35 @@ struct Quotient {
         back = a / two_power;
         inverse = two_power * __frcp_rn(a);
     }
+    // an infinity as the largest finite magnitude, which becomes +-top; a NaN passes
+    __device__ __forceinline__ float finite(float x) const { return fabsf(x) > m ? copysignf(m, x) : x; }
     __device__ __forceinline__ float operator()(float x) const {
-        x = fabsf(x) > m ? copysignf(m, x) : x;                  // an infinity; a NaN passes
         const float u = x * (0.875f * 9.5367431640625e-07f);     // exact: three more bits
         const float z = u * inverse;
         return fmaf(fmaf(-z, back, u), inverse, z);
+    }
+};
+
+// The same on two numbers at once: the packed FP32 instructions round each half as the single ones do.
+struct Quotient2 {
+    uint64_t unit, minus_back, inverse;
+    static __device__ __forceinline__ uint64_t twice(float v) { return pack(make_float2(v, v)); }
+    static __device__ __forceinline__ uint64_t pack(float2 v) {
+        uint64_t r;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+        return r;
+    }
+    __device__ __forceinline__ explicit Quotient2(const Quotient& q)
+        : unit(twice(0.875f * 9.5367431640625e-07f)), minus_back(twice(-q.back)), inverse(twice(q.inverse)) {}
+    __device__ __forceinline__ float2 operator()(float2 x) const {
+        uint64_t u, z, r;
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(u) : "l"(pack(x)), "l"(unit));
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(z) : "l"(u), "l"(inverse));
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(z), "l"(minus_back), "l"(u));
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(r), "l"(inverse), "l"(z));
+        float2 v;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+        return v;
     }
 };
 
@@ -68,17 +97,92 @@ __device__ __forceinline__ float finite_abs(uint16_t bits) {
     return BF16 ? __uint_as_float(static_cast<uint32_t>(mag) << 16) : __half2float(__ushort_as_half(mag));
 }
 
+// the largest of non-negative numbers (ordered like their bit patterns) over a warp, over a block
+__device__ __forceinline__ float warp_max(float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); }
 __device__ __forceinline__ float block_max(float v, float* shared) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    v = warp_max(v);
     const int warps = blockDim.x >> 5;
     if (warps == 1) return v;
     if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = static_cast<int>(threadIdx.x & 31) < warps ? shared[threadIdx.x & 31] : 0.0f;
+    return warp_max(static_cast<int>(threadIdx.x & 31) < warps ? shared[threadIdx.x & 31] : 0.0f);
+}
+
+// The larger magnitude of two pairs of 16-bit floats; a NaN loses against a number.
+template <bool BF16>
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+    b &= 0x7FFF7FFFu;
+    if constexpr (BF16) {
+        const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+        const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+
+// THREADS == 32: four rows to a block of four warps; else one row to a block.
+template <bool BF16, int Q, int THREADS>
+__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) quantize_rows_kernel(const QuantizeArgs args) {
+    __shared__ float shared[THREADS / 32];
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    const long long r = THREADS == 32 ? blockIdx.x * 4ll + (threadIdx.x >> 5) : blockIdx.x;
+    if (THREADS == 32 && r >= args.rows) return;
+    const int t = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x;
+    const int pieces = args.k / 8;
+    const int src = args.index ? __ldg(args.index + r) : static_cast<int>(r);
+    const bool have = src >= 0 && src < args.source_rows;
+    const uint4* x = reinterpret_cast<const uint4*>(args.x + static_cast<long long>(have ? src : 0) * args.ldx);
+    uint4 v[kQuantizePieces];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+    for (int i = 0; i < kQuantizePieces; ++i) {
+        v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (have && t + i * THREADS < pieces) v[i] = __ldg(x + t + i * THREADS);
+    }
+    uint32_t both = 0u;
+#pragma unroll
+    for (int i = 0; i < kQuantizePieces; ++i)
+        both = max_abs2<BF16>(max_abs2<BF16>(max_abs2<BF16>(max_abs2<BF16>(both, v[i].x), v[i].y), v[i].z), v[i].w);
+    const float2 two = unpack16<BF16>(both);
+    auto across = [&](float m) {
+        if constexpr (THREADS == 32) return warp_max(m);
+        else return block_max(m, shared);
+    };
+    float most = across(fmaxf(two.x, two.y));
+    const bool infinite = isinf(most);
+    if (infinite) {                                               // rare: the largest finite magnitude, one element at a time
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kQuantizePieces; ++i) {
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(finite_abs<BF16>(static_cast<uint16_t>(w[j])), finite_abs<BF16>(static_cast<uint16_t>(w[j] >> 16))));
+        }
+        if constexpr (THREADS != 32) __syncthreads();            // everybody has read the first maximum
+        most = across(m);
+    }
+    most = fmaxf(most, kQuantizeLeast);
+    const Quotient quotient(most, Q == 0 ? 512.0f : 65536.0f);
+    uint2* q = reinterpret_cast<uint2*>(args.q + r * args.ldq);
+    auto convert = [&](auto value) {
+#pragma unroll
+        for (int i = 0; i < kQuantizePieces; ++i) {
+            if (t + i * THREADS >= pieces) break;
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            uint32_t b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                b[j] = __nv_cvt_float2_to_fp8x2(value(unpack16<BF16>(w[j])), __NV_SATFINITE, Q == 0 ? __NV_E4M3 : __NV_E5M2);
+            }
+            q[t + i * THREADS] = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+        }
+    };
+    // the comparison with the maximum would be a third of the instructions of a row without infinities
+    const Quotient2 quotient2(quotient);
+    if (infinite) convert([&](float2 f) { return quotient2(make_float2(quotient.finite(f.x), quotient.finite(f.y))); });
+    else convert([&](float2 f) { return quotient2(f); });
+    if (t == 0) args.scale[r] = most / (Q == 0 ? 448.0f : 57344.0f);
 }
 
 // One block per row, any K and any alignment of 2 / 1 bytes: two passes over the row.
@@ -100,7 +204,7 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const QuantizeAr
     const __nv_fp8_interpretation_t kind = args.q_dtype == 0 ? __NV_E4M3 : __NV_E5M2;
     for (int k = threadIdx.x; k < args.k; k += blockDim.x) {
         const float v = have ? unpack16<BF16>(x[k]).x : 0.0f;
-        q[k] = __nv_cvt_float_to_fp8(quotient(v), __NV_SATFINITE, kind);
+        q[k] = __nv_cvt_float_to_fp8(quotient(quotient.finite(v)), __NV_SATFINITE, kind);
     }
     if (threadIdx.x == 0) args.scale[r] = most / (args.q_dtype == 0 ? 448.0f : 57344.0f);
 }
