@@ -101,10 +101,10 @@ struct GroupedCall {
     Epilogue epi;
 };
 
-template <int MODE, int BN, int STAGES, int CTAS>
+template <int MODE, int BN, int CTAS, int OB>
 cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStream_t stream) {
-    using L = GroupedSmem<BN, STAGES, CTAS>;
-    cudaError_t e = allow_smem<gemm_fp8_grouped_kernel<MODE, BN, STAGES, CTAS>>(L::kDynamicBytes);
+    using L = GroupedSmem<BN, CTAS, OB>;
+    cudaError_t e = allow_smem<gemm_fp8_grouped_kernel<MODE, BN, CTAS, OB>>(L::kDynamicBytes);
     if (e != cudaSuccess) return e;
     constexpr int kTile = kTileM * CTAS;
     GroupedArgs args{};
@@ -124,7 +124,7 @@ cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStre
     args.a_cols = c.n;                                            // wgrad
     args.status = dev.status;
     args.epi = c.epi;
-    const int out_bytes = out_dtype_bytes(c.d_dtype);
+    constexpr int out_bytes = OB;
     args.tma_store = (c.ldd * out_bytes) % 16 == 0 && (static_cast<long long>(args.cols) * out_bytes) % 16 == 0 &&
                      (MODE != kGroupedWgrad || (c.stride_d * out_bytes) % 16 == 0) && aligned(c.d, 16);
 
@@ -152,10 +152,10 @@ cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStre
     if (args.tma_store) {
         const CUtensorMapDataType type = out_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : out_bytes == 1 ? u8
                                          : c.d_dtype == B200FP8_OUT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-        const CUtensorMapSwizzle sw = out_bytes == 4 ? s128 : out_bytes == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE;
+        const CUtensorMapSwizzle sw = out_bytes == 1 ? CU_TENSOR_MAP_SWIZZLE_64B : s128;
         const bool wg = MODE == kGroupedWgrad;
         if ((e = encode_3d(dev, &maps.d, type, out_bytes, c.d, args.cols, wg ? c.n : rows, wg ? c.experts : 1, c.ldd,
-                           wg ? c.stride_d : c.ldd * rows, 32, 32, sw)) != cudaSuccess)
+                           wg ? c.stride_d : c.ldd * rows, L::kBoxCols, 32, sw)) != cudaSuccess)
             return e;
     }
     // no more CTAs than there can be tiles: the sizes of the groups are known on the device only
@@ -165,11 +165,11 @@ cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStre
     int units = dev.sm_count / CTAS;
     if (c.max_ctas > 0) units = std::max(1, std::min(units, c.max_ctas / CTAS));
     units = static_cast<int>(std::min<long long>(units, tiles));
-    return launch(gemm_fp8_grouped_kernel<MODE, BN, STAGES, CTAS>, dev.pdl, dim3(static_cast<unsigned>(units * CTAS), 1, 1), kGemmThreads, L::kDynamicBytes, CTAS, stream, maps, args);
+    return launch(gemm_fp8_grouped_kernel<MODE, BN, CTAS, OB>, dev.pdl, dim3(static_cast<unsigned>(units * CTAS), 1, 1), kGemmThreads, L::kDynamicBytes, CTAS, stream, maps, args);
 }
 
-template <int MODE>
-cudaError_t dispatch_grouped(const HostDevice& dev, const GroupedCall& c, int kernel, cudaStream_t stream) {
+template <int MODE, int OB>
+cudaError_t dispatch_grouped_to(const HostDevice& dev, const GroupedCall& c, int kernel, cudaStream_t stream) {
     if (kernel == B200FP8_KERNEL_AUTO) {
         const long long rows = MODE == kGroupedWgrad ? c.n : c.rows / std::max(1, c.experts);   // rows of D per group
         const long long cols = MODE == kGroupedForward ? c.n : c.k;
@@ -179,10 +179,19 @@ cudaError_t dispatch_grouped(const HostDevice& dev, const GroupedCall& c, int ke
                                                                           : B200FP8_KERNEL_CTA1_N128;
     }
     switch (kernel) {
-        case B200FP8_KERNEL_PAIR_N256: return launch_grouped<MODE, 256, 6, 2>(dev, c, stream);
-        case B200FP8_KERNEL_CTA1_N256: return launch_grouped<MODE, 256, 4, 1>(dev, c, stream);
-        case B200FP8_KERNEL_CTA1_N128: return launch_grouped<MODE, 128, 6, 1>(dev, c, stream);
+        case B200FP8_KERNEL_PAIR_N256: return launch_grouped<MODE, 256, 2, OB>(dev, c, stream);
+        case B200FP8_KERNEL_CTA1_N256: return launch_grouped<MODE, 256, 1, OB>(dev, c, stream);
+        case B200FP8_KERNEL_CTA1_N128: return launch_grouped<MODE, 128, 1, OB>(dev, c, stream);
         default: return cudaErrorInvalidValue;
+    }
+}
+
+template <int MODE>
+cudaError_t dispatch_grouped(const HostDevice& dev, const GroupedCall& c, int kernel, cudaStream_t stream) {
+    switch (out_dtype_bytes(c.d_dtype)) {
+        case 4: return dispatch_grouped_to<MODE, 4>(dev, c, kernel, stream);
+        case 2: return dispatch_grouped_to<MODE, 2>(dev, c, kernel, stream);
+        default: return dispatch_grouped_to<MODE, 1>(dev, c, kernel, stream);
     }
 }
 

@@ -148,16 +148,24 @@ struct GroupedWalk {
     }
 };
 
-template <int BN, int STAGES, int CTAS>
+// OB: bytes of an output element
+template <int BN, int CTAS, int OB>
 struct GroupedSmem {
     static constexpr int kABytes = kTileM * kBlockK;
     static constexpr int kBRows = BN / CTAS;
     static constexpr int kBBytes = kBRows * kBlockK;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kEpiBufBytes = 32 * 32 * 4;
-    static constexpr int kEpiOff = STAGES * kStageBytes;
-    static constexpr int kBarOff = kEpiOff + kEpiWarps * kEpiBufBytes;
-    static constexpr int kNumBars = 2 * STAGES + 4;
+    // An epilogue warp stores 32 rows x BN / 2 columns as boxes of 32 rows x 128 bytes (64 for 8-bit outputs), through two
+    // staging buffers where it has two boxes or more: a box is written while the one before it is still read.
+    static constexpr int kBoxCols = OB == 4 ? 32 : 64;
+    static constexpr int kBoxes = BN / 2 / kBoxCols;
+    static constexpr int kBuffers = kBoxes >= 2 ? 2 : 1;
+    static constexpr int kEpiBufBytes = 4096;
+    static constexpr int kEpiBytes = kEpiWarps * kBuffers * kEpiBufBytes;
+    static constexpr int kStages = (227 * 1024 - 1024 - 256 - kEpiBytes) / kStageBytes;   // what is left is the ring
+    static constexpr int kEpiOff = kStages * kStageBytes;
+    static constexpr int kBarOff = kEpiOff + kEpiBytes;
+    static constexpr int kNumBars = 3 * kStages + 4;          // full[] empty[] tfull[2] tempty[2] ragged[]
     static constexpr int kTmemSlotOff = kBarOff + 8 * kNumBars;
     static constexpr int kAbortOff = kTmemSlotOff + 8;
     static constexpr int kDynamicBytes = kAbortOff + 8 + 1024;
@@ -182,11 +190,12 @@ __device__ __forceinline__ void grouped_load_ragged(uint32_t dst, const uint8_t*
     }
 }
 
-template <int MODE, int BN, int STAGES, int CTAS>
+template <int MODE, int BN, int CTAS, int OB>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedArgs args)
 {
-    using L = GroupedSmem<BN, STAGES, CTAS>;
+    using L = GroupedSmem<BN, CTAS, OB>;
+    constexpr int STAGES = L::kStages;
     constexpr bool kPair = CTAS == 2;
     constexpr bool kAMn = MODE == kGroupedWgrad;              // A's row index is the contiguous one
     constexpr bool kBMn = MODE != kGroupedForward;
@@ -204,6 +213,7 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
     const uint32_t bar_empty = bar_full + 8 * STAGES;
     const uint32_t bar_tfull = bar_empty + 8 * STAGES;
     const uint32_t bar_tempty = bar_tfull + 16;
+    const uint32_t bar_ragged = bar_tempty + 16;
     const uint32_t tmem_slot = smem_base + L::kTmemSlotOff;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + L::kAbortOff);
     volatile uint32_t* tmem_slot_gen = reinterpret_cast<volatile uint32_t*>(smem_gen + L::kTmemSlotOff);
@@ -211,9 +221,11 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < STAGES; ++s) {
-            // ragged pairs: the second CTA announces its ordinary stores by an arrival of its own
-            ptx::mbar_init(bar_full + 8 * s, kRagged ? CTAS : 1);
+            ptx::mbar_init(bar_full + 8 * s, 1);
             ptx::mbar_init(bar_empty + 8 * s, 1);
+            // ragged pairs: the second CTA announces its ordinary stores to the leader, for blocks that have some only (an
+            // arrival in the other CTA for every block, as a second arrival on the full barrier, halved the rate)
+            ptx::mbar_init(bar_ragged + 8 * s, 1);
         }
         for (int b = 0; b < 2; ++b) {
             ptx::mbar_init(bar_tfull + 8 * b, 1);
@@ -244,6 +256,7 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
     if (warp == 0) {
         // ---------------- TMA producer: warp-uniform loop, one elected lane issues ----------------
         const uint32_t full0 = kPair ? ptx::mapa(bar_full, 0) : bar_full;   // the leader's full barriers
+        const uint32_t ragged0 = kPair ? ptx::mapa(bar_ragged, 0) : bar_ragged;
         int s = 0, issued = 0;
         uint32_t ph = 0;
         bool ok = true;
@@ -286,7 +299,7 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
                     }
                     if (ptx::elect_one()) {
                         const uint32_t bytes = whole * 4096 * (1 + L::kBRows / 128) * CTAS;
-                        if (rank != 0) ptx::mbar_arrive_cluster(fullr);
+                        if (rank != 0) { if (rest) ptx::mbar_arrive_cluster(ragged0 + 8 * s); }
                         else if (bytes) ptx::mbar_arrive_expect_tx(fullb, bytes);
                         else ptx::mbar_arrive(fullb);
                         for (int p = 0; p < whole; ++p) {
@@ -298,7 +311,6 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
                     }
                 } else if (ptx::elect_one()) {
                     if (rank == 0) ptx::mbar_arrive_expect_tx(fullb, block_bytes * CTAS);
-                    else if (kRagged) ptx::mbar_arrive_cluster(fullr);
                     if (kAMn) load(a_dst, &maps.a[3], row0, k, 0);
                     else load(a_dst, &maps.a[box], k, row0, 0);
                     if (!kBMn) load(b_dst, &maps.b, k, nb0, w.e);
@@ -327,7 +339,7 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
         // ---------------- MMA issuer: leader CTA, warp-uniform loop, one elected lane issues ----------------
         if (rank == 0) {
             int s = 0, it = 0;                                    // `it` counts tiles that have an accumulator
-            uint32_t ph = 0;
+            uint32_t ph = 0, ragged_ph = 0;                       // the latter one bit per slot
             bool ok = true;
             Walk walk(args);
             GroupedTile w;
@@ -345,6 +357,14 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
                         record_failure(args.status, abort_flag, kStatusMmaTimeout);
                         ok = false;
                         break;
+                    }
+                    if (kRagged && kPair && w.k_end - k < kBlockK && (w.k_end - k) % 32 != 0) {
+                        if (!wait_bounded(bar_ragged + 8 * s, (ragged_ph >> s) & 1u, abort_flag, true)) {
+                            record_failure(args.status, abort_flag, kStatusMmaTimeout);
+                            ok = false;
+                            break;
+                        }
+                        ragged_ph ^= 1u << s;
                     }
                     ptx::tc_fence_after();
                     const uint32_t a_src = smem_base + s * L::kStageBytes;
@@ -376,16 +396,19 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
         // ---------------- epilogue warps ----------------
         const int q = warp & 3;                                   // TMEM lane quarter this warp may read
         const int grp = (warp - 2) >> 2;                          // 0 or 1: which half of the tile's columns
-        const uint32_t sb = smem_base + L::kEpiOff + (warp - 2) * L::kEpiBufBytes;   // this warp's staging box
+        const uint32_t staging = smem_base + L::kEpiOff + (warp - 2) * L::kBuffers * L::kEpiBufBytes;
         const uint32_t tempty0 = kPair ? ptx::mapa(bar_tempty, 0) : bar_tempty;
         const bool issuer = ptx::elect_one();                    // this lane owns the warp's bulk-store groups
         constexpr int kChunks = BN / 64;                          // 32-column chunks this warp drains per tile
+        constexpr int kChunksPerBox = L::kBoxCols / 32;
         const int out_dtype = args.epi.out_dtype;
-        const int out_bytes = out_dtype_bytes(out_dtype);
         float alpha0 = args.epi.alpha, dscale = 1.0f, amax = 0.0f;
         if (args.epi.a_scale) alpha0 *= *args.epi.a_scale;
         if (args.epi.b_scale) alpha0 *= *args.epi.b_scale;
         if (args.epi.d_scale) dscale = *args.epi.d_scale;
+        // what few calls ask for sits behind one branch
+        const bool more = args.epi.beta != 0.0f || args.epi.activation != 0 || args.epi.amax != nullptr || args.epi.d_scale != nullptr;
+        int box = 0;                                              // boxes stored so far: they take turns in the staging buffers
         int it = 0;
         Walk walk(args);
         GroupedTile w;
@@ -409,28 +432,29 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
             const int z = MODE == kGroupedWgrad ? w.e : 0;
             const float alpha = (args.epi.a_row_scale != nullptr && lane < rows) ? alpha0 * __ldg(args.epi.a_row_scale + row0 + lane) : alpha0;
 
+            // a box across a group's end must not reach the next group's rows: masked stores; a box across the end of D
+            // itself (wgrad: of D[e]) is clipped by the hardware
+            const bool by_tma = args.tma_store && (rows == 32 || (MODE == kGroupedWgrad && rows > 0));
             auto scale = [&](uint32_t (&v)[32], int col0) {
                 if (args.epi.b_row_scale != nullptr) {
                     const float mine = (col0 + lane < args.cols) ? __ldg(args.epi.b_row_scale + vec_base + col0 + lane) : 1.0f;
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__shfl_sync(0xffffffffu, mine, i) * __uint_as_float(v[i]));
                 }
-                if (args.epi.beta != 0.0f && lane < rows) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(alpha * __uint_as_float(v[i]));
+                if (more && args.epi.beta != 0.0f && lane < rows) {
                     const long long at = d_base + static_cast<long long>(row0 + lane) * args.ldd + col0;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float old = (col0 + i < args.cols) ? load_out(args.d, at + i, out_dtype) : 0.0f;
-                        v[i] = __float_as_uint(alpha * __uint_as_float(v[i]) + args.epi.beta * old);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(alpha * __uint_as_float(v[i]));
+                    for (int i = 0; i < 32; ++i)
+                        if (col0 + i < args.cols) v[i] = __float_as_uint(fmaf(args.epi.beta, load_out(args.d, at + i, out_dtype), __uint_as_float(v[i])));
                 }
                 if (args.epi.bias != nullptr) {
                     const float mine = (col0 + lane < args.cols) ? load_out(args.epi.bias, vec_base + col0 + lane, args.epi.bias_dtype) : 0.0f;
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __shfl_sync(0xffffffffu, mine, i));
                 }
+                if (!more) return;
                 if (args.epi.activation == 1) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(relu(__uint_as_float(v[i])));
@@ -451,105 +475,96 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
                     for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(dscale * __uint_as_float(v[i]));
                 }
             };
-            auto emit = [&](const uint32_t (&v)[32], int col0) {
-                // a box across a group's end must not reach the next group's rows: masked stores; a box across the end
-                // of D itself (wgrad: of D[e]) is clipped by the hardware
-                const bool by_tma = args.tma_store && (rows == 32 || (MODE == kGroupedWgrad && rows > 0));
-                if (issuer) ptx::bulk_wait_group_read<0>();       // the previous store has finished reading the box
-                __syncwarp();
-                if (by_tma && out_bytes == 1) {
-                    const uint32_t at = sb + lane * 32;
+            // Chunk c in registers -> its box; `next` starts the load of the chunk behind it as soon as the registers are free.
+            auto emit = [&](uint32_t (&v)[32], int c, auto next) {
+                const int col0 = w.n0 + grp * (BN / 2) + c * 32;
+                const uint32_t sb = staging + (L::kBuffers == 2 ? (box & 1) * L::kEpiBufBytes : 0);
+                const int part = c % kChunksPerBox;
+                if (by_tma) {
+                    constexpr int kWords = 8 * OB;                // of this chunk per row
+                    uint32_t p[kWords];
+                    if constexpr (OB == 4) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        uint32_t p[4];
+                        for (int i = 0; i < 32; ++i) p[i] = v[i];
+                    } else if constexpr (OB == 2) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            p[j] = pack8(__uint_as_float(v[16 * i + 4 * j]), __uint_as_float(v[16 * i + 4 * j + 1]),
-                                         __uint_as_float(v[16 * i + 4 * j + 2]), __uint_as_float(v[16 * i + 4 * j + 3]), out_dtype);
-                        ptx::st_shared_v4(at + i * 16, p[0], p[1], p[2], p[3]);
+                        for (int i = 0; i < 16; ++i) p[i] = pack16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), out_dtype);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            p[i] = pack8(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]), out_dtype);
                     }
-                } else if (by_tma && out_bytes == 2) {
-                    // rows of 64 bytes under the 64-byte swizzle (16-byte chunk ^ (row / 2) mod 4): no bank conflicts
-                    const uint32_t at = sb + lane * 64;
+                    next();
+                    if (part == 0) {                              // the box that used this buffer before has been read
+                        if (issuer) ptx::bulk_wait_group_read<L::kBuffers - 1>();
+                        __syncwarp();
+                    }
+                    // rows of 128 bytes under the 128-byte swizzle, of 64 under the 64-byte one: no bank conflicts
+                    const uint32_t at = sb + lane * (L::kBoxCols * OB);
+                    const int swizzle = OB == 1 ? (lane >> 1) & 3 : lane & 7;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        ptx::st_shared_v4(at + ((i ^ ((lane >> 1) & 3)) << 4),
-                                          pack16(__uint_as_float(v[8 * i]), __uint_as_float(v[8 * i + 1]), out_dtype),
-                                          pack16(__uint_as_float(v[8 * i + 2]), __uint_as_float(v[8 * i + 3]), out_dtype),
-                                          pack16(__uint_as_float(v[8 * i + 4]), __uint_as_float(v[8 * i + 5]), out_dtype),
-                                          pack16(__uint_as_float(v[8 * i + 6]), __uint_as_float(v[8 * i + 7]), out_dtype));
+                    for (int i = 0; i < kWords / 4; ++i)
+                        ptx::st_shared_v4(at + (((part * (kWords / 4) + i) ^ swizzle) << 4), p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
+                    if (part == kChunksPerBox - 1) {
+                        ptx::fence_proxy_async_smem();
+                        __syncwarp();
+                        const int box0 = col0 - part * 32;
+                        if (issuer) {
+                            if (box0 < args.cols) ptx::tma_store_3d(&maps.d, sb, box0, row0, z);
+                            ptx::bulk_commit_group();
+                        }
+                        ++box;
+                    }
                 } else {
+                    if (issuer) ptx::bulk_wait_group_read<0>();
+                    __syncwarp();
                     const uint32_t at = sb + lane * 128;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         ptx::st_shared_v4(at + ((i ^ (lane & 7)) << 4), v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                }
-                if (by_tma) {
-                    ptx::fence_proxy_async_smem();
-                    __syncwarp();
-                    if (issuer) {
-                        if (col0 < args.cols) ptx::tma_store_3d(&maps.d, sb, col0, row0, z);
-                        ptx::bulk_commit_group();
-                    }
-                } else {
+                    next();
                     __syncwarp();
                     const int col = col0 + lane;                  // one instruction writes 32 elements of one row
                     if (col < args.cols) {
-                        long long at = d_base + static_cast<long long>(row0) * args.ldd + col;
-                        for (int r = 0; r < rows; ++r, at += args.ldd) {
+                        long long to = d_base + static_cast<long long>(row0) * args.ldd + col;
+                        for (int r = 0; r < rows; ++r, to += args.ldd) {
                             const uint32_t bits = ptx::ld_shared_u32(sb + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2)));
-                            store_out(args.d, at, __uint_as_float(bits), out_dtype);
+                            store_out(args.d, to, __uint_as_float(bits), out_dtype);
                         }
                     }
                     __syncwarp();
                 }
             };
 
-            const int col_base = w.n0 + grp * (BN / 2);
-            if (empty) {
-                uint32_t v[32];
-#pragma unroll 1
-                for (int c = 0; c < kChunks; ++c) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = 0u;
-                    scale(v, col_base + c * 32);
-                    emit(v, col_base + c * 32);
-                }
-                continue;
-            }
-            auto release_slot = [&]() {                           // accumulator columns of this warp are in registers
+            if (!empty && rows <= 0) {                            // nothing of this quarter belongs to the group
                 ptx::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
                     if (kPair) ptx::mbar_arrive_cluster(tempty0 + 8 * slot);
                     else ptx::mbar_arrive(bar_tempty + 8 * slot);
                 }
-            };
-            if (rows <= 0) {                                      // nothing of this quarter belongs to the group
-                release_slot();
                 continue;
             }
-            // two register sets: the TMEM load of chunk c+1 is in flight while chunk c is stored
-            uint32_t va[32], vb[32];
-            ptx::tmem_ld_32x32(t_addr, va);
-            if constexpr (kChunks == 1) {
-                ptx::tmem_ld_wait();
-                release_slot();
-                scale(va, col_base);
-                emit(va, col_base);
-            } else {
+            uint32_t v[32];
+            if (!empty) ptx::tmem_ld_32x32(t_addr, v);
 #pragma unroll 1
-                for (int c = 0; c < kChunks; c += 2) {
+            for (int c = 0; c < kChunks; ++c) {
+                if (empty) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = 0u;
+                } else {
                     ptx::tmem_ld_wait();
-                    ptx::tmem_ld_32x32(t_addr + (c + 1) * 32, vb);
-                    scale(va, col_base + c * 32);
-                    emit(va, col_base + c * 32);
-                    ptx::tmem_ld_wait();
-                    if (c + 2 < kChunks) ptx::tmem_ld_32x32(t_addr + (c + 2) * 32, va);
-                    else release_slot();
-                    scale(vb, col_base + (c + 1) * 32);
-                    emit(vb, col_base + (c + 1) * 32);
+                    if (c == kChunks - 1) {                       // the accumulator's columns of this warp are in registers
+                        ptx::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (kPair) ptx::mbar_arrive_cluster(tempty0 + 8 * slot);
+                            else ptx::mbar_arrive(bar_tempty + 8 * slot);
+                        }
+                    }
                 }
+                scale(v, w.n0 + grp * (BN / 2) + c * 32);
+                emit(v, c, [&]() { if (!empty && c + 1 < kChunks) ptx::tmem_ld_32x32(t_addr + (c + 1) * 32, v); });
             }
         }
         // the staging box must outlive the stores' reads of it; the writes themselves complete with the grid
