@@ -101,71 +101,63 @@ struct GroupedCall {
     Epilogue epi;
 };
 
-template <int MODE, int BN, int CTAS, int OB>
+template <int MODE, int ROWS, int CTAS, int OB>
 cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStream_t stream) {
-    using L = GroupedSmem<BN, CTAS, OB>;
-    cudaError_t e = allow_smem<gemm_fp8_grouped_kernel<MODE, BN, CTAS, OB>>(L::kDynamicBytes);
+    using L = GroupedSmem<ROWS, CTAS>;
+    constexpr bool wgrad = MODE == kGroupedWgrad;
+    cudaError_t e = allow_smem<gemm_fp8_grouped_kernel<MODE, ROWS, CTAS, OB>>(L::kDynamicBytes);
     if (e != cudaSuccess) return e;
-    constexpr int kTile = kTileM * CTAS;
     GroupedArgs args{};
     args.experts = c.experts;
     args.rows = c.rows;
     args.cols = MODE == kGroupedForward ? c.n : c.k;
     args.depth = MODE == kGroupedForward ? c.k : c.n;
-    args.tile_rows_all = c.n;
+    args.d_rows = c.n;                                            // wgrad
     args.ends = c.ends;
-    args.m_tiles = (c.n + kTile - 1) / kTile;                     // wgrad
-    args.n_tiles = (args.cols + BN - 1) / BN;
-    args.group_m = 16;
-    args.idesc = make_idesc_f8(c.a_dtype, c.b_dtype, kTile, BN) | (MODE == kGroupedWgrad ? 1u << 15 : 0u) | (MODE != kGroupedForward ? 1u << 16 : 0u);
+    args.row_tiles = (c.n + ROWS - 1) / ROWS;                     // wgrad
+    args.col_tiles = (args.cols + 128 * CTAS - 1) / (128 * CTAS);
+    args.group_rows = 16;
+    // the operand of D's columns is the instruction's A, that of D's rows its B; bits 15 and 16: MN-major
+    const void* w = c.b;
+    const int w_dtype = c.b_dtype, r_dtype = c.a_dtype;
+    args.idesc = make_idesc_f8(w_dtype, r_dtype, 128 * CTAS, 0) | (MODE != kGroupedForward ? 1u << 15 : 0u) | (wgrad ? 1u << 16 : 0u);
     args.d = c.d; args.ldd = c.ldd; args.stride_d = c.stride_d;
-    args.a = static_cast<const uint8_t*>(c.a); args.lda = c.lda;
-    args.b = static_cast<const uint8_t*>(c.b); args.ldb = c.ldb;
-    args.a_cols = c.n;                                            // wgrad
+    args.w = static_cast<const uint8_t*>(w); args.ldw = c.ldb;
+    args.r = static_cast<const uint8_t*>(c.a); args.ldr = c.lda;
     args.status = dev.status;
     args.epi = c.epi;
-    constexpr int out_bytes = OB;
-    args.tma_store = (c.ldd * out_bytes) % 16 == 0 && (static_cast<long long>(args.cols) * out_bytes) % 16 == 0 &&
-                     (MODE != kGroupedWgrad || (c.stride_d * out_bytes) % 16 == 0) && aligned(c.d, 16);
+    args.packed_store = OB == 2 && args.cols % 2 == 0 && c.ldd % 2 == 0 && (!wgrad || c.stride_d % 2 == 0) && aligned(c.d, 4);
 
     GroupedMaps maps;
     const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const CUtensorMapSwizzle s128 = CU_TENSOR_MAP_SWIZZLE_128B;
-    const uint64_t a_cols = MODE == kGroupedForward ? c.k : c.n;
     const uint64_t rows = static_cast<uint64_t>(std::max(1, c.rows));
-    for (int i = 0; i < 4; ++i) {
-        if (i < 3 && (MODE == kGroupedWgrad ? i != 1 : CTAS == 2)) { continue; }
-        const uint32_t box = MODE == kGroupedWgrad && i == 1 ? 32 : 16u << i;
-        if ((e = encode_3d(dev, &maps.a[i], u8, 1, c.a, a_cols, rows, 1, c.lda, c.lda * rows, kBlockK, box, s128)) != cudaSuccess) return e;
-    }
-    if (MODE == kGroupedWgrad) {
-        const uint64_t whole = c.ldb * rows;
-        if ((e = encode_3d(dev, &maps.b, u8, 1, c.b, c.k, rows, 1, c.ldb, whole, kBlockK, 128, s128)) != cudaSuccess) return e;
-        if ((e = encode_3d(dev, &maps.b32, u8, 1, c.b, c.k, rows, 1, c.ldb, whole, kBlockK, 32, s128)) != cudaSuccess) return e;
-    } else if ((e = encode_3d(dev, &maps.b, u8, 1, c.b, c.k, c.n, c.experts, c.ldb, c.stride_b, kBlockK, MODE == kGroupedForward ? L::kBRows : 128, s128)) != cudaSuccess) {
-        return e;
-    }
-    for (int i = 0; i < 3; ++i)
-        if (MODE == kGroupedWgrad ? i != 1 : CTAS == 2) maps.a[i] = maps.a[3];    // not used by this kernel
-    if (MODE != kGroupedWgrad) maps.b32 = maps.b;
-    maps.d = maps.b;
-    if (args.tma_store) {
-        const CUtensorMapDataType type = out_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : out_bytes == 1 ? u8
-                                         : c.d_dtype == B200FP8_OUT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-        const CUtensorMapSwizzle sw = out_bytes == 1 ? CU_TENSOR_MAP_SWIZZLE_64B : s128;
-        const bool wg = MODE == kGroupedWgrad;
-        if ((e = encode_3d(dev, &maps.d, type, out_bytes, c.d, args.cols, wg ? c.n : rows, wg ? c.experts : 1, c.ldd,
-                           wg ? c.stride_d : c.ldd * rows, L::kBoxCols, 32, sw)) != cudaSuccess)
-            return e;
+    auto ragged = [&](CUtensorMap* map, const void* base, uint64_t cols, long long ld, uint32_t box) {
+        return encode_3d(dev, map, u8, 1, base, cols, rows, 1, ld, ld * rows, kBlockK, box, s128);
+    };
+    const uint64_t r_cols = MODE == kGroupedForward ? c.k : c.n;
+    if (wgrad) {
+        if ((e = ragged(&maps.w, w, c.k, c.ldb, 128)) != cudaSuccess) return e;
+        if ((e = ragged(&maps.w32, w, c.k, c.ldb, 32)) != cudaSuccess) return e;
+        if ((e = ragged(&maps.r[3], c.a, r_cols, c.lda, 128)) != cudaSuccess) return e;
+        if ((e = ragged(&maps.r32, c.a, r_cols, c.lda, 32)) != cudaSuccess) return e;
+        maps.r[0] = maps.r[1] = maps.r[2] = maps.r[3];            // not used
+    } else {
+        if ((e = encode_3d(dev, &maps.w, u8, 1, w, c.k, c.n, c.experts, c.ldb, c.stride_b, kBlockK, 128, s128)) != cudaSuccess) return e;
+        for (int i = 0; i < 4; ++i)
+            if ((e = ragged(&maps.r[i], c.a, r_cols, c.lda, 16u << i)) != cudaSuccess) return e;
+        maps.w32 = maps.w;                                        // not used
+        maps.r32 = maps.r[3];
     }
     // no more CTAs than there can be tiles: the sizes of the groups are known on the device only
-    const long long groups = MODE == kGroupedWgrad ? c.experts : std::min(c.experts, c.rows);
-    const long long tiles = (MODE == kGroupedWgrad ? groups * args.m_tiles : groups + c.rows / kTile) * args.n_tiles;
+    const long long groups = wgrad ? c.experts : std::min(c.experts, c.rows);
+    const long long tiles = (wgrad ? groups * args.row_tiles : groups + c.rows / ROWS) * args.col_tiles;
     if (tiles > (1LL << 30)) return cudaErrorInvalidValue;
     int units = dev.sm_count / CTAS;
     if (c.max_ctas > 0) units = std::max(1, std::min(units, c.max_ctas / CTAS));
     units = static_cast<int>(std::min<long long>(units, tiles));
-    return launch(gemm_fp8_grouped_kernel<MODE, BN, CTAS, OB>, dev.pdl, dim3(static_cast<unsigned>(units * CTAS), 1, 1), kGemmThreads, L::kDynamicBytes, CTAS, stream, maps, args);
+    return launch(gemm_fp8_grouped_kernel<MODE, ROWS, CTAS, OB>, dev.pdl, dim3(static_cast<unsigned>(units * CTAS), 1, 1), kGemmThreads, L::kDynamicBytes,
+                  CTAS, stream, maps, args);
 }
 
 template <int MODE, int OB>
@@ -173,15 +165,19 @@ cudaError_t dispatch_grouped_to(const HostDevice& dev, const GroupedCall& c, int
     if (kernel == B200FP8_KERNEL_AUTO) {
         const long long rows = MODE == kGroupedWgrad ? c.n : c.rows / std::max(1, c.experts);   // rows of D per group
         const long long cols = MODE == kGroupedForward ? c.n : c.k;
-        const long long tiles = static_cast<long long>(c.experts) * ((rows + 127) / 128) * ((cols + 255) / 256);
+        const long long tiles = static_cast<long long>(c.experts) * ((rows + 255) / 256) * ((cols + 127) / 128);
         kernel = rows >= 192 && cols > 128 && tiles >= 2LL * dev.sm_count ? B200FP8_KERNEL_PAIR_N256
-                 : tiles >= dev.sm_count && rows > 64                     ? B200FP8_KERNEL_CTA1_N256
-                                                                          : B200FP8_KERNEL_CTA1_N128;
+                 : rows > 64                                              ? B200FP8_KERNEL_CTA1_N128
+                 : MODE == kGroupedWgrad                                  ? B200FP8_KERNEL_CTA1_N128
+                                                                          : B200FP8_KERNEL_CTA1_N64;
     }
     switch (kernel) {
         case B200FP8_KERNEL_PAIR_N256: return launch_grouped<MODE, 256, 2, OB>(dev, c, stream);
         case B200FP8_KERNEL_CTA1_N256: return launch_grouped<MODE, 256, 1, OB>(dev, c, stream);
         case B200FP8_KERNEL_CTA1_N128: return launch_grouped<MODE, 128, 1, OB>(dev, c, stream);
+        case B200FP8_KERNEL_CTA1_N64:
+            if constexpr (MODE != kGroupedWgrad) return launch_grouped<MODE, 64, 1, OB>(dev, c, stream);
+            return cudaErrorInvalidValue;
         default: return cudaErrorInvalidValue;
     }
 }
@@ -228,7 +224,8 @@ cudaError_t grouped(int mode, int experts, int rows, int k, int n, const int* en
         if (static_cast<double>(rows) * static_cast<double>(lda) > 5e11 || static_cast<double>(rows) * static_cast<double>(wgrad ? ldb : ldd) * out_bytes > 1e12) return cudaErrorInvalidValue;
     }
     const int kernel = options ? options->kernel : B200FP8_KERNEL_AUTO;
-    if (kernel != B200FP8_KERNEL_AUTO && kernel != B200FP8_KERNEL_PAIR_N256 && kernel != B200FP8_KERNEL_CTA1_N256 && kernel != B200FP8_KERNEL_CTA1_N128)
+    if (kernel != B200FP8_KERNEL_AUTO && kernel != B200FP8_KERNEL_PAIR_N256 && kernel != B200FP8_KERNEL_CTA1_N256 &&
+        kernel != B200FP8_KERNEL_CTA1_N128 && (wgrad || kernel != B200FP8_KERNEL_CTA1_N64))
         return cudaErrorInvalidValue;
     HostDevice dev;
     cudaError_t e = host_device(&dev);
@@ -329,7 +326,6 @@ cudaError_t launch_w4_type(const HostDevice& dev, const W4Args& args, cudaStream
 }
 
 cudaError_t w4(const W4Args& args, int x_dtype, cudaStream_t stream) {
-    const bool by_expert = args.expert != nullptr;
     if (args.n < 0 || args.k <= 0 || args.m < 0 || args.code_ld > (1LL << 39) || args.code_stride > (1LL << 39)) return cudaErrorInvalidValue;
     if (x_dtype != B200FP8_OUT_BF16 && x_dtype != B200FP8_OUT_F16) return cudaErrorInvalidValue;
     if (args.y_dtype != x_dtype && args.y_dtype != B200FP8_OUT_F32) return cudaErrorInvalidValue;

@@ -14,17 +14,25 @@
 //
 // Structure: that of the dense kernel (gemm_sm100.cuh) -- a persistent CTA or CTA pair per SM, warp 0 TMA producer into a
 // ring of k-blocks (128 bytes of contraction each), warp 1 MMA issue, warps 2-9 epilogue out of two TMEM accumulator
-// slots -- with a walk over tiles that every warp derives from `ends` by itself (32 groups at a time in the lanes of a
-// warp, one scan and one ballot per tile), so there is no schedule to build, no workspace and no second launch.
+// slots -- with two differences:
 //
-//   * Rows behind a group's end inside a tile belong to the next group.  Forward and dgrad multiply them (each row of a
-//     product depends on its own row of A only) and do not store them: 32-row boxes that lie inside the group go out
-//     by TMA, the box across the end by masked stores.  A one-CTA tile picks the shortest of four A boxes (16, 32, 64,
-//     128 rows) that covers its rows, so a decode step's few rows per expert cost few bytes next to the weights.
-//   * wgrad contracts over the rows, so the block across a group's end must not see the next group: it is loaded as 32-row
-//     TMA boxes, and the last, ragged 32 rows with ordinary loads that put zeros behind the end (a product with
-//     zero would not do: the other operand's foreign rows may hold infinities or NaN).  The MMA issues only as many
-//     K = 32 steps as there are rows.  A group without rows stores zeros (or beta * D).
+//   * The walk over tiles: every warp derives it from `ends` by itself (32 groups at a time in the lanes of a warp, one scan
+//     and one ballot per tile), so there is no schedule to build, no workspace and no second launch.
+//   * The accumulator is D transposed: the columns of D (128 per CTA, contiguous in memory) are the tensor core's M index
+//     = the lanes of TMEM, the ragged rows its N index.  N is set per tile to the tile's rows rounded up to 16 (32 for a
+//     pair), so a group's last tile costs what its rows cost: with 256-row tiles and groups of about a thousand rows,
+//     tiles of full height wasted an eighth of the multiplications (and, in a power-limited run, of the energy); a decode
+//     step's few rows per expert cost few bytes and cycles next to the weights (a tile loads the shortest of four boxes,
+//     16 to 128 rows, that covers them).  In the epilogue a lane owns one column, so the vectors per column (b_row_scale,
+//     bias) are one register, a warp's store of one row is contiguous, rows behind a group's end are simply not stored,
+//     and D needs neither staging nor TMA nor any alignment beyond its element.
+//
+// Rows behind a group's end inside a tile belong to the next group.  Forward and dgrad may load and multiply them (each
+// row of a product depends on its own row of A only) and do not store them.  wgrad contracts over the rows, so the block
+// across a group's end must not see the next group: it is loaded as 32-row TMA boxes, and the last, ragged 32 rows
+// with ordinary loads that put zeros behind the end (a product with zero would not do: the other operand's foreign rows
+// may hold infinities or NaN).  The MMA issues only as many K = 32 steps as there are rows.  A group without rows stores
+// zeros (or beta * D).
 //
 // Every wait on an mbarrier is bounded, as in the dense kernel.
 #pragma once
@@ -37,31 +45,31 @@ namespace b200fp8 {
 
 enum GroupedMode : int { kGroupedForward = 0, kGroupedDgrad = 1, kGroupedWgrad = 2 };
 
+// The operand whose index becomes the columns of D (W: the weights; wgrad: the input X) and the one whose index becomes its
+// rows (R: the ragged rows; wgrad: the output's gradient, N columns).
 struct GroupedMaps {
-    CUtensorMap a[4];     // forward, dgrad: boxes of 16, 32, 64, 128 rows; wgrad: [1] 32 rows, [3] 128 rows
-    CUtensorMap b;        // forward: BN / CTAS rows of 128 bytes; dgrad, wgrad: 128 rows of 128 bytes
-    CUtensorMap b32;      // wgrad: 32 rows
-    CUtensorMap d;        // 32 x 32 boxes of D
+    CUtensorMap w;        // 128 x 128 boxes
+    CUtensorMap r[4];     // forward, dgrad: boxes of 16, 32, 64, 128 rows; wgrad: [3] 128 x 128
+    CUtensorMap w32, r32; // wgrad: 32 rows of 128 bytes
 };
 
 struct GroupedArgs {
     int experts;
     int rows;             // rows of the ragged operands
-    int tile_rows_all;    // wgrad: rows of D per expert (N)
+    int d_rows;           // wgrad: rows of D per expert (N)
     int cols;             // columns of D
     int depth;            // contraction extent: K forward, N dgrad (wgrad: the group's rows)
     const int* ends;
-    int m_tiles;          // wgrad: tiles along the rows of D[e]
-    int n_tiles;
-    int group_m;          // forward, dgrad: tiles are walked down `group_m` M-tiles before moving along the columns
-    uint32_t idesc;
-    int tma_store;
+    int row_tiles;        // wgrad: tiles along the rows of D[e]
+    int col_tiles;
+    int group_rows;       // tiles are walked down this many row tiles before the next column tile
+    uint32_t idesc;       // without N
+    int packed_store;     // 16-bit D: two neighbouring columns can be stored as one 32-bit word
     void* d;
     long long ldd, stride_d;
-    const uint8_t* a;     // wgrad: base pointers of the ragged rows' ordinary loads
-    const uint8_t* b;
-    long long lda, ldb;
-    int a_cols;
+    const uint8_t* w;     // wgrad: base pointers of the ragged rows' ordinary loads
+    const uint8_t* r;
+    long long ldw, ldr;
     int* status;
     Epilogue epi;
 };
@@ -69,14 +77,14 @@ struct GroupedArgs {
 // One tile: expert, position, and what it multiplies.
 struct GroupedTile {
     int e;
-    int row0;     // forward, dgrad: first row of the tile in A and D; wgrad: first row of the tile in D[e]
-    int row_end;  // first row that is not the tile's to store
-    int n0;
+    int row0;        // forward, dgrad: first row of the tile in R and D; wgrad: first row of the tile in D[e]
+    int rows;        // rows of the tile (>= 1)
+    int col0;        // first column of the tile (of the pair)
     int k0, k_end;   // contraction range (wgrad: rows of the group)
 };
 
 // Walk over the tiles of all groups in order.  All 32 lanes call it together.
-template <int MODE, int TILE_M, int BN>
+template <int MODE, int TILE_ROWS, int TILE_COLS>
 struct GroupedWalk {
     const GroupedArgs& args;
     int lane;
@@ -101,8 +109,8 @@ struct GroupedWalk {
         start = __shfl_up_sync(0xffffffffu, end, 1);
         if (lane == 0) start = carry;
         carry = __shfl_sync(0xffffffffu, end, 31);
-        if (MODE == kGroupedWgrad) upto = e < args.experts ? args.m_tiles * args.n_tiles : 0;
-        else upto = (end - start + TILE_M - 1) / TILE_M * args.n_tiles;
+        if (MODE == kGroupedWgrad) upto = e < args.experts ? args.row_tiles * args.col_tiles : 0;
+        else upto = (end - start + TILE_ROWS - 1) / TILE_ROWS * args.col_tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int other = __shfl_up_sync(0xffffffffu, upto, o);
@@ -125,22 +133,22 @@ struct GroupedWalk {
         const int before = who == 0 ? 0 : __shfl_sync(0xffffffffu, upto, who - 1);
         const int r = local - before;
         w.e = chunk + who;
-        const int m_tiles = MODE == kGroupedWgrad ? args.m_tiles : (f - s + TILE_M - 1) / TILE_M;
-        const int per_group = args.group_m * args.n_tiles;
+        const int extent = MODE == kGroupedWgrad ? args.d_rows : f - s;
+        const int row_tiles = MODE == kGroupedWgrad ? args.row_tiles : (extent + TILE_ROWS - 1) / TILE_ROWS;
+        const int per_group = args.group_rows * args.col_tiles;
         const int g = r / per_group;
-        const int first_m = g * args.group_m;
-        const int gsz = min(args.group_m, m_tiles - first_m);
+        const int first = g * args.group_rows;
+        const int size = min(args.group_rows, row_tiles - first);
         const int in_group = r - g * per_group;
-        const int m0 = (first_m + in_group % gsz) * TILE_M;
-        w.n0 = in_group / gsz * BN;
+        const int at = (first + in_group % size) * TILE_ROWS;
+        w.col0 = in_group / size * TILE_COLS;
+        w.rows = min(TILE_ROWS, extent - at);
         if (MODE == kGroupedWgrad) {
-            w.row0 = m0;
-            w.row_end = args.tile_rows_all;
+            w.row0 = at;
             w.k0 = s;
             w.k_end = f;
         } else {
-            w.row0 = s + m0;
-            w.row_end = f;
+            w.row0 = s + at;
             w.k0 = 0;
             w.k_end = args.depth;
         }
@@ -148,28 +156,23 @@ struct GroupedWalk {
     }
 };
 
-// OB: bytes of an output element
-template <int BN, int CTAS, int OB>
+// ROWS: rows of D per tile (of the pair), the largest N of the MMA
+template <int ROWS, int CTAS>
 struct GroupedSmem {
-    static constexpr int kABytes = kTileM * kBlockK;
-    static constexpr int kBRows = BN / CTAS;
-    static constexpr int kBBytes = kBRows * kBlockK;
-    static constexpr int kStageBytes = kABytes + kBBytes;
-    // An epilogue warp stores 32 rows x BN / 2 columns as boxes of 32 rows x 128 bytes (64 for 8-bit outputs), through two
-    // staging buffers where it has two boxes or more: a box is written while the one before it is still read.
-    static constexpr int kBoxCols = OB == 4 ? 32 : 64;
-    static constexpr int kBoxes = BN / 2 / kBoxCols;
-    static constexpr int kBuffers = kBoxes >= 2 ? 2 : 1;
-    static constexpr int kEpiBufBytes = 4096;
-    static constexpr int kEpiBytes = kEpiWarps * kBuffers * kEpiBufBytes;
-    static constexpr int kStages = (227 * 1024 - 1024 - 256 - kEpiBytes) / kStageBytes;   // what is left is the ring
-    static constexpr int kEpiOff = kStages * kStageBytes;
-    static constexpr int kBarOff = kEpiOff + kEpiBytes;
-    static constexpr int kNumBars = 3 * kStages + 4;          // full[] empty[] tfull[2] tempty[2] ragged[]
+    static constexpr int kWBytes = 128 * kBlockK;
+    static constexpr int kRRows = ROWS / CTAS;
+    static constexpr int kRBytes = kRRows * kBlockK;
+    static constexpr int kStageBytes = kWBytes + kRBytes;
+    static constexpr int kScaleBytes = kEpiWarps * ROWS / 2 * 4;             // row scales of a warp's rows
+    static constexpr int kStages = (227 * 1024 - 1024 - 384 - kScaleBytes) / kStageBytes;   // what is left is the ring
+    static constexpr int kScaleOff = kStages * kStageBytes;
+    static constexpr int kBarOff = kScaleOff + kScaleBytes;
+    static constexpr int kNumBars = 3 * kStages + 4;                        // full[] empty[] tfull[2] tempty[2] ragged[]
     static constexpr int kTmemSlotOff = kBarOff + 8 * kNumBars;
     static constexpr int kAbortOff = kTmemSlotOff + 8;
     static constexpr int kDynamicBytes = kAbortOff + 8 + 1024;
-    static constexpr int kTmemCols = 2 * BN;
+    static constexpr int kTmemCols = 2 * ROWS;                              // two accumulator slots
+    static_assert(8 * kNumBars + 16 <= 384 && kTmemCols <= 512, "layout");
 };
 
 // `rows` (< 32) rows of 128 bytes of a row-contiguous operand into a 32-row piece of a swizzled box, zeros behind them and
@@ -190,17 +193,19 @@ __device__ __forceinline__ void grouped_load_ragged(uint32_t dst, const uint8_t*
     }
 }
 
-template <int MODE, int BN, int CTAS, int OB>
+template <int MODE, int ROWS, int CTAS, int OB>               // OB: bytes of an element of D
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedArgs args)
 {
-    using L = GroupedSmem<BN, CTAS, OB>;
+    using L = GroupedSmem<ROWS, CTAS>;
     constexpr int STAGES = L::kStages;
     constexpr bool kPair = CTAS == 2;
-    constexpr bool kAMn = MODE == kGroupedWgrad;              // A's row index is the contiguous one
-    constexpr bool kBMn = MODE != kGroupedForward;
+    constexpr bool kWMn = MODE != kGroupedForward;            // W's row index (of memory) is the contraction
+    constexpr bool kRMn = MODE == kGroupedWgrad;              // ... and R's
     constexpr bool kRagged = MODE == kGroupedWgrad;           // the contraction ends inside a block
-    static_assert(BN % 64 == 0 && BN <= 256 && (!kBMn || L::kBRows % 128 == 0), "tile");
+    constexpr int kStep = kPair ? 32 : 16;                    // granularity of N
+    constexpr int kRBoxes = kRMn ? L::kRRows / 128 : 1;       // boxes of 128 columns of R per block (wgrad)
+    static_assert(ROWS % 64 == 0 && ROWS <= 256 && (!kRMn || L::kRRows % 128 == 0), "tile");
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_addr(smem_raw));
@@ -232,9 +237,8 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
             ptx::mbar_init(bar_tempty + 8 * b, kEpiWarps * CTAS);
         }
         ptx::fence_mbar_init();
-        ptx::prefetch_tensormap(&maps.a[3]);
-        ptx::prefetch_tensormap(&maps.b);
-        ptx::prefetch_tensormap(&maps.d);
+        ptx::prefetch_tensormap(&maps.w);
+        ptx::prefetch_tensormap(&maps.r[3]);
     }
     if (warp == 1) {
         ptx::tmem_alloc<CTAS>(tmem_slot, L::kTmemCols);
@@ -251,11 +255,11 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
 
     const int step = gridDim.x / CTAS;
     const int first = blockIdx.x / CTAS;
-    using Walk = GroupedWalk<MODE, kTileM * CTAS, BN>;
+    using Walk = GroupedWalk<MODE, ROWS, 128 * CTAS>;
 
     if (warp == 0) {
         // ---------------- TMA producer: warp-uniform loop, one elected lane issues ----------------
-        const uint32_t full0 = kPair ? ptx::mapa(bar_full, 0) : bar_full;   // the leader's full barriers
+        const uint32_t full0 = kPair ? ptx::mapa(bar_full, 0) : bar_full;   // the leader's barriers
         const uint32_t ragged0 = kPair ? ptx::mapa(bar_ragged, 0) : bar_ragged;
         int s = 0, issued = 0;
         uint32_t ph = 0;
@@ -263,22 +267,20 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
         Walk walk(args);
         GroupedTile w;
         for (long long t = first; ok && walk.seek(t, w); t += step) {
-            const int row0 = w.row0 + static_cast<int>(rank) * kTileM;       // this CTA's rows of the tile
-            const int nb0 = w.n0 + static_cast<int>(rank) * L::kBRows;
-            int box = 3;                                                     // A boxes of 16 << box rows
-            if (!kPair && !kRagged) {
-                const int have = w.row_end - row0;
-                box = have > 64 ? 3 : have > 32 ? 2 : have > 16 ? 1 : 0;
-            }
-            const uint32_t block_bytes = kRagged ? L::kStageBytes : (16 << box) * kBlockK + L::kBBytes;
+            const int n = (w.rows + kStep - 1) / kStep * kStep;              // the MMA's N
+            const int mine = n / CTAS;                                       // rows of R in this CTA
+            const int col0 = w.col0 + static_cast<int>(rank) * 128, row0 = w.row0 + static_cast<int>(rank) * mine;
+            const int box = kRMn ? 3 : mine > 64 ? 3 : mine > 32 ? 2 : mine > 16 ? 1 : 0;   // boxes of 16 << box rows
+            const int boxes = kRMn ? kRBoxes : (mine + 127) / 128;           // one box, two for more than 128 rows
+            const uint32_t block_bytes = L::kWBytes + boxes * ((16 << box) * kBlockK);
             for (int k = w.k0; k < w.k_end; k += kBlockK) {
                 if (!wait_bounded(bar_empty + 8 * s, ph ^ 1u, abort_flag, kPair)) {
                     record_failure(args.status, abort_flag, kStatusProducerTimeout);
                     ok = false;
                     break;
                 }
-                const uint32_t a_dst = smem_base + s * L::kStageBytes;
-                const uint32_t b_dst = a_dst + L::kABytes;
+                const uint32_t w_dst = smem_base + s * L::kStageBytes;
+                const uint32_t r_dst = w_dst + L::kWBytes;
                 const uint32_t fullb = bar_full + 8 * s, fullr = full0 + 8 * s;
                 auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y, int z) {
                     if (kPair) ptx::tma_load_3d_pair(dst, map, x, y, z, fullr);
@@ -289,35 +291,37 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
                     // the block across the group's end: whole 32-row pieces by TMA, the ragged one with ordinary loads
                     const int whole = valid / 32, rest = valid % 32;
                     if (rest) {
-                        grouped_load_ragged(a_dst + whole * 4096, args.a + (static_cast<long long>(k) + whole * 32) * args.lda + row0, args.lda, rest, args.a_cols - row0);
+                        const long long at = static_cast<long long>(k) + whole * 32;
+                        grouped_load_ragged(w_dst + whole * 4096, args.w + at * args.ldw + col0, args.ldw, rest, args.cols - col0);
 #pragma unroll
-                        for (int j = 0; j < L::kBRows / 128; ++j)
-                            grouped_load_ragged(b_dst + j * 16384 + whole * 4096, args.b + (static_cast<long long>(k) + whole * 32) * args.ldb + nb0 + j * 128,
-                                                args.ldb, rest, args.cols - nb0 - j * 128);
+                        for (int j = 0; j < kRBoxes; ++j)
+                            grouped_load_ragged(r_dst + j * 16384 + whole * 4096, args.r + at * args.ldr + row0 + j * 128, args.ldr, rest,
+                                                args.d_rows - row0 - j * 128);
                         ptx::fence_proxy_async_smem();
                         __syncwarp();
                     }
                     if (ptx::elect_one()) {
-                        const uint32_t bytes = whole * 4096 * (1 + L::kBRows / 128) * CTAS;
+                        const uint32_t bytes = whole * 4096 * (1 + kRBoxes) * CTAS;
                         if (rank != 0) { if (rest) ptx::mbar_arrive_cluster(ragged0 + 8 * s); }
                         else if (bytes) ptx::mbar_arrive_expect_tx(fullb, bytes);
                         else ptx::mbar_arrive(fullb);
                         for (int p = 0; p < whole; ++p) {
-                            load(a_dst + p * 4096, &maps.a[1], row0, k + p * 32, 0);
+                            load(w_dst + p * 4096, &maps.w32, col0, k + p * 32, 0);
 #pragma unroll
-                            for (int j = 0; j < L::kBRows / 128; ++j)
-                                load(b_dst + j * 16384 + p * 4096, &maps.b32, nb0 + j * 128, k + p * 32, 0);
+                            for (int j = 0; j < kRBoxes; ++j)
+                                load(r_dst + j * 16384 + p * 4096, &maps.r32, row0 + j * 128, k + p * 32, 0);
                         }
                     }
                 } else if (ptx::elect_one()) {
                     if (rank == 0) ptx::mbar_arrive_expect_tx(fullb, block_bytes * CTAS);
-                    if (kAMn) load(a_dst, &maps.a[3], row0, k, 0);
-                    else load(a_dst, &maps.a[box], k, row0, 0);
-                    if (!kBMn) load(b_dst, &maps.b, k, nb0, w.e);
-                    else {
+                    if (kWMn) load(w_dst, &maps.w, col0, k, MODE == kGroupedWgrad ? 0 : w.e);
+                    else load(w_dst, &maps.w, k, col0, w.e);
+                    if (kRMn) {
 #pragma unroll
-                        for (int j = 0; j < L::kBRows / 128; ++j)
-                            load(b_dst + j * 16384, &maps.b, nb0 + j * 128, k, MODE == kGroupedWgrad ? 0 : w.e);
+                        for (int j = 0; j < kRBoxes; ++j) load(r_dst + j * 16384, &maps.r[3], row0 + j * 128, k, 0);
+                    } else {
+                        load(r_dst, &maps.r[box], k, row0, 0);
+                        if (L::kRRows > 128 && boxes > 1) load(r_dst + 16384, &maps.r[3], k, row0 + 128, 0);
                     }
                 }
                 __syncwarp();
@@ -351,7 +355,8 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
                     break;
                 }
                 ptx::tc_fence_after();
-                const uint32_t d_tmem = tmem_base + slot * BN;
+                const uint32_t d_tmem = tmem_base + slot * ROWS;
+                const uint32_t idesc = args.idesc | (static_cast<uint32_t>((w.rows + kStep - 1) / kStep * kStep) >> 3) << 17;
                 for (int k = w.k0; k < w.k_end; k += kBlockK) {
                     if (!wait_bounded(bar_full + 8 * s, ph, abort_flag, kPair)) {
                         record_failure(args.status, abort_flag, kStatusMmaTimeout);
@@ -367,17 +372,16 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
                         ragged_ph ^= 1u << s;
                     }
                     ptx::tc_fence_after();
-                    const uint32_t a_src = smem_base + s * L::kStageBytes;
-                    const uint32_t b_src = a_src + L::kABytes;
-                    const uint64_t adesc = kAMn ? ptx::umma_desc_mn128(a_src, L::kABytes) : ptx::umma_desc_k128(a_src);
-                    const uint64_t bdesc = kBMn ? ptx::umma_desc_mn128(b_src, 16384) : ptx::umma_desc_k128(b_src);
+                    const uint32_t w_src = smem_base + s * L::kStageBytes;
+                    const uint32_t r_src = w_src + L::kWBytes;
+                    const uint64_t wdesc = kWMn ? ptx::umma_desc_mn128(w_src, 16384) : ptx::umma_desc_k128(w_src);
+                    const uint64_t rdesc = kRMn ? ptx::umma_desc_mn128(r_src, 16384) : ptx::umma_desc_k128(r_src);
                     const int steps = min(kBlockK / 32, (w.k_end - k + 31) / 32);
                     if (ptx::elect_one()) {
 #pragma unroll
                         for (int i = 0; i < kBlockK / 32; ++i)    // 32 of the contraction per instruction: 32 bytes or 32 rows
                             if (i < steps)
-                                ptx::umma_f8<CTAS>(d_tmem, adesc + (kAMn ? 256 : 2) * i, bdesc + (kBMn ? 256 : 2) * i, args.idesc,
-                                                   k != w.k0 || i != 0);
+                                ptx::umma_f8<CTAS>(d_tmem, wdesc + (kWMn ? 256 : 2) * i, rdesc + (kRMn ? 256 : 2) * i, idesc, k != w.k0 || i != 0);
                         if (kPair) ptx::umma_commit_pair(bar_empty + 8 * s, 0x3);
                         else ptx::umma_commit(bar_empty + 8 * s);
                     }
@@ -393,14 +397,11 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
             }
         }
     } else {
-        // ---------------- epilogue warps ----------------
+        // ---------------- epilogue warps: a lane owns a column, the registers run along the rows ----------------
         const int q = warp & 3;                                   // TMEM lane quarter this warp may read
-        const int grp = (warp - 2) >> 2;                          // 0 or 1: which half of the tile's columns
-        const uint32_t staging = smem_base + L::kEpiOff + (warp - 2) * L::kBuffers * L::kEpiBufBytes;
+        const int grp = (warp - 2) >> 2;                          // 0 or 1: every second chunk of 32 rows
         const uint32_t tempty0 = kPair ? ptx::mapa(bar_tempty, 0) : bar_tempty;
-        const bool issuer = ptx::elect_one();                    // this lane owns the warp's bulk-store groups
-        constexpr int kChunks = BN / 64;                          // 32-column chunks this warp drains per tile
-        constexpr int kChunksPerBox = L::kBoxCols / 32;
+        float* row_scales = reinterpret_cast<float*>(smem_gen + L::kScaleOff) + (warp - 2) * (ROWS / 2);
         const int out_dtype = args.epi.out_dtype;
         float alpha0 = args.epi.alpha, dscale = 1.0f, amax = 0.0f;
         if (args.epi.a_scale) alpha0 *= *args.epi.a_scale;
@@ -408,15 +409,25 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
         if (args.epi.d_scale) dscale = *args.epi.d_scale;
         // what few calls ask for sits behind one branch
         const bool more = args.epi.beta != 0.0f || args.epi.activation != 0 || args.epi.amax != nullptr || args.epi.d_scale != nullptr;
-        int box = 0;                                              // boxes stored so far: they take turns in the staging buffers
         int it = 0;
         Walk walk(args);
         GroupedTile w;
         for (long long t = first; walk.seek(t, w); t += step) {
             const bool empty = w.k0 >= w.k_end;
-            const int row0 = w.row0 + static_cast<int>(rank) * kTileM + q * 32;
-            const int rows = min(32, w.row_end - row0);          // rows of this warp's boxes to store (may be <= 0)
             const int slot = it & 1;
+            const int chunks = (w.rows + 31) / 32;
+            const int col = w.col0 + static_cast<int>(rank) * 128 + q * 32 + lane;
+            const bool have = col < args.cols;
+            const long long vec = static_cast<long long>(w.e) * args.cols + col;        // b_row_scale, bias: [E][cols]
+            float factor = alpha0, bias = 0.0f;
+            if (have && args.epi.b_row_scale != nullptr) factor *= __ldg(args.epi.b_row_scale + vec);
+            if (have && args.epi.bias != nullptr) bias = load_out(args.epi.bias, vec, args.epi.bias_dtype);
+            if (args.epi.a_row_scale != nullptr) {                // this warp's rows: chunk c at 16 c in its own array
+                __syncwarp();
+                for (int c = grp; c < chunks; c += 2)
+                    row_scales[(c >> 1) * 32 + lane] = c * 32 + lane < w.rows ? __ldg(args.epi.a_row_scale + w.row0 + c * 32 + lane) : 0.0f;
+                __syncwarp();
+            }
             if (!empty) {
                 if (!wait_bounded(bar_tfull + 8 * slot, static_cast<uint32_t>((it >> 1) & 1), abort_flag, kPair)) {
                     record_failure(args.status, abort_flag, kStatusEpilogueTimeout);
@@ -426,149 +437,88 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
                 ptx::tc_fence_after();
                 ++it;
             }
-            const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + slot * BN + grp * (BN / 2);
-            const long long d_base = MODE == kGroupedWgrad ? w.e * args.stride_d : 0;   // elements
-            const long long vec_base = static_cast<long long>(w.e) * args.cols;         // b_row_scale, bias: [E][cols]
-            const int z = MODE == kGroupedWgrad ? w.e : 0;
-            const float alpha = (args.epi.a_row_scale != nullptr && lane < rows) ? alpha0 * __ldg(args.epi.a_row_scale + row0 + lane) : alpha0;
+            const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + slot * ROWS;
+            const long long d_base = (MODE == kGroupedWgrad ? w.e * args.stride_d : 0) + static_cast<long long>(w.row0) * args.ldd;   // elements
 
-            // a box across a group's end must not reach the next group's rows: masked stores; a box across the end of D
-            // itself (wgrad: of D[e]) is clipped by the hardware
-            const bool by_tma = args.tma_store && (rows == 32 || (MODE == kGroupedWgrad && rows > 0));
-            auto scale = [&](uint32_t (&v)[32], int col0) {
-                if (args.epi.b_row_scale != nullptr) {
-                    const float mine = (col0 + lane < args.cols) ? __ldg(args.epi.b_row_scale + vec_base + col0 + lane) : 1.0f;
+            uint32_t v[32];
+#pragma unroll 1
+            for (int c = grp; c < chunks; c += 2) {
+                const int rows = min(32, w.rows - c * 32);
+                if (empty) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__shfl_sync(0xffffffffu, mine, i) * __uint_as_float(v[i]));
-                }
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(alpha * __uint_as_float(v[i]));
-                if (more && args.epi.beta != 0.0f && lane < rows) {
-                    const long long at = d_base + static_cast<long long>(row0 + lane) * args.ldd + col0;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (col0 + i < args.cols) v[i] = __float_as_uint(fmaf(args.epi.beta, load_out(args.d, at + i, out_dtype), __uint_as_float(v[i])));
-                }
-                if (args.epi.bias != nullptr) {
-                    const float mine = (col0 + lane < args.cols) ? load_out(args.epi.bias, vec_base + col0 + lane, args.epi.bias_dtype) : 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __shfl_sync(0xffffffffu, mine, i));
-                }
-                if (!more) return;
-                if (args.epi.activation == 1) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(relu(__uint_as_float(v[i])));
-                } else if (args.epi.activation == 2) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(gelu_erf(__uint_as_float(v[i])));
-                } else if (args.epi.activation == 3) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(gelu_tanh(__uint_as_float(v[i])));
-                }
-                if (args.epi.amax != nullptr && lane < rows) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (col0 + i < args.cols) amax = fmaxf(amax, fabsf(__uint_as_float(v[i])));
-                }
-                if (args.epi.d_scale != nullptr) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(dscale * __uint_as_float(v[i]));
-                }
-            };
-            // Chunk c in registers -> its box; `next` starts the load of the chunk behind it as soon as the registers are free.
-            auto emit = [&](uint32_t (&v)[32], int c, auto next) {
-                const int col0 = w.n0 + grp * (BN / 2) + c * 32;
-                const uint32_t sb = staging + (L::kBuffers == 2 ? (box & 1) * L::kEpiBufBytes : 0);
-                const int part = c % kChunksPerBox;
-                if (by_tma) {
-                    constexpr int kWords = 8 * OB;                // of this chunk per row
-                    uint32_t p[kWords];
-                    if constexpr (OB == 4) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) p[i] = v[i];
-                    } else if constexpr (OB == 2) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) p[i] = pack16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), out_dtype);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            p[i] = pack8(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]), out_dtype);
-                    }
-                    next();
-                    if (part == 0) {                              // the box that used this buffer before has been read
-                        if (issuer) ptx::bulk_wait_group_read<L::kBuffers - 1>();
-                        __syncwarp();
-                    }
-                    // rows of 128 bytes under the 128-byte swizzle, of 64 under the 64-byte one: no bank conflicts
-                    const uint32_t at = sb + lane * (L::kBoxCols * OB);
-                    const int swizzle = OB == 1 ? (lane >> 1) & 3 : lane & 7;
-#pragma unroll
-                    for (int i = 0; i < kWords / 4; ++i)
-                        ptx::st_shared_v4(at + (((part * (kWords / 4) + i) ^ swizzle) << 4), p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
-                    if (part == kChunksPerBox - 1) {
-                        ptx::fence_proxy_async_smem();
-                        __syncwarp();
-                        const int box0 = col0 - part * 32;
-                        if (issuer) {
-                            if (box0 < args.cols) ptx::tma_store_3d(&maps.d, sb, box0, row0, z);
-                            ptx::bulk_commit_group();
-                        }
-                        ++box;
-                    }
+                    for (int i = 0; i < 32; ++i) v[i] = 0u;
                 } else {
-                    if (issuer) ptx::bulk_wait_group_read<0>();
-                    __syncwarp();
-                    const uint32_t at = sb + lane * 128;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        ptx::st_shared_v4(at + ((i ^ (lane & 7)) << 4), v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                    next();
-                    __syncwarp();
-                    const int col = col0 + lane;                  // one instruction writes 32 elements of one row
-                    if (col < args.cols) {
-                        long long to = d_base + static_cast<long long>(row0) * args.ldd + col;
-                        for (int r = 0; r < rows; ++r, to += args.ldd) {
-                            const uint32_t bits = ptx::ld_shared_u32(sb + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2)));
-                            store_out(args.d, to, __uint_as_float(bits), out_dtype);
-                        }
-                    }
-                    __syncwarp();
+                    ptx::tmem_ld_32x32(t_addr + c * 32, v);
+                    ptx::tmem_ld_wait();
                 }
-            };
-
-            if (!empty && rows <= 0) {                            // nothing of this quarter belongs to the group
+                const long long at = d_base + static_cast<long long>(c) * 32 * args.ldd;
+                if (args.epi.a_row_scale != nullptr) {
+                    const float4* ra = reinterpret_cast<const float4*>(row_scales + (c >> 1) * 32);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 f = ra[i];                   // one address for all lanes
+                        v[4 * i] = __float_as_uint(__uint_as_float(v[4 * i]) * f.x);
+                        v[4 * i + 1] = __float_as_uint(__uint_as_float(v[4 * i + 1]) * f.y);
+                        v[4 * i + 2] = __float_as_uint(__uint_as_float(v[4 * i + 2]) * f.z);
+                        v[4 * i + 3] = __float_as_uint(__uint_as_float(v[4 * i + 3]) * f.w);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(fmaf(factor, __uint_as_float(v[i]), bias));
+                if (more) {
+                    if (args.epi.beta != 0.0f && have) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i < rows) v[i] = __float_as_uint(fmaf(args.epi.beta, load_out(args.d, at + i * args.ldd + col, out_dtype), __uint_as_float(v[i])));
+                    }
+                    if (args.epi.activation == 1) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(relu(__uint_as_float(v[i])));
+                    } else if (args.epi.activation == 2) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(gelu_erf(__uint_as_float(v[i])));
+                    } else if (args.epi.activation == 3) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(gelu_tanh(__uint_as_float(v[i])));
+                    }
+                    if (args.epi.amax != nullptr && have) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i < rows) amax = fmaxf(amax, fabsf(__uint_as_float(v[i])));
+                    }
+                    if (args.epi.d_scale != nullptr) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(dscale * __uint_as_float(v[i]));
+                    }
+                }
+                if (OB == 2 && args.packed_store) {
+                    // Two rows at a time: neighbouring lanes swap, so that an even lane holds its row's and its neighbour's
+                    // column of the first row and an odd one both of the second: 32-bit stores, 64 bytes of each row.
+                    const bool odd = lane & 1;
+                    uint16_t* to = static_cast<uint16_t*>(args.d) + at + (odd ? args.ldd : 0) + (col & ~1);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float give = __uint_as_float(odd ? v[i] : v[i + 1]);
+                        const float got = __shfl_xor_sync(0xffffffffu, give, 1);
+                        const uint32_t two = odd ? pack16(got, __uint_as_float(v[i + 1]), out_dtype) : pack16(__uint_as_float(v[i]), got, out_dtype);
+                        if (have && i + odd < rows) *reinterpret_cast<uint32_t*>(to) = two;
+                        to += 2 * args.ldd;
+                    }
+                } else if (have) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (i < rows) store_out(args.d, at + i * args.ldd + col, __uint_as_float(v[i]), OB == 4 ? 0 : out_dtype);
+                }
+            }
+            if (!empty) {                                         // this warp's part of the accumulator has been read
                 ptx::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
                     if (kPair) ptx::mbar_arrive_cluster(tempty0 + 8 * slot);
                     else ptx::mbar_arrive(bar_tempty + 8 * slot);
                 }
-                continue;
-            }
-            uint32_t v[32];
-            if (!empty) ptx::tmem_ld_32x32(t_addr, v);
-#pragma unroll 1
-            for (int c = 0; c < kChunks; ++c) {
-                if (empty) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = 0u;
-                } else {
-                    ptx::tmem_ld_wait();
-                    if (c == kChunks - 1) {                       // the accumulator's columns of this warp are in registers
-                        ptx::tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (kPair) ptx::mbar_arrive_cluster(tempty0 + 8 * slot);
-                            else ptx::mbar_arrive(bar_tempty + 8 * slot);
-                        }
-                    }
-                }
-                scale(v, w.n0 + grp * (BN / 2) + c * 32);
-                emit(v, c, [&]() { if (!empty && c + 1 < kChunks) ptx::tmem_ld_32x32(t_addr + (c + 1) * 32, v); });
             }
         }
-        // the staging box must outlive the stores' reads of it; the writes themselves complete with the grid
-        if (issuer) ptx::bulk_wait_group_read<0>();
         __syncwarp();
         if (args.epi.amax != nullptr) amax_merge_warp(args.epi.amax, amax);
     }

@@ -144,6 +144,9 @@ def test_quantize_rows_gathers_with_strides_and_padding(g):
 # ---- products grouped by expert --------------------------------------------------------------------------------------
 
 
+KERNELS = [0, 1, 2, 3, 7]      # automatic, one CTA with 256-, 128-row tiles, a pair, one CTA with 64-row tiles
+
+
 SIZES = {
     "one": [1], "few": [3, 0, 1, 17, 0, 40], "skewed": [0, 700, 2, 0, 129, 128, 127, 31, 33, 0, 1, 255], "all_empty": [0, 0, 0],
     "many": [(i * 7) % 19 for i in range(70)], "even": [256, 256, 512],
@@ -197,14 +200,16 @@ def operands(kind, sizes, slack, n, k, da, db, seed):
 
 
 def call(g, kind):
-    return {"forward": g.gemm_grouped, "dgrad": g.gemm_grouped_dgrad, "wgrad": g.gemm_grouped_wgrad}[kind]
+    f = {"forward": g.gemm_grouped, "dgrad": g.gemm_grouped_dgrad, "wgrad": g.gemm_grouped_wgrad}[kind]
+    # wgrad has no 64-row tiles
+    return f if kind != "wgrad" else lambda *args, kernel=0, **kw: f(*args, kernel=0 if kernel == 7 else kernel, **kw)
 
 
 def deepest(kind, sizes, n, k):
     return {"forward": k, "dgrad": n, "wgrad": max(sizes)}[kind]
 
 
-@pytest.mark.parametrize("kernel", [0, 1, 2, 3])
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("kind", ["forward", "dgrad", "wgrad"])
 @pytest.mark.parametrize("sizes", list(SIZES))
 @pytest.mark.parametrize("n,k", [(256, 128), (528, 400), (16, 1040), (1040, 16), (144, 272)])
@@ -224,7 +229,7 @@ def test_grouped_products_plain(g, kernel, kind, sizes, n, k):
 @pytest.mark.parametrize("db", [E4, E5])
 @pytest.mark.parametrize("kind", ["forward", "dgrad", "wgrad"])
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("kernel", [0, 1, 2, 3])
+@pytest.mark.parametrize("kernel", KERNELS)
 def test_grouped_products_types(g, da, db, kind, out, kernel):
     sizes, n, k = [130, 0, 300, 1], 272, 304
     a, b, shape = operands(kind, sizes, 0, n, k, da, db, 5)
@@ -237,7 +242,7 @@ def test_grouped_products_types(g, da, db, kind, out, kernel):
 
 @pytest.mark.parametrize("n", [1, 7, 33, 129, 250, 515])
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("kernel", [0, 1, 2, 3])
+@pytest.mark.parametrize("kernel", KERNELS)
 def test_grouped_forward_takes_any_number_of_columns(g, n, out, kernel):
     sizes, k = [3, 140, 0, 64], 144
     a, b, shape = operands("forward", sizes, 2, n, k, E4, E4, n)
@@ -251,7 +256,7 @@ def test_grouped_forward_takes_any_number_of_columns(g, n, out, kernel):
 
 
 @pytest.mark.parametrize("kind", ["forward", "dgrad", "wgrad"])
-@pytest.mark.parametrize("kernel", [0, 1, 2, 3])
+@pytest.mark.parametrize("kernel", KERNELS)
 def test_grouped_products_strides(g, kind, kernel):
     sizes, n, k = [70, 0, 33, 200], 160, 208
     a, b, shape = operands(kind, sizes, 4, n, k, E4, E4, 3)
@@ -284,7 +289,7 @@ def activation64(t, name):
 @pytest.mark.parametrize("kind", ["forward", "dgrad"])
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16, E4, E5])
-@pytest.mark.parametrize("kernel", [0, 1, 2, 3])
+@pytest.mark.parametrize("kernel", KERNELS)
 def test_grouped_epilogue(g, kind, act, out, kernel):
     sizes, n, k = [65, 0, 300, 31], 272, 240
     a, b, shape = operands(kind, sizes, 6, n, k, E4, E4, 11)
@@ -319,7 +324,7 @@ def test_grouped_epilogue(g, kind, act, out, kernel):
     assert abs(amax.item() - top) <= tol[:used].max().item() + 2.0 ** -22 * top
 
 
-@pytest.mark.parametrize("kernel", [0, 1, 2, 3])
+@pytest.mark.parametrize("kernel", KERNELS[:4])
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
 def test_wgrad_adds_to_what_is_there(g, kernel, out):
     sizes, n, k = [40, 0, 257, 3], 144, 272
@@ -339,7 +344,7 @@ def test_wgrad_adds_to_what_is_there(g, kernel, out):
 
 
 @pytest.mark.parametrize("kind", ["forward", "dgrad", "wgrad"])
-@pytest.mark.parametrize("kernel", [0, 1, 2, 3])
+@pytest.mark.parametrize("kernel", KERNELS)
 def test_other_groups_infinities_and_nans_stay_out(g, kind, kernel):
     """Every second group and the rows behind the last one hold NaN and infinities: the other groups' results are those of
     clean operands, bit for bit."""
@@ -364,7 +369,7 @@ def test_other_groups_infinities_and_nans_stay_out(g, kind, kernel):
 
 
 @pytest.mark.parametrize("kind", ["forward", "dgrad", "wgrad"])
-@pytest.mark.parametrize("kernel", [1, 3])
+@pytest.mark.parametrize("kernel", KERNELS[1:])
 def test_ends_are_clamped(g, kind, kernel):
     """Ends that fall or leave [0, rows] mean what their clamped running maximum means."""
     rows, n, k = 300, 144, 272
@@ -394,7 +399,7 @@ def test_grouped_forward_is_the_dense_operator_group_by_group(g):
     """The same kernel shape on each group's rows: same sums, same order, same bits."""
     sizes, n, k = [200, 1, 0, 640], 512, 1024
     a, b, shape = operands("forward", sizes, 0, n, k, E4, E4, 6)
-    for kernel in (1, 2, 3):
+    for kernel in (1, 2, 3, 7):
         d = torch.zeros(shape, device="cuda")
         g.gemm_grouped(a, b, d, ends_of(sizes), kernel=kernel)
         for e, lo, hi in spans(sizes):
