@@ -126,7 +126,7 @@ cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStre
     args.r = static_cast<const uint8_t*>(c.a); args.ldr = c.lda;
     args.status = dev.status;
     args.epi = c.epi;
-    args.packed_store = OB == 2 && args.cols % 2 == 0 && c.ldd % 2 == 0 && (!wgrad || c.stride_d % 2 == 0) && aligned(c.d, 4);
+    args.wide_store = OB == 2 && args.cols % 8 == 0 && c.ldd % 8 == 0 && (!wgrad || c.stride_d % 8 == 0) && aligned(c.d, 16);
 
     GroupedMaps maps;
     const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;

@@ -23,9 +23,12 @@
 //     pair), so a group's last tile costs what its rows cost: with 256-row tiles and groups of about a thousand rows,
 //     tiles of full height wasted an eighth of the multiplications (and, in a power-limited run, of the energy); a decode
 //     step's few rows per expert cost few bytes and cycles next to the weights (a tile loads the shortest of four boxes,
-//     16 to 128 rows, that covers them).  In the epilogue a lane owns one column, so the vectors per column (b_row_scale,
-//     bias) are one register, a warp's store of one row is contiguous, rows behind a group's end are simply not stored,
-//     and D needs neither staging nor TMA nor any alignment beyond its element.
+//     16 to 128 rows, that covers them).  In the epilogue a lane owns columns, so the vectors per column (b_row_scale,
+//     bias) are a few registers.  FP32 rows go out as they are, 128 bytes per instruction.  16-bit ones are read from TMEM
+//     in the matrix-fragment distribution, packed in pairs along the rows and transposed on the way through shared memory
+//     by stmatrix, then stored 16 bytes per lane (swapping columns between neighbouring lanes instead took four times the
+//     instructions, and the epilogue bounds products with a short contraction).  Rows behind a group's end are simply not
+//     stored, and D needs no TMA.
 //
 // Rows behind a group's end inside a tile belong to the next group.  Forward and dgrad may load and multiply them (each
 // row of a product depends on its own row of A only) and do not store them.  wgrad contracts over the rows, so the block
@@ -64,7 +67,7 @@ struct GroupedArgs {
     int col_tiles;
     int group_rows;       // tiles are walked down this many row tiles before the next column tile
     uint32_t idesc;       // without N
-    int packed_store;     // 16-bit D: two neighbouring columns can be stored as one 32-bit word
+    int wide_store;       // 16-bit D: eight neighbouring columns can be stored as 16 bytes
     void* d;
     long long ldd, stride_d;
     const uint8_t* w;     // wgrad: base pointers of the ragged rows' ordinary loads
@@ -164,9 +167,11 @@ struct GroupedSmem {
     static constexpr int kRBytes = kRRows * kBlockK;
     static constexpr int kStageBytes = kWBytes + kRBytes;
     static constexpr int kScaleBytes = kEpiWarps * ROWS / 2 * 4;             // row scales of a warp's rows
-    static constexpr int kStages = (227 * 1024 - 1024 - 384 - kScaleBytes) / kStageBytes;   // what is left is the ring
+    static constexpr int kTurnBytes = 32 * 64;                              // 32 rows x 32 columns of 16 bits, per epilogue warp
+    static constexpr int kStages = (227 * 1024 - 1024 - 384 - kScaleBytes - kEpiWarps * kTurnBytes) / kStageBytes;   // the rest is the ring
     static constexpr int kScaleOff = kStages * kStageBytes;
-    static constexpr int kBarOff = kScaleOff + kScaleBytes;
+    static constexpr int kTurnOff = kScaleOff + kScaleBytes;
+    static constexpr int kBarOff = kTurnOff + kEpiWarps * kTurnBytes;
     static constexpr int kNumBars = 3 * kStages + 4;                        // full[] empty[] tfull[2] tempty[2] ragged[]
     static constexpr int kTmemSlotOff = kBarOff + 8 * kNumBars;
     static constexpr int kAbortOff = kTmemSlotOff + 8;
@@ -401,6 +406,7 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
         const int q = warp & 3;                                   // TMEM lane quarter this warp may read
         const int grp = (warp - 2) >> 2;                          // 0 or 1: every second chunk of 32 rows
         const uint32_t tempty0 = kPair ? ptx::mapa(bar_tempty, 0) : bar_tempty;
+        const uint32_t turn = smem_base + L::kTurnOff + (warp - 2) * L::kTurnBytes;
         float* row_scales = reinterpret_cast<float*>(smem_gen + L::kScaleOff) + (warp - 2) * (ROWS / 2);
         const int out_dtype = args.epi.out_dtype;
         float alpha0 = args.epi.alpha, dscale = 1.0f, amax = 0.0f;
@@ -416,12 +422,19 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
             const bool empty = w.k0 >= w.k_end;
             const int slot = it & 1;
             const int chunks = (w.rows + 31) / 32;
-            const int col = w.col0 + static_cast<int>(rank) * 128 + q * 32 + lane;
-            const bool have = col < args.cols;
-            const long long vec = static_cast<long long>(w.e) * args.cols + col;        // b_row_scale, bias: [E][cols]
-            float factor = alpha0, bias = 0.0f;
-            if (have && args.epi.b_row_scale != nullptr) factor *= __ldg(args.epi.b_row_scale + vec);
-            if (have && args.epi.bias != nullptr) bias = load_out(args.epi.bias, vec, args.epi.bias_dtype);
+            const int col_base = w.col0 + static_cast<int>(rank) * 128 + q * 32;         // of this warp
+            // This lane's columns: one (col_base + lane), or four for 16-bit outputs (col_base + 8 m + lane / 4).
+            constexpr int kCols = OB == 2 ? 4 : 1;
+            auto col = [&](int m) { return OB == 2 ? col_base + 8 * m + (lane >> 2) : col_base + lane; };
+            float factor[kCols], bias[kCols];
+#pragma unroll
+            for (int m = 0; m < kCols; ++m) {
+                const long long vec = static_cast<long long>(w.e) * args.cols + col(m);  // b_row_scale, bias: [E][cols]
+                factor[m] = alpha0;
+                bias[m] = 0.0f;
+                if (col(m) < args.cols && args.epi.b_row_scale != nullptr) factor[m] *= __ldg(args.epi.b_row_scale + vec);
+                if (col(m) < args.cols && args.epi.bias != nullptr) bias[m] = load_out(args.epi.bias, vec, args.epi.bias_dtype);
+            }
             if (args.epi.a_row_scale != nullptr) {                // this warp's rows: chunk c at 16 c in its own array
                 __syncwarp();
                 for (int c = grp; c < chunks; c += 2)
@@ -440,6 +453,10 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
             const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + slot * ROWS;
             const long long d_base = (MODE == kGroupedWgrad ? w.e * args.stride_d : 0) + static_cast<long long>(w.row0) * args.ldd;   // elements
 
+            // Element i of a lane: its row within the chunk and which of its columns.  16-bit outputs: register 16 h + 4 j + 2 u + s
+            // is row 8 j + 2 (lane % 4) + s of column block 2 h + u.
+            auto row_of = [&](int i) { return OB == 2 ? 8 * ((i >> 2) & 3) + 2 * (lane & 3) + (i & 1) : i; };
+            auto block_of = [&](int i) { return OB == 2 ? 2 * (i >> 4) + ((i >> 1) & 1) : 0; };
             uint32_t v[32];
 #pragma unroll 1
             for (int c = grp; c < chunks; c += 2) {
@@ -448,28 +465,47 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = 0u;
                 } else {
-                    ptx::tmem_ld_32x32(t_addr + c * 32, v);
+                    if constexpr (OB == 2) {
+                        ptx::tmem_ld_16x32(t_addr + c * 32, v);
+                        ptx::tmem_ld_16x32(t_addr + (16u << 16) + c * 32, v + 16);
+                    } else {
+                        ptx::tmem_ld_32x32(t_addr + c * 32, v);
+                    }
                     ptx::tmem_ld_wait();
                 }
                 const long long at = d_base + static_cast<long long>(c) * 32 * args.ldd;
                 if (args.epi.a_row_scale != nullptr) {
-                    const float4* ra = reinterpret_cast<const float4*>(row_scales + (c >> 1) * 32);
+                    const float* ra = row_scales + (c >> 1) * 32;
+                    if constexpr (OB == 2) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float4 f = ra[i];                   // one address for all lanes
-                        v[4 * i] = __float_as_uint(__uint_as_float(v[4 * i]) * f.x);
-                        v[4 * i + 1] = __float_as_uint(__uint_as_float(v[4 * i + 1]) * f.y);
-                        v[4 * i + 2] = __float_as_uint(__uint_as_float(v[4 * i + 2]) * f.z);
-                        v[4 * i + 3] = __float_as_uint(__uint_as_float(v[4 * i + 3]) * f.w);
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 f = *reinterpret_cast<const float2*>(ra + 8 * j + 2 * (lane & 3));
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) {
+                                uint32_t* p = v + 16 * (m >> 1) + 4 * j + 2 * (m & 1);
+                                p[0] = __float_as_uint(__uint_as_float(p[0]) * f.x);
+                                p[1] = __float_as_uint(__uint_as_float(p[1]) * f.y);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float4 f = reinterpret_cast<const float4*>(ra)[i];   // one address for all lanes
+                            v[4 * i] = __float_as_uint(__uint_as_float(v[4 * i]) * f.x);
+                            v[4 * i + 1] = __float_as_uint(__uint_as_float(v[4 * i + 1]) * f.y);
+                            v[4 * i + 2] = __float_as_uint(__uint_as_float(v[4 * i + 2]) * f.z);
+                            v[4 * i + 3] = __float_as_uint(__uint_as_float(v[4 * i + 3]) * f.w);
+                        }
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(fmaf(factor, __uint_as_float(v[i]), bias));
+                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(fmaf(factor[block_of(i)], __uint_as_float(v[i]), bias[block_of(i)]));
                 if (more) {
-                    if (args.epi.beta != 0.0f && have) {
+                    if (args.epi.beta != 0.0f) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (i < rows) v[i] = __float_as_uint(fmaf(args.epi.beta, load_out(args.d, at + i * args.ldd + col, out_dtype), __uint_as_float(v[i])));
+                            if (row_of(i) < rows && col(block_of(i)) < args.cols)
+                                v[i] = __float_as_uint(fmaf(args.epi.beta, load_out(args.d, at + row_of(i) * args.ldd + col(block_of(i)), out_dtype), __uint_as_float(v[i])));
                     }
                     if (args.epi.activation == 1) {
 #pragma unroll
@@ -481,33 +517,51 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(gelu_tanh(__uint_as_float(v[i])));
                     }
-                    if (args.epi.amax != nullptr && have) {
+                    if (args.epi.amax != nullptr) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (i < rows) amax = fmaxf(amax, fabsf(__uint_as_float(v[i])));
+                            if (row_of(i) < rows && col(block_of(i)) < args.cols) amax = fmaxf(amax, fabsf(__uint_as_float(v[i])));
                     }
                     if (args.epi.d_scale != nullptr) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(dscale * __uint_as_float(v[i]));
                     }
                 }
-                if (OB == 2 && args.packed_store) {
-                    // Two rows at a time: neighbouring lanes swap, so that an even lane holds its row's and its neighbour's
-                    // column of the first row and an odd one both of the second: 32-bit stores, 64 bytes of each row.
-                    const bool odd = lane & 1;
-                    uint16_t* to = static_cast<uint16_t*>(args.d) + at + (odd ? args.ldd : 0) + (col & ~1);
+                if (OB == 2 && args.wide_store) {
+                    // rows of 64 bytes, 16-byte chunk ^ (row / 2) mod 4: neither side has bank conflicts
+                    __syncwarp();                                 // the chunk before has been read
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float give = __uint_as_float(odd ? v[i] : v[i + 1]);
-                        const float got = __shfl_xor_sync(0xffffffffu, give, 1);
-                        const uint32_t two = odd ? pack16(got, __uint_as_float(v[i + 1]), out_dtype) : pack16(__uint_as_float(v[i]), got, out_dtype);
-                        if (have && i + odd < rows) *reinterpret_cast<uint32_t*>(to) = two;
-                        to += 2 * args.ldd;
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t p[4];
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            const uint32_t* s = v + 16 * (m >> 1) + 4 * j + 2 * (m & 1);
+                            p[m] = pack16(__uint_as_float(s[0]), __uint_as_float(s[1]), out_dtype);
+                        }
+                        ptx::stmatrix_x4_trans(turn + 512 * j + (lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4), p[0], p[1], p[2], p[3]);
                     }
-                } else if (have) {
+                    __syncwarp();
+                    const int chunk = lane & 3;                   // eight columns
+                    const bool in = col_base + 8 * chunk < args.cols;
+                    char* to = reinterpret_cast<char*>(static_cast<uint16_t*>(args.d) + at + (lane >> 2) * args.ldd + col_base + 8 * chunk);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 8 * i + (lane >> 2);
+                        const uint4 two = ptx::ld_shared_v4(turn + r * 64 + ((chunk ^ ((r >> 1) & 3)) << 4));
+                        if (in && r < rows) *reinterpret_cast<uint4*>(to) = two;
+                        to += 16 * args.ldd;                      // eight rows, in bytes
+                    }
+                } else if (OB == 4 && rows == 32) {
+                    if (col_base + lane < args.cols) {
+                        float* to = static_cast<float*>(args.d) + at + col_base + lane;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i, to += args.ldd) *to = __uint_as_float(v[i]);
+                    }
+                } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
-                        if (i < rows) store_out(args.d, at + i * args.ldd + col, __uint_as_float(v[i]), OB == 4 ? 0 : out_dtype);
+                        if (row_of(i) < rows && col(block_of(i)) < args.cols)
+                            store_out(args.d, at + row_of(i) * args.ldd + col(block_of(i)), __uint_as_float(v[i]), OB == 4 ? 0 : out_dtype);
                 }
             }
             if (!empty) {                                         // this warp's part of the accumulator has been read
