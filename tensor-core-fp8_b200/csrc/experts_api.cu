@@ -4,6 +4,7 @@
 #include <atomic>
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdint>
 
 #include "../../include/b200fp8.h"
@@ -160,17 +161,34 @@ cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStre
                   CTAS, stream, maps, args);
 }
 
+// The automatic choice.  The sizes of the groups are known on the device only, so it goes by their average.
+int choose_grouped(int sm_count, int mode, const GroupedCall& c) {
+    const double experts = std::max(1, std::min(c.experts, c.rows)), average = c.rows / experts;
+    if (mode == kGroupedWgrad) {
+        // Tiles are of equal size and their contraction is the group.  With few rows per group the product is a store of D and
+        // twice as many CTAs store it faster; from about 600 on the pair's lower operand traffic decides (8 experts of
+        // 4096 x 4096: 74.9 us with one CTA, 93.6 with pairs at 48 rows; 89 / 103 at 400; 118.8 / 115.8 at 700).
+        if (c.n <= 128) return B200FP8_KERNEL_CTA1_N128;
+        return average >= 600 ? B200FP8_KERNEL_PAIR_N256 : B200FP8_KERNEL_CTA1_N256;
+    }
+    // Rounds of tiles that each shape needs (whole ones while they are few) times what a round costs: a round of 256 x 256 pair
+    // tiles takes about 1.3 times one of 128 x 128 tiles (one group of 256 rows, 8192 x 8192: 25.4 against 20.4 us in one round
+    // each; 400 rows: 27.6 in one round against 32.3 in two), one of 64-row tiles, with more of the weights in flight, 0.88
+    // (100 rows: 17.0 against 19.2 us).  256-row tiles of one CTA were never ahead by more than 3 %.
+    const double cols = mode == kGroupedForward ? c.n : c.k;
+    auto cost = [&](int tile_rows, int tile_cols, int units, double per_round) {
+        const double per_group = experts == 1 ? std::ceil(average / tile_rows) : 2 * average <= tile_rows ? 1.0 : average / tile_rows + 0.5;
+        const double rounds = experts * per_group * std::ceil(cols / tile_cols) / units;
+        return per_round * (rounds < 4 ? std::ceil(rounds) : rounds);
+    };
+    const double low = cost(64, 128, sm_count, 0.88), mid = cost(128, 128, sm_count, 1.0), pair = cost(256, 256, sm_count / 2, 1.3);
+    if (pair <= mid && pair <= low) return B200FP8_KERNEL_PAIR_N256;
+    return mid <= low ? B200FP8_KERNEL_CTA1_N128 : B200FP8_KERNEL_CTA1_N64;
+}
+
 template <int MODE, int OB>
 cudaError_t dispatch_grouped_to(const HostDevice& dev, const GroupedCall& c, int kernel, cudaStream_t stream) {
-    if (kernel == B200FP8_KERNEL_AUTO) {
-        const long long rows = MODE == kGroupedWgrad ? c.n : c.rows / std::max(1, c.experts);   // rows of D per group
-        const long long cols = MODE == kGroupedForward ? c.n : c.k;
-        const long long tiles = static_cast<long long>(c.experts) * ((rows + 255) / 256) * ((cols + 127) / 128);
-        kernel = rows >= 192 && cols > 128 && tiles >= 2LL * dev.sm_count ? B200FP8_KERNEL_PAIR_N256
-                 : rows > 64                                              ? B200FP8_KERNEL_CTA1_N128
-                 : MODE == kGroupedWgrad                                  ? B200FP8_KERNEL_CTA1_N128
-                                                                          : B200FP8_KERNEL_CTA1_N64;
-    }
+    if (kernel == B200FP8_KERNEL_AUTO) kernel = choose_grouped(dev.sm_count, MODE, c);
     switch (kernel) {
         case B200FP8_KERNEL_PAIR_N256: return launch_grouped<MODE, 256, 2, OB>(dev, c, stream);
         case B200FP8_KERNEL_CTA1_N256: return launch_grouped<MODE, 256, 1, OB>(dev, c, stream);
