@@ -291,12 +291,12 @@ cudaError_t launch_quantize(const HostDevice& dev, const QuantizeArgs& args, cud
     return launch(quantize_rows_kernel<BF16, Q, 512>, dev.pdl, dim3(rows, 1, 1), 512, 0, 1, stream, args);
 }
 
-template <bool BF16, int G, int NT, bool WIDE>
+template <bool BF16, int G, int NT, bool WIDE, bool INT>
 cudaError_t launch_w4(const HostDevice& dev, W4Args args, cudaStream_t stream) {
-    using L = W4Smem<NT>;
+    using L = W4Smem<NT, INT>;
     const int list_bytes = args.expert ? 4 * args.m : 0;
     const int bytes = L::kFixedBytes + list_bytes;
-    cudaError_t e = allow_smem<gemv_w4_kernel<BF16, G, NT, WIDE>>(L::kFixedBytes + 4 * kW4MostRows);
+    cudaError_t e = allow_smem<gemv_w4_kernel<BF16, G, NT, WIDE, INT>>(L::kFixedBytes + 4 * kW4MostRows);
     if (e != cudaSuccess) return e;
     const int slots = args.expert ? std::min(args.experts, args.m) : 1;
     const int tiles = (args.n + kW4TileRows - 1) / kW4TileRows;
@@ -312,7 +312,7 @@ cudaError_t launch_w4(const HostDevice& dev, W4Args args, cudaStream_t stream) {
     // all), so more of them lose (8192 x 8192, one vector: 25.3 / 16.5 / 15.0 / 21.9 us in 1 / 2 / 4 / 8 parts; 28672 x 8192, eight
     // vectors: 47 / 53 / 55 / 74)
     int splits = 1;
-    while (splits < 8 && 2 * splits <= units && static_cast<long long>(slots) * tiles * splits < (dev.sm_count * 3) / 2) splits *= 2;
+    while (splits < kW4MostSplits && 2 * splits <= units && static_cast<long long>(slots) * tiles * splits < (dev.sm_count * 3) / 2) splits *= 2;
     args.splits = splits;
     CUtensorMap map;
     const uint64_t experts = args.expert ? args.experts : 1;
@@ -320,18 +320,29 @@ cudaError_t launch_w4(const HostDevice& dev, W4Args args, cudaStream_t stream) {
                        experts > 1 ? args.code_stride : args.code_ld * static_cast<long long>(args.n), kW4BoxBytes, 16,
                        CU_TENSOR_MAP_SWIZZLE_128B)) != cudaSuccess)
         return e;
-    return launch(gemv_w4_kernel<BF16, G, NT, WIDE>, dev.pdl, dim3(splits, static_cast<unsigned>(tiles), static_cast<unsigned>(slots)), kW4Threads, bytes, splits,
+    return launch(gemv_w4_kernel<BF16, G, NT, WIDE, INT>, dev.pdl, dim3(splits, static_cast<unsigned>(tiles), static_cast<unsigned>(slots)), kW4Threads, bytes, splits,
                   stream, map, args);
+}
+
+template <bool BF16, int G, bool WIDE>
+cudaError_t launch_w4_form(const HostDevice& dev, const W4Args& args, cudaStream_t stream) {
+    // One or two vectors (a token's experts are different ones, so two tokens give an expert two rows at most) take the
+    // integer form: 8192 x 8192 with groups of 128 12.4 us against 14.4, 16384 x 16384 31.8 against 39.4; with groups of 32
+    // its work per group outweighs that for a short K (four experts of 1000 x 2048: 8.2 against 7.5 us).  Filling two tiles of
+    // columns with five vectors' digits lost to the FP16 form everywhere.
+    const int vectors = args.expert ? args.m / args.rows_per_x : args.m;
+    if (vectors <= 2 && (G > 32 || args.k >= 4096)) return launch_w4<BF16, G, 1, WIDE, true>(dev, args, stream);
+    // The FP16 form takes eight vectors to a pass, or sixteen.  By expert the number of rows that share an expert is known on
+    // the device only: their average.
+    const long long shared = args.expert ? args.experts : 1;
+    if (args.m <= 8 * shared) return launch_w4<BF16, G, 1, WIDE, false>(dev, args, stream);
+    return launch_w4<BF16, G, 2, WIDE, false>(dev, args, stream);
 }
 
 template <bool BF16, int G>
 cudaError_t launch_w4_group(const HostDevice& dev, const W4Args& args, cudaStream_t stream) {
-    // by expert most experts have at most eight rows (a decode step); where they have more on average, and for more than
-    // eight dense vectors, sixteen share a pass over the weights
-    const bool two = args.expert ? args.m > 8 * args.experts : args.m > 8;
-    const bool wide = args.scale_dtype == B200FP8_OUT_F32;
-    if (two) return wide ? launch_w4<BF16, G, 2, true>(dev, args, stream) : launch_w4<BF16, G, 2, false>(dev, args, stream);
-    return wide ? launch_w4<BF16, G, 1, true>(dev, args, stream) : launch_w4<BF16, G, 1, false>(dev, args, stream);
+    if (args.scale_dtype == B200FP8_OUT_F32) return launch_w4_form<BF16, G, true>(dev, args, stream);
+    return launch_w4_form<BF16, G, false>(dev, args, stream);
 }
 
 template <bool BF16>

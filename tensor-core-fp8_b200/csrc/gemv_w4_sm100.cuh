@@ -62,6 +62,7 @@ constexpr int kW4MostExperts = 4096;
 constexpr int kW4TileRows = 128;
 constexpr int kW4Warps = 8;
 constexpr int kW4Threads = 32 * kW4Warps;
+constexpr int kW4MostSplits = 8;         // portable cluster size
 constexpr int kW4Stages = 4;
 constexpr int kW4BoxBytes = 128;         // of codes per row and ring slot: 256 of K
 constexpr int kW4BoxK = 2 * kW4BoxBytes;
@@ -134,6 +135,87 @@ __device__ __forceinline__ uint4 w4_vector_piece(uint4 v, float& back) {
     }
 }
 
+// ---- the integer form --------------------------------------------------------------------------------------------------
+// A few vectors leave most of the instruction's eight columns empty, and unpacking codes to FP16 is what bounds the form
+// above.  Here an x becomes a whole number of 23 bits and a sign (scaled by a power of two per vector and 256 of K so that
+// the largest lies in [2^21, 2^22): what is rounded off is below FP32's rounding of a sum with that element), cut into three
+// signed bytes that take a column each.  The codes then go into m16n8k32 as bytes, two masks and a shift per eight, the
+// sums are exact integers (at most 128 * 15 * 128 in magnitude), z enters as z times the digits' sum over the group, and the
+// columns meet with weights 1, 256, 65536.  Two vectors fill a tile of eight columns.
+constexpr int kW4Magic = 0x4B400000;     // the FP32 number 3 * 2^22: adding a small integer to its bits adds it to its value
+
+template <bool FIRST>
+__device__ __forceinline__ void mma_16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (FIRST)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kW4Magic));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Eight consecutive x of one vector as digits d[0..2]: .x the even k's, .y the odd ones.  A whole warp calls it with 256
+// consecutive k; `back` undoes the scaling.  Numbers that are not finite count as zeros here (true is returned: see w4_special).
+template <bool BF16>
+__device__ __forceinline__ bool w4_digits(uint4 v, float& back, uint2 (&d)[3]) {
+    constexpr uint32_t kInfinite = BF16 ? 0x7F80u : 0x7C00u;
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t most = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = max(most, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+    most = __reduce_max_sync(0xffffffffu, most);
+    const bool bad = most >= kInfinite;
+    if (bad) {
+        most = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if ((w[i] & 0x7FFFu) >= kInfinite) w[i] &= 0xFFFF0000u;
+            if (((w[i] >> 16) & 0x7FFFu) >= kInfinite) w[i] &= 0xFFFFu;
+            most = max(most, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+    }
+    // exponent of the largest: |x| < 2^(e + 1); a subnormal FP16 number counts as the smallest exponent
+    const int e = BF16 ? static_cast<int>(most >> 7) - 127 : max(static_cast<int>(most >> 10), 1) - 15;
+    const int up = min(126, 21 - e);
+    const float forth = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+    back = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float2 f;
+        if constexpr (BF16) f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+        else f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        // the integer nearest to x * forth, plus 0x808080: its bytes are the balanced digits plus 128
+        u[2 * i] = __float_as_uint(fmaf(f.x, forth, 12582912.0f)) + (0x00808080u - kW4Magic);
+        u[2 * i + 1] = __float_as_uint(fmaf(f.y, forth, 12582912.0f)) + (0x00808080u - kW4Magic);
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const uint32_t pick = i | (4 + i) << 4;
+        d[i].x = __byte_perm(__byte_perm(u[0], u[2], pick), __byte_perm(u[4], u[6], pick), 0x5410) ^ 0x80808080u;
+        d[i].y = __byte_perm(__byte_perm(u[1], u[3], pick), __byte_perm(u[5], u[7], pick), 0x5410) ^ 0x80808080u;
+    }
+    return bad;
+}
+
+// What the infinities and NaNs of x[k0 .. k1) add to the product with one row of the weights (the other elements are skipped).
+template <bool BF16, int G>
+__device__ __noinline__ float w4_special(const uint8_t* codes, const void* scales, long long scale_at, int scale_dtype, const uint8_t* zeros,
+                                         const uint16_t* x, int k0, int k1) {
+    float sum = 0.0f;
+    for (int k = k0; k < k1; ++k) {
+        const uint32_t bits = x[k];
+        if ((bits & 0x7FFFu) < (BF16 ? 0x7F80u : 0x7C00u)) continue;
+        const uint32_t two = codes[k / 2];
+        const int c = k & 1 ? two >> 4 : two & 15u;
+        const int z = zeros ? zeros[k / G] & 15 : 8;
+        sum += static_cast<float>(c - z) * load_out(scales, scale_at + k / G, scale_dtype) *
+               (BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(bits))));
+    }
+    return sum;
+}
+
 // Four scales in a row from group `at` on (a multiple of four) as they are stored: FP32, or 16-bit ones two to a word.
 template <bool WIDE> struct W4Scales;
 template <> struct W4Scales<true> {
@@ -179,17 +261,19 @@ __device__ __forceinline__ uint32_t w4_zeros(const W4Args& args, const uint8_t* 
     return v;
 }
 
-template <int NT>
+template <int NT, bool INT>
 struct W4Smem {
-    static constexpr int kXK = 2048 / NT;                        // of K whose x is staged at a time
-    static constexpr int kXPitch = kXK * 2 + 64;                 // bytes; two vectors' lanes meet different banks
+    static constexpr int kVectors = INT ? 8 * NT / 3 : 8 * NT;   // of x that share a pass over the weights
+    static constexpr int kXK = INT ? 2048 : 2048 / NT;           // of K whose x is staged at a time
+    static constexpr int kXPitch = kXK * (INT ? 1 : 2) + 64;     // bytes; two columns' lanes meet different banks
     static constexpr int kPartPitch = kW4TileRows + 4;           // floats
     static constexpr int kXOff = kW4Warps * kW4Stages * kW4SlotBytes;
-    static constexpr int kBackOff = kXOff + 8 * NT * kXPitch;     // powers of two [blocks][vectors]
-    static constexpr int kPartOff = kBackOff + kXK / kW4BoxK * 8 * NT * 4;
+    static constexpr int kBackOff = kXOff + 8 * NT * kXPitch;     // powers of two [blocks][columns]
+    static constexpr int kSumOff = kBackOff + kXK / kW4BoxK * 8 * NT * 4;               // INT: digits' sums [groups][columns]
+    static constexpr int kPartOff = kSumOff + (INT ? kXK / 32 * 8 * NT * 4 : 0);
     static constexpr int kBarOff = kPartOff + 8 * NT * kPartPitch * 4;   // full[warp][stage], ready, done
-    static constexpr int kMiscOff = kBarOff + 8 * (kW4Warps * kW4Stages + 2);   // abort flag
-    static constexpr int kListOff = kMiscOff + 16;                       // by expert: rows of y (the call's row count)
+    static constexpr int kMiscOff = kBarOff + 8 * (kW4Warps * kW4Stages + 2);   // abort flag, vectors with numbers that are not finite
+    static constexpr int kListOff = kMiscOff + 48;                       // by expert: rows of y (the call's row count)
     static constexpr int kFixedBytes = kListOff + 1024;                  // with the slack for 1024-byte alignment
 };
 
@@ -217,11 +301,12 @@ __device__ __forceinline__ int w4_find_rows(const W4Args& args, int slot, int* l
     return count > 0 ? e : -1;
 }
 
-template <bool BF16, int G, int NT, bool WIDE>                     // WIDE: FP32 scales
+template <bool BF16, int G, int NT, bool WIDE, bool INT>           // WIDE: FP32 scales
 __global__ void __launch_bounds__(kW4Threads, 2)
 gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)      // codes [experts][N][K/2], box 128 bytes x 16 rows
 {
-    using L = W4Smem<NT>;
+    using L = W4Smem<NT, INT>;
+    static_assert(!INT || NT == 1, "the integer form has one tile of columns");
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_addr(smem_raw));
@@ -231,6 +316,7 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
     const uint32_t bar_ready = smem_base + L::kBarOff + 8 * kW4Warps * kW4Stages, bar_done = bar_ready + 8;
     const uint32_t ring = smem_base + warp * kW4Stages * kW4SlotBytes;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + L::kMiscOff);
+    volatile int* bad = reinterpret_cast<volatile int*>(smem_gen + L::kMiscOff + 8);   // [vector of the batch]
     int* list = reinterpret_cast<int*>(smem_gen + L::kListOff);
     const bool clustered = args.splits > 1;
 
@@ -258,7 +344,7 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
     const int units = (args.k_blocks + args.k_unit - 1) / args.k_unit;
     const int kb0 = static_cast<int>(static_cast<long long>(units) * split / args.splits) * args.k_unit;
     const int kb1 = min(args.k_blocks, static_cast<int>(static_cast<long long>(units) * (split + 1) / args.splits) * args.k_unit);
-    const int batches = (have + 8 * NT - 1) / (8 * NT);
+    const int batches = (have + L::kVectors - 1) / L::kVectors;
     int to_fill = batches * (kb1 - kb0);                         // blocks of this warp's rows still to be asked for
     int fill_kb = kb0;
     // one lane: the next block into slot s
@@ -304,7 +390,8 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
     uint32_t ph = 0, round = 0;
     bool ok = true;                                              // after a wait that ran out: no more waits, no more copies, and on to the end
     for (int b = 0; b < batches; ++b) {
-        const int m0 = b * 8 * NT, cols = min(8 * NT, have - m0);
+        const int m0 = b * L::kVectors, cols = min(L::kVectors, have - m0);   // vectors of this batch
+        if (INT && threadIdx.x < L::kVectors) bad[threadIdx.x] = 0;
         float y[NT][4];
 #pragma unroll
         for (int j = 0; j < NT; ++j) y[j][0] = y[j][1] = y[j][2] = y[j][3] = 0.0f;
@@ -318,9 +405,50 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
             constexpr int kBlocks = L::kXK / kW4BoxK;             // a chunk's: eight, or four
             const int block = warp % kBlocks;
             const int limit = kc == kb0 ? 8 * NT : cols;
-            if (kc + block < kend || kc == kb0) {
+            const int rest = lane % (4 * kWords);                 // piece within the group: lane rest / kWords's word rest % kWords
+            if (INT && (kc + block < kend || kc == kb0)) {
                 const int k = (kc + block) * kW4BoxK + lane * 8;
-                const int rest = lane % (4 * kWords), pos = lane - rest + rest % kWords * 4 + rest / kWords;   // within the group
+                const int word = (lane - rest) / 4 + rest % kWords;
+                const uint32_t to = smem_base + L::kXOff + block * kW4BoxK + (word >> 1) * 64 + rest / kWords * 16 + (word & 1) * 8;
+                float* sums = reinterpret_cast<float*>(smem_gen + L::kSumOff) + (block * kGroups + lane / (4 * kWords)) * 8 * NT;
+                float* backs = reinterpret_cast<float*>(smem_gen + L::kBackOff) + block * 8 * NT;
+                uint4 v[L::kVectors];
+#pragma unroll
+                for (int i = 0; i < L::kVectors; ++i) {
+                    v[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (i < cols && k < args.k && kc + block < kend) {
+                        const int row = args.expert ? list[m0 + i] / args.rows_per_x : m0 + i;
+                        v[i] = __ldg(reinterpret_cast<const uint4*>(args.x + row * args.ldx + k));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < L::kVectors; ++i) {
+                    if (i >= cols && kc != kb0) break;
+                    float back;
+                    uint2 d[3];
+                    if (w4_digits<BF16>(v[i], back, d)) bad[i] = 1;
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) {
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + (3 * i + q) * L::kXPitch), "r"(d[q].x), "r"(d[q].y) : "memory");
+                        int sum = __dp4a(static_cast<int>(d[q].x), 0x01010101, __dp4a(static_cast<int>(d[q].y), 0x01010101, 0));
+#pragma unroll
+                        for (int o = 1; o < 4 * kWords; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                        if (rest == 0) sums[3 * i + q] = static_cast<float>(sum);
+                        if (lane == 0) backs[3 * i + q] = back * (q == 0 ? 1.0f : q == 1 ? 256.0f : 65536.0f);
+                    }
+                }
+                if (kc == kb0) {
+#pragma unroll
+                    for (int i = 3 * L::kVectors; i < 8 * NT; ++i) {      // columns that no vector has
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(to + i * L::kXPitch), "r"(0u) : "memory");
+                        if (rest == 0) sums[i] = 0.0f;
+                        if (lane == 0) backs[i] = 0.0f;
+                    }
+                }
+            }
+            if (!INT && (kc + block < kend || kc == kb0)) {
+                const int k = (kc + block) * kW4BoxK + lane * 8;
+                const int pos = lane - rest + rest % kWords * 4 + rest / kWords;
                 const uint32_t to = smem_base + L::kXOff + (block * (kW4BoxK / 8) + pos) * 16;
                 for (int c0 = warp / kBlocks * 4; c0 < limit; c0 += 4 * NT) {
                     uint4 v[4];
@@ -384,9 +512,10 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
                 if (ok && to_fill > 0) fill(s);
                 __syncwarp();
                 if (++s == kW4Stages) { s = 0; ph ^= 1u; }
-                const uint32_t x_at = x_lane + (kb - kc) * (2 * kW4BoxK);
+                const uint32_t x_at = x_lane + (kb - kc) * (INT ? 1 : 2) * kW4BoxK;
                 float2 two_lo, two_hi;
                 uint32_t zl = 0x08080808u, zh = 0x08080808u;
+                uint4 digits[NT];
                 float ys[NT][4];                                  // this slot's sums, in the scaling of its x
 #pragma unroll
                 for (int j = 0; j < NT; ++j) ys[j][0] = ys[j][1] = ys[j][2] = ys[j][3] = 0.0f;
@@ -405,6 +534,35 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
                         zh = __shfl_sync(0xffffffffu, z_now[1], from);
                     }
                     const uint32_t place = kGroups == 2 ? (rel + i) & 3 : i & 3;
+                    if constexpr (INT) {
+                        int c[NT][4];
+#pragma unroll
+                        for (int w = i * kWords; w < (i + 1) * kWords; ++w) {
+                            const uint32_t le = lo[w] & 0x0F0F0F0Fu, lo4 = (lo[w] >> 4) & 0x0F0F0F0Fu;
+                            const uint32_t he = hi[w] & 0x0F0F0F0Fu, hi4 = (hi[w] >> 4) & 0x0F0F0F0Fu;
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) {
+                                if ((w & 1) == 0) digits[j] = ptx::ld_shared_v4(x_at + 8 * j * L::kXPitch + (w >> 1) * 64);   // two words'
+                                const uint32_t b0 = w & 1 ? digits[j].z : digits[j].x, b1 = w & 1 ? digits[j].w : digits[j].y;
+                                if (w == i * kWords) mma_16832<true>(c[j], le, he, lo4, hi4, b0, b1);
+                                else mma_16832<false>(c[j], le, he, lo4, hi4, b0, b1);
+                            }
+                        }
+                        // z as a number: its byte below the bits of 2^23
+                        const float zf_lo = __uint_as_float(__byte_perm(zl, 0x4B000000u, 0x7540u | place)) - 8388608.0f;
+                        const float zf_hi = __uint_as_float(__byte_perm(zh, 0x4B000000u, 0x7540u | place)) - 8388608.0f;
+                        const float* sums = reinterpret_cast<const float*>(smem_gen + L::kSumOff) + ((kb - kc) * kGroups + i) * 8 * NT + 2 * t;
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            const float2 d = *reinterpret_cast<const float2*>(sums + 8 * j);
+                            // exact: whole numbers below 2^24
+                            ys[j][0] = fmaf(cs_lo, fmaf(-zf_lo, d.x, __int_as_float(c[j][0])) - 12582912.0f, ys[j][0]);
+                            ys[j][1] = fmaf(cs_lo, fmaf(-zf_lo, d.y, __int_as_float(c[j][1])) - 12582912.0f, ys[j][1]);
+                            ys[j][2] = fmaf(cs_hi, fmaf(-zf_hi, d.x, __int_as_float(c[j][2])) - 12582912.0f, ys[j][2]);
+                            ys[j][3] = fmaf(cs_hi, fmaf(-zf_hi, d.y, __int_as_float(c[j][3])) - 12582912.0f, ys[j][3]);
+                        }
+                        continue;
+                    }
                     const __half2 m_lo = w4_minus(zl, place), m_hi = w4_minus(zh, place);
                     float c[NT][4];
 #pragma unroll
@@ -429,7 +587,7 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
                         sum[3] = fmaf(cs_hi, c[j][3], sum[3]);
                     }
                 }
-                if (BF16) {
+                if (BF16 || INT) {
                     const float* back = reinterpret_cast<const float*>(smem_gen + L::kBackOff) + (kb - kc) * 8 * NT + 2 * t;
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
@@ -442,12 +600,26 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
                 }
             }
         }
+        if constexpr (INT) {                                      // rare: infinities and NaNs in these vectors
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int column = 8 * j + 2 * t + (i & 1), vector = column / 3;
+                    if (vector < cols && column % 3 == 0 && bad[vector]) {
+                        const int row = args.expert ? list[m0 + vector] / args.rows_per_x : m0 + vector;
+                        y[j][i] += w4_special<BF16, G>(args.codes + e * args.code_stride + (i >> 1 ? n_hi : n_lo) * args.code_ld, args.scales,
+                                                       i >> 1 ? s_hi : s_lo, args.scale_dtype, i >> 1 ? z_hi : z_lo, args.x + row * args.ldx,
+                                                       kb0 * kW4BoxK, min(kb1 * kW4BoxK, args.k));
+                    }
+                }
+        }
         // the parts of K meet: every CTA lays its sums out in its shared memory and adds a share of the rows
         float* part = reinterpret_cast<float*>(smem_gen + L::kPartOff);
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[(8 * j + 2 * t + (i & 1)) * L::kPartPitch + (i >> 1 ? r_hi : r_lo)] = 1024.0f * y[j][i];   // see w4_unpack
+            for (int i = 0; i < 4; ++i) part[(8 * j + 2 * t + (i & 1)) * L::kPartPitch + (i >> 1 ? r_hi : r_lo)] = INT ? y[j][i] : 1024.0f * y[j][i];   // see w4_unpack
         if (clustered) {
             if (b == 0) ptx::cluster_wait();                     // every CTA of the cluster has its barriers
             __syncthreads();
@@ -461,11 +633,19 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
         for (int i = threadIdx.x; i < cols * share && ok; i += 32 * kW4Warps) {
             const int c = i / share, r = split * share + i - c * share;
             float sum = 0.0f;
-            if (clustered) {
-                const uint32_t at = part_addr + (c * L::kPartPitch + r) * 4;
-                for (int p = 0; p < args.splits; ++p) sum += __uint_as_float(ptx::ld_shared_cluster_u32(ptx::mapa(at, p)));
-            } else {
-                sum = part[c * L::kPartPitch + r];
+#pragma unroll
+            for (int q = 0; q < (INT ? 3 : 1); ++q) {
+                const int column = (INT ? 3 : 1) * c + q;
+                if (clustered) {
+                    const uint32_t at = part_addr + (column * L::kPartPitch + r) * 4;
+                    float v[kW4MostSplits];                       // all loads in flight, then added in the order of K
+#pragma unroll
+                    for (int p = 0; p < kW4MostSplits; ++p) v[p] = p < args.splits ? __uint_as_float(ptx::ld_shared_cluster_u32(ptx::mapa(at, p))) : 0.0f;
+#pragma unroll
+                    for (int p = 0; p < kW4MostSplits; ++p) sum += v[p];
+                } else {
+                    sum += part[column * L::kPartPitch + r];
+                }
             }
             if (n0 + r < args.n) store_out(args.y, static_cast<long long>(args.expert ? list[m0 + c] : m0 + c) * args.ldy + n0 + r, sum, args.y_dtype);
         }

@@ -469,7 +469,7 @@ def w4_close(y, w, x, k, dtype):
 @pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("zeros", [False, True])
-@pytest.mark.parametrize("m", [1, 2, 7, 8, 9, 16, 17, 40])
+@pytest.mark.parametrize("m", [1, 2, 3, 5, 6, 8, 9, 17, 40])
 @pytest.mark.parametrize("n,blocks", [(1, 1), (16, 2), (130, 3), (1000, 8), (515, 17)])
 def test_w4_products(g, x_dtype, group, zeros, m, n, blocks):
     k = group * blocks
@@ -525,6 +525,49 @@ def test_w4_special_values(g):
     done(g)
     assert (y[0, ::2] == 15.0 * k).all() and (y[0, 1::2] == 0).all()
     assert torch.isinf(y[1, ::2]).all() and torch.isnan(y[2]).all()
+
+
+@pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [1, 4, 7])
+def test_w4_infinities_and_nans_add_what_their_weights_say(g, x_dtype, m):
+    """inf and NaN in x times a weight of either sign or zero, in several vectors and blocks of K."""
+    n, k, group = 48, 2304, 64
+    codes, scales, z = weights((), n, k, group, torch.float16, 1, True)
+    x = torch.randn((m, k), generator=gen(9), device="cuda").to(x_dtype)
+    inf = float("inf")
+    x[0, 3], x[m - 1, 2303] = inf, -inf
+    x[m // 2, 700] = inf
+    y = torch.zeros((m, n), device="cuda")
+    g.gemv_w4(codes, scales, x, y, zeros=z)
+    done(g)
+    w = weights64(codes, scales, z)
+    want = (x.double()[:, None, :] * w[None]).sum(-1)
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.isinf(y), torch.isinf(want))
+    assert torch.equal(torch.sign(y[torch.isinf(y)]).double(), torch.sign(want[torch.isinf(want)]))
+
+
+@pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [1, 5, 8])
+def test_w4_vectors_of_any_size(g, x_dtype, m):
+    """Very large, very small and very uneven vectors: the scaling per vector and 256 of K loses nothing that FP32 sums keep."""
+    n, k, group = 64, 1024, 32
+    codes, scales, z = weights((), n, k, group, torch.float32, 1, True)
+    x = torch.randn((m, k), generator=gen(9), device="cuda").double()
+    e = 100.0 if x_dtype == torch.bfloat16 else 12.0
+    x *= torch.exp2(torch.linspace(-e, e, m, device="cuda").double().round())[:, None] if m > 1 else 2.0 ** e
+    x[:, 256:512] *= 2.0 ** -20
+    x[:, 512:768] = 0
+    x = x.to(x_dtype)
+    y = torch.zeros((m, n), device="cuda")
+    g.gemv_w4(codes, scales, x, y, zeros=z)
+    done(g)
+    w, v = weights64(codes, scales, z), x.double()
+    # on top of the sums' bound, a scaled element is off by at most 2^-23 of the largest of its 256: FP16's subnormals by far
+    # less, the integers' last bit by half of it
+    blocks = v.abs().unflatten(1, (-1, 256)).amax(-1, keepdim=True).expand(-1, -1, 256).flatten(1)
+    s = v.abs() @ w.abs().T
+    tol = (k / 16 + k / 32 + 8) * 2.0 ** -23 * s + 2.0 ** -23 * (blocks @ w.abs().T)
+    close(y, v @ w.T, tol, torch.float32)
 
 
 @pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float16])
