@@ -211,8 +211,11 @@ int b200fp8_spmv_bell_f32(int m, int k, const void* ell_values, int a_dtype, lon
  *
  * ld*: row pitches; stride_b / stride_d: pitch from one expert's matrix to the next (elements; not read for one expert).
  * Requirements: A and B 16-byte aligned; K, lda, ldb, stride_b and, in dgrad and wgrad, N multiples of 16; D aligned to its
- * element (16 bytes, and rows of a multiple of 16 bytes, for the fast store path).  options: kernel (AUTO, PAIR_N256,
- * CTA1_N256 or CTA1_N128) and max_ctas; depth and split_k must be 0.  Results do not depend on the kernel's schedule.
+ * element (16-bit outputs: 16 bytes, and rows of a multiple of 16 bytes, for the fast store path).  options: max_ctas and
+ * kernel, which here names the most rows of D per tile: PAIR_N256 (a CTA pair, 256 columns x 256 rows), CTA1_N256,
+ * CTA1_N128 and, not in wgrad, CTA1_N64 (one CTA, 128 columns), or AUTO (by the average group); depth and split_k must be
+ * 0.  The kernel is a matter of speed.  Outputs must not overlap inputs.  Nothing is allocated per call and no workspace
+ * is shared between calls, so calls on several streams, and graphs that hold them, may run at once.
  */
 int b200fp8_gemm_grouped(int experts, int rows, int k, int n, const int* ends, const void* a, int a_dtype, long long lda,
                          const void* b, int b_dtype, long long ldb, long long stride_b, void* d, int d_dtype, long long ldd,
@@ -247,7 +250,7 @@ int b200fp8_quantize_rows(int source_rows, int rows, int k, const void* x, int x
  * multiple of 16.  scales: N rows of K/group values of scale_dtype (B200FP8_OUT_F32, _BF16 or _F16); zeros: N rows of
  * K/group bytes (their low four bits), or NULL for 8 throughout.  group is 32, 64 or 128 and divides K.  x: BF16 or FP16,
  * 16-byte aligned, ldx a multiple of 8; y: x's type or FP32.  Sums are FP32, the products before them exact.  Made for
- * few vectors: weights are read once per sixteen of them.
+ * few vectors: weights are read once per sixteen of them.  An infinity or NaN in x counts as it does in the formula.
  *
  * b200fp8_gemv_w4_experts: row r of y takes the weights of expert[r] (DEVICE, int32) and row r / (rows / tokens) of x --
  * `rows` is a multiple of `tokens`, at most 4096; experts at most 4096.  A row whose expert lies outside [0, experts) is

@@ -507,6 +507,7 @@ cudaError_t host_device(HostDevice* out) {
     out->status = ctx->status;
     out->encode = g_encode;
     out->pdl = tune().pdl != 0;
+    out->debug = tune().debug & 512;
     return cudaSuccess;
 }
 void count_launch() { ++t_launches; }

@@ -17,7 +17,7 @@ namespace b200fp8 {
 namespace {
 
 constexpr int kDevices = 64;
-constexpr int kMaxRows = 1 << 30;
+constexpr int kMaxRows = 1 << 30;        // and columns: index arithmetic in 32 bits has room for a tile beyond them
 constexpr int kMaxExperts = 1 << 16;
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -126,6 +126,7 @@ cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStre
     args.w = static_cast<const uint8_t*>(w); args.ldw = c.ldb;
     args.r = static_cast<const uint8_t*>(c.a); args.ldr = c.lda;
     args.status = dev.status;
+    args.debug = dev.debug;
     args.epi = c.epi;
     args.wide_store = OB == 2 && args.cols % 8 == 0 && c.ldd % 8 == 0 && (!wgrad || c.stride_d % 8 == 0) && aligned(c.d, 16);
 
@@ -218,7 +219,7 @@ cudaError_t grouped(int mode, int experts, int rows, int k, int n, const int* en
     if (ep && ep->struct_bytes != static_cast<int>(sizeof(b200fp8_epilogue)) && ep->struct_bytes != B200FP8_EPILOGUE_V1_BYTES) return cudaErrorInvalidValue;
     const bool extended = ep && ep->struct_bytes == static_cast<int>(sizeof(b200fp8_epilogue));
     if (extended && (ep->activation < B200FP8_ACT_NONE || ep->activation > B200FP8_ACT_GELU_TANH)) return cudaErrorInvalidValue;
-    if (experts < 0 || rows < 0 || k <= 0 || n <= 0 || experts > kMaxExperts || rows > kMaxRows || !fp8(a_dtype) || !fp8(b_dtype)) return cudaErrorInvalidValue;
+    if (experts < 0 || rows < 0 || k <= 0 || n <= 0 || experts > kMaxExperts || rows > kMaxRows || k > kMaxRows || n > kMaxRows || !fp8(a_dtype) || !fp8(b_dtype)) return cudaErrorInvalidValue;
     if (d_dtype < B200FP8_OUT_F32 || d_dtype > B200FP8_OUT_E5M2) return cudaErrorInvalidValue;
     const bool wgrad = mode == kGroupedWgrad;
     if (ep && ep->bias && (ep->bias_dtype < B200FP8_OUT_F32 || ep->bias_dtype > B200FP8_OUT_F16 || !aligned(ep->bias, out_dtype_bytes(ep->bias_dtype)))) return cudaErrorInvalidValue;
@@ -300,9 +301,9 @@ cudaError_t launch_w4(const HostDevice& dev, W4Args args, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     const int slots = args.expert ? std::min(args.experts, args.m) : 1;
     const int tiles = (args.n + kW4TileRows - 1) / kW4TileRows;
-    if (tiles > 65535) return cudaErrorInvalidValue;             // N beyond 8 million
     args.k_blocks = (args.k + kW4BoxK - 1) / kW4BoxK;
     args.status = dev.status;
+    args.debug = dev.debug;
     args.k_unit = G == 128 ? 2 : 1;
     const int units = (args.k_blocks + args.k_unit - 1) / args.k_unit;
     const int scale_bytes = out_dtype_bytes(args.scale_dtype);
@@ -355,7 +356,7 @@ cudaError_t launch_w4_type(const HostDevice& dev, const W4Args& args, cudaStream
 }
 
 cudaError_t w4(const W4Args& args, int x_dtype, cudaStream_t stream) {
-    if (args.n < 0 || args.k <= 0 || args.m < 0 || args.code_ld > (1LL << 39) || args.code_stride > (1LL << 39)) return cudaErrorInvalidValue;
+    if (args.n < 0 || args.k <= 0 || args.m < 0 || args.n > 65535 * kW4TileRows || args.k > kMaxRows || args.m > kMaxRows || args.code_ld > (1LL << 39) || args.code_stride > (1LL << 39)) return cudaErrorInvalidValue;
     if (x_dtype != B200FP8_OUT_BF16 && x_dtype != B200FP8_OUT_F16) return cudaErrorInvalidValue;
     if (args.y_dtype != x_dtype && args.y_dtype != B200FP8_OUT_F32) return cudaErrorInvalidValue;
     if (args.scale_dtype < B200FP8_OUT_F32 || args.scale_dtype > B200FP8_OUT_F16) return cudaErrorInvalidValue;
@@ -406,7 +407,7 @@ int b200fp8_gemm_grouped_wgrad(int experts, int rows, int k, int n, const int* e
 
 int b200fp8_quantize_rows(int source_rows, int rows, int k, const void* x, int x_dtype, long long ldx, const int* index, void* q, int q_dtype,
                           long long ldq, float* scale, void* stream) {
-    if (source_rows < 0 || rows < 0 || k < 0 || !fp8(q_dtype) || (x_dtype != B200FP8_OUT_BF16 && x_dtype != B200FP8_OUT_F16)) return cudaErrorInvalidValue;
+    if (source_rows < 0 || rows < 0 || k < 0 || k > kMaxRows || !fp8(q_dtype) || (x_dtype != B200FP8_OUT_BF16 && x_dtype != B200FP8_OUT_F16)) return cudaErrorInvalidValue;
     if (ldx < k || ldq < k || (!index && rows > source_rows)) return cudaErrorInvalidValue;
     if (rows == 0) return cudaSuccess;
     if (!scale || !aligned(scale, 4) || !aligned(index, 4) || !aligned(x, 2)) return cudaErrorInvalidValue;

@@ -55,6 +55,7 @@ struct W4Args {
     int vector_scales, vector_zeros;   // four scales (zero points) of a row can be loaded at once
     int splits;            // parts of K = CTAs of a cluster
     int* status;
+    int debug;             // 512: the third slot of the first warp stays unloaded
 };
 
 constexpr int kW4MostRows = 4096;        // rows of y of one call by expert: their list is held in shared memory
@@ -345,11 +346,11 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
     const int kb0 = static_cast<int>(static_cast<long long>(units) * split / args.splits) * args.k_unit;
     const int kb1 = min(args.k_blocks, static_cast<int>(static_cast<long long>(units) * (split + 1) / args.splits) * args.k_unit);
     const int batches = (have + L::kVectors - 1) / L::kVectors;
-    int to_fill = batches * (kb1 - kb0);                         // blocks of this warp's rows still to be asked for
+    long long to_fill = static_cast<long long>(batches) * (kb1 - kb0);                         // blocks of this warp's rows still to be asked for
     int fill_kb = kb0;
     // one lane: the next block into slot s
     auto fill = [&](int s) {
-        if (ptx::elect_one()) {
+        if (!(args.debug && warp == 0 && fill_kb == kb0 + 2) && ptx::elect_one()) {
             ptx::mbar_arrive_expect_tx(bar_full + 8 * s, kW4SlotBytes);
             ptx::tma_load_3d(ring + s * kW4SlotBytes, &tmap, fill_kb * kW4BoxBytes, n0 + warp * 16, e, bar_full + 8 * s);
         }

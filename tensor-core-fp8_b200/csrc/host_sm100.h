@@ -12,6 +12,7 @@ struct HostDevice {
                        const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                        CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     bool pdl;         // launch with programmatic stream serialization
+    int debug;        // 512: a kernel leaves one block of its ring unloaded (exercises the bounded waits)
 };
 
 // state of the current device, made on its first use

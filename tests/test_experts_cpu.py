@@ -29,7 +29,8 @@ GROUPED = dict(experts=4, rows=64, k=128, n=256, ends=P, a=P, a_dtype=0, lda=256
 @pytest.mark.parametrize("bad", [dict(experts=-1), dict(rows=-1), dict(k=0), dict(n=0), dict(k=-16), dict(ends=None), dict(ends=ODD),
                                  dict(a=None), dict(a=ODD), dict(b=None), dict(b=ODD), dict(d=None), dict(d=ODD), dict(a_dtype=2),
                                  dict(b_dtype=-1), dict(d_dtype=5), dict(d_dtype=-1), dict(k=120), dict(lda=250), dict(ldb=136), dict(ldb=64),
-                                 dict(ldd=64), dict(experts=1 << 17), dict(rows=(1 << 30) + 1), dict(lda=1 << 62), dict(epilogue="size"),
+                                 dict(ldd=64), dict(experts=1 << 17), dict(rows=(1 << 30) + 1), dict(k=(1 << 30) + 16, lda=1 << 31, ldb=1 << 31, stride_b=1 << 38),
+                                 dict(n=(1 << 30) + 16, lda=1 << 31, ldd=1 << 31, stride_b=1 << 38), dict(lda=1 << 62), dict(epilogue="size"),
                                  dict(epilogue="activation"), dict(options="size"), dict(options="depth"), dict(options="split"),
                                  dict(options="kernel"), dict(options="ctas")])
 def test_grouped_products_refuse(pkg, entry, bad):
@@ -71,7 +72,7 @@ def test_grouped_products_refuse_what_only_one_of_them_refuses(pkg):
         assert lib.b200fp8_gemm_grouped_wgrad(4, 64, 128, 256, P, P, 0, 256, P, 0, 128, P, 0, 128, 256 * 128, ctypes.byref(ep), None, None) == INVALID
 
 
-@pytest.mark.parametrize("bad", [dict(source=-1), dict(rows=-1), dict(k=-1), dict(x_dtype=0), dict(x_dtype=3), dict(q_dtype=2), dict(ldx=63),
+@pytest.mark.parametrize("bad", [dict(source=-1), dict(rows=-1), dict(k=-1), dict(k=(1 << 30) + 1, ldx=1 << 31, ldq=1 << 31), dict(x_dtype=0), dict(x_dtype=3), dict(q_dtype=2), dict(ldx=63),
                                  dict(ldq=63), dict(rows=11), dict(scale=None), dict(scale=ODD), dict(x=None), dict(x=ODD), dict(q=None),
                                  dict(index=ODD)])
 def test_quantize_rows_refuses(pkg, bad):
@@ -85,7 +86,7 @@ W4 = dict(m=2, k=256, n=64, group=64, codes=P, code_ld=128, scales=P, scale_dtyp
           y_dtype=1, ldy=64)
 
 
-@pytest.mark.parametrize("bad", [dict(m=-1), dict(k=-64), dict(n=-1), dict(group=0), dict(group=48), dict(group=256), dict(k=224), dict(codes=None),
+@pytest.mark.parametrize("bad", [dict(m=-1), dict(k=-64), dict(k=0), dict(n=-1), dict(n=(1 << 23) + 1, ldy=1 << 24), dict(group=0), dict(group=48), dict(group=256), dict(k=224), dict(codes=None),
                                  dict(codes=ODD), dict(code_ld=112), dict(code_ld=136), dict(scales=None), dict(scales=ODD), dict(scale_dtype=3),
                                  dict(scale_ld=3), dict(zero_ld=3), dict(x=None), dict(x=ODD), dict(x_dtype=0), dict(ldx=248), dict(ldx=260),
                                  dict(y=None), dict(y=ODD), dict(y_dtype=2), dict(ldy=63)])

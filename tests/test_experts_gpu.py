@@ -7,6 +7,9 @@ bound, sum |a b|.  So a product is within (K / 32 + 8) * 2^-23 * S of the exact 
 terms' magnitudes), GELU 2e-6 relative / 1e-6 absolute of |t|, and the output's rounding is half a step of its type.
 FP8 outputs and the quantiser are compared value for value (or within one rounding of the two ends of the tolerance)."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -780,3 +783,54 @@ def test_offsets_beyond_32_bits(g):
     g.gemv_w4_experts(codes, scales, x, y, torch.tensor([159], dtype=torch.int32, device="cuda"))
     done(g)
     w4_close(y, weights64(codes[-1], scales[-1], None), x, k, torch.float32)
+
+
+# ---- a wait that runs out ---------------------------------------------------------------------------------------------
+
+
+CHILD = r"""
+import sys, time
+sys.path[:0] = [%r, %r]
+import torch
+import test_experts_gpu as T
+from __graft_entry__ import load_package
+g = load_package().gemm
+torch.cuda.set_device(0)
+
+
+def run(k):
+    a, b, shape = T.operands("forward", [300, 700], 0, 512, k, T.E4, T.E4, 1)
+    ends = T.ends_of([300, 700])
+    for kernel in (2, 3):
+        yield lambda: g.gemm_grouped(a, b, torch.zeros(shape, device="cuda"), ends, kernel=kernel), (101, 102, 103)
+    # wgrad contracts over the rows: 300 and 700 of them, or 100 and 200 where no block may be left out
+    few = T.ends_of([300, 700] if k > 256 else [100, 200])
+    for kernel in (1, 3):
+        yield lambda: g.gemm_grouped_wgrad(a, a, torch.zeros((2, k, k), device="cuda"), few, kernel=kernel), (101, 102, 103)
+    codes, scales, z = T.weights((), 512, 4 * k, 128, torch.float32, 1, True)
+    for m in (1, 8):
+        x = torch.ones((m, 4 * k), dtype=torch.bfloat16, device="cuda")
+        yield lambda: g.gemv_w4(codes, scales, x, torch.zeros((m, 512), device="cuda"), zeros=z), (106,)
+
+
+for call, codes in run(2048):
+    t0 = time.time()
+    call()
+    torch.cuda.synchronize()                      # must return: no hang, no CUDA error
+    status, seconds = g.device_status(reset=True), time.time() - t0
+    print("status", status, "seconds", round(seconds, 2), flush=True)
+    assert status in codes and seconds < 60, (status, seconds)
+for call, codes in run(256):                      # the context is intact: problems without a third block run through
+    call()
+    torch.cuda.synchronize()
+    assert g.device_status() == 0
+print("OK")
+"""
+
+
+def test_an_expired_wait_ends_the_kernels_with_a_status():
+    here = os.path.dirname(os.path.abspath(__file__))
+    res = subprocess.run([sys.executable, "-c", CHILD % (os.path.dirname(here), here)], env=dict(os.environ, B200FP8_DEBUG="512"), capture_output=True,
+                         text=True, timeout=600)
+    assert res.returncode == 0, res.stdout + res.stderr
+    assert "OK" in res.stdout
