@@ -412,6 +412,62 @@ def test_grouped_forward_is_the_dense_operator_group_by_group(g):
     done(g)
 
 
+@pytest.mark.parametrize("kind", ["forward", "dgrad", "wgrad"])
+@pytest.mark.parametrize("max_ctas", [1, 3, 40])
+def test_grouped_products_do_not_depend_on_the_grid_or_the_run(g, kind, max_ctas):
+    """A thousand groups, most of them small or empty, on few CTAs and on all: the same bits every time."""
+    rng = np.random.RandomState(5)
+    sizes = [int(v) for v in rng.poisson(1.5, 1000) * (rng.rand(1000) < 0.7)]
+    sizes[500] = 900
+    n, k = 80, 96
+    a, b, shape = operands(kind, sizes, 3, n, k, E4, E4, 8)
+    want = torch.full(shape, 2.0, dtype=torch.bfloat16, device="cuda")
+    call(g, kind)(a, b, want, ends_of(sizes), alpha=0.01)
+    for kernel in KERNELS:
+        d = torch.full(shape, 2.0, dtype=torch.bfloat16, device="cuda")
+        call(g, kind)(a, b, d, ends_of(sizes), alpha=0.01, kernel=kernel, max_ctas=max_ctas)
+        assert torch.equal(d, want), kernel
+    done(g)
+    t, s = product64(kind, a, b, sizes, shape)
+    close(want, t * 0.01, steps(900) * s * 0.01 + 2.0 ** -23 * s * 0.01, torch.bfloat16)
+
+
+@pytest.mark.parametrize("bias_dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("out", [torch.float16, torch.float32, E4])
+def test_grouped_bias_types_and_one_vector_at_a_time(g, bias_dtype, out):
+    sizes, n, k = [20, 0, 70], 136, 64
+    a, b, shape = operands("forward", sizes, 1, n, k, E4, E4, 2)
+    bias = torch.randn((3, n), generator=gen(3), device="cuda").to(bias_dtype)
+    rb = torch.rand((3, n), generator=gen(2), device="cuda") * 0.001
+    t, s = product64("forward", a, b, sizes, shape)
+    of = torch.cat([torch.full((hi - lo,), e, device="cuda") for e, lo, hi in spans(sizes)] + [torch.zeros(1, device="cuda")]).long()
+    for kw, want, scale in (({"bias": bias}, t / 1024 + bias.double()[of], 1 / 1024), ({"b_row_scale": rb}, t / 1024 * rb.double()[of], rb.double()[of] / 1024)):
+        d = torch.zeros(shape, device="cuda").to(out)
+        g.gemm_grouped(a, b, d, ends_of(sizes), alpha=1 / 1024, **kw)
+        done(g)
+        tol = steps(k) * s * scale + 2.0 ** -22 * torch.nan_to_num(want).abs()
+        if out in TOP:
+            lo, hi = (nearest8(want + sign * tol, out) for sign in (-1, 1))
+            have = d.double()
+            assert (((have >= lo) & (have <= hi)) | torch.isnan(want)).all()
+        else:
+            close(d, want, tol, out)
+
+
+@pytest.mark.parametrize("out", [E4, E5])
+def test_wgrad_to_fp8(g, out):
+    sizes, n, k = [33, 0, 200], 48, 112
+    a, b, shape = operands("wgrad", sizes, 0, n, k, E5, E4, 2)
+    d = torch.ones(shape, device="cuda").to(out)
+    g.gemm_grouped_wgrad(a, b, d, ends_of(sizes), alpha=2.0 ** -7, d_scale=torch.tensor([0.5], device="cuda"))
+    done(g)
+    t, s = product64("wgrad", a, b, sizes, shape)
+    lo, hi = (nearest8((t + sign * steps(200) * s) * 2.0 ** -8, out) for sign in (-1, 1))
+    have = d.double()
+    assert ((have >= lo) & (have <= hi)).all()
+    assert not d[1].float().any()
+
+
 @pytest.mark.parametrize("kind", ["dgrad", "wgrad"])
 def test_grouped_gradients_against_differences(g, kind):
     """A gradient's elements against the change of a scalar function of the forward product along FP8-exact steps."""
@@ -592,6 +648,31 @@ def test_w4_by_expert(g, x_dtype, group, zeros, tokens, top_k, experts, n, block
             w4_close(y[r:r + 1], weights64(codes[e], scales[e], None if z is None else z[e]), x[r // top_k:r // top_k + 1], k, x_dtype)
         else:
             assert (y[r] == 5.0).all()
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 20])
+def test_w4_by_expert_strides_and_repeats(g, tokens):
+    """Experts' matrices inside wider buffers; a token that names one expert twice; the same bits on every run."""
+    experts, n, k, group, top_k = 5, 70, 512, 64, 3
+    codes, scales, z = weights((experts,), n, k, group, torch.float32, 4, True)
+    def wide(t, rows, cols):
+        big = torch.full((experts, n + rows, t.shape[-1] + cols), 255, dtype=torch.uint8, device="cuda").to(t.dtype)
+        big[:, :n, :t.shape[-1]] = t
+        return big[:, :n, :t.shape[-1]]
+    x = torch.randn((tokens, k), generator=gen(9), device="cuda").half()
+    expert = torch.randint(0, experts, (tokens * top_k,), generator=gen(5), device="cuda", dtype=torch.int32)
+    expert[1] = expert[0]
+    buf = torch.full((tokens * top_k, n + 2), 5.0, dtype=torch.float16, device="cuda")
+    y = buf[:, :n]
+    g.gemv_w4_experts(wide(codes, 2, 16), wide(scales, 1, 3), x, y, expert, zeros=wide(z, 3, 5))
+    first = y.clone()
+    for _ in range(5):
+        g.gemv_w4_experts(codes, scales, x, y, expert, zeros=z)
+        assert torch.equal(y, first)
+    done(g)
+    assert torch.equal(y[0], y[1]) and (buf[:, n:] == 5.0).all()
+    for r, e in enumerate(expert.tolist()):
+        w4_close(y[r:r + 1], weights64(codes[e], scales[e], z[e]), x[r // top_k:r // top_k + 1], k, torch.float16)
 
 
 def test_w4_by_expert_at_its_limits(g):
