@@ -292,15 +292,15 @@ cudaError_t launch_quantize(const HostDevice& dev, const QuantizeArgs& args, cud
     return launch(quantize_rows_kernel<BF16, Q, 512>, dev.pdl, dim3(rows, 1, 1), 512, 0, 1, stream, args);
 }
 
-template <bool BF16, int G, int NT, bool WIDE, bool INT>
+template <bool BF16, int G, int NT, int RT, bool WIDE, bool INT>
 cudaError_t launch_w4(const HostDevice& dev, W4Args args, cudaStream_t stream) {
-    using L = W4Smem<NT, INT>;
+    using L = W4Smem<NT, RT, INT>;
     const int list_bytes = args.expert ? 4 * args.m : 0;
     const int bytes = L::kFixedBytes + list_bytes;
-    cudaError_t e = allow_smem<gemv_w4_kernel<BF16, G, NT, WIDE, INT>>(L::kFixedBytes + 4 * kW4MostRows);
+    cudaError_t e = allow_smem<gemv_w4_kernel<BF16, G, NT, RT, WIDE, INT>>(L::kFixedBytes + 4 * kW4MostRows);
     if (e != cudaSuccess) return e;
     const int slots = args.expert ? std::min(args.experts, args.m) : 1;
-    const int tiles = (args.n + kW4TileRows - 1) / kW4TileRows;
+    const int tiles = (args.n + L::kTileRows - 1) / L::kTileRows;
     args.k_blocks = (args.k + kW4BoxK - 1) / kW4BoxK;
     args.status = dev.status;
     args.debug = dev.debug;
@@ -318,10 +318,10 @@ cudaError_t launch_w4(const HostDevice& dev, W4Args args, cudaStream_t stream) {
     CUtensorMap map;
     const uint64_t experts = args.expert ? args.experts : 1;
     if ((e = encode_3d(dev, &map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, args.codes, args.k / 2, args.n, experts, args.code_ld,
-                       experts > 1 ? args.code_stride : args.code_ld * static_cast<long long>(args.n), kW4BoxBytes, 16,
+                       experts > 1 ? args.code_stride : args.code_ld * static_cast<long long>(args.n), kW4BoxBytes, 16 * RT,
                        CU_TENSOR_MAP_SWIZZLE_128B)) != cudaSuccess)
         return e;
-    return launch(gemv_w4_kernel<BF16, G, NT, WIDE, INT>, dev.pdl, dim3(splits, static_cast<unsigned>(tiles), static_cast<unsigned>(slots)), kW4Threads, bytes, splits,
+    return launch(gemv_w4_kernel<BF16, G, NT, RT, WIDE, INT>, dev.pdl, dim3(splits, static_cast<unsigned>(tiles), static_cast<unsigned>(slots)), kW4Threads, bytes, splits,
                   stream, map, args);
 }
 
@@ -332,12 +332,20 @@ cudaError_t launch_w4_form(const HostDevice& dev, const W4Args& args, cudaStream
     // its work per group outweighs that for a short K (four experts of 1000 x 2048: 8.2 against 7.5 us).  Filling two tiles of
     // columns with five vectors' digits lost to the FP16 form everywhere.
     const int vectors = args.expert ? args.m / args.rows_per_x : args.m;
-    if (vectors <= 2 && (G > 32 || args.k >= 4096)) return launch_w4<BF16, G, 1, WIDE, true>(dev, args, stream);
+    if (vectors <= 2 && (G > 32 || args.k >= 4096)) return launch_w4<BF16, G, 1, 1, WIDE, true>(dev, args, stream);
     // The FP16 form takes eight vectors to a pass, or sixteen.  By expert the number of rows that share an expert is known on
     // the device only: their average.
     const long long shared = args.expert ? args.experts : 1;
-    if (args.m <= 8 * shared) return launch_w4<BF16, G, 1, WIDE, false>(dev, args, stream);
-    return launch_w4<BF16, G, 2, WIDE, false>(dev, args, stream);
+    if (args.m <= 8 * shared) {
+        // With more CTAs than fit at once, half as many with 32 rows per warp stage x half as often and have twice the
+        // independent work per warp.  16 tokens, 8 of 64 experts each, groups of 128: 2048 x 4096 52.4 -> 44.8 us,
+        // 4096 x 1024 63.2 -> 48.7, 1024 x 1024 22.1 -> 16.9 (1.7 CTAs of 256 rows per SM); 4 of 32 experts, 1024 x 1024
+        // (0.9) 11.5 -> 13.3.
+        const long long blocks = static_cast<long long>(args.expert ? std::min(args.experts, args.m) : 1) * ((args.n + 255) / 256);
+        if (blocks > dev.sm_count) return launch_w4<BF16, G, 1, 2, WIDE, false>(dev, args, stream);
+        return launch_w4<BF16, G, 1, 1, WIDE, false>(dev, args, stream);
+    }
+    return launch_w4<BF16, G, 2, 1, WIDE, false>(dev, args, stream);
 }
 
 template <bool BF16, int G>
@@ -356,7 +364,7 @@ cudaError_t launch_w4_type(const HostDevice& dev, const W4Args& args, cudaStream
 }
 
 cudaError_t w4(const W4Args& args, int x_dtype, cudaStream_t stream) {
-    if (args.n < 0 || args.k <= 0 || args.m < 0 || args.n > 65535 * kW4TileRows || args.k > kMaxRows || args.m > kMaxRows || args.code_ld > (1LL << 39) || args.code_stride > (1LL << 39)) return cudaErrorInvalidValue;
+    if (args.n < 0 || args.k <= 0 || args.m < 0 || args.n > 65535 * 128 || args.k > kMaxRows || args.m > kMaxRows || args.code_ld > (1LL << 39) || args.code_stride > (1LL << 39)) return cudaErrorInvalidValue;
     if (x_dtype != B200FP8_OUT_BF16 && x_dtype != B200FP8_OUT_F16) return cudaErrorInvalidValue;
     if (args.y_dtype != x_dtype && args.y_dtype != B200FP8_OUT_F32) return cudaErrorInvalidValue;
     if (args.scale_dtype < B200FP8_OUT_F32 || args.scale_dtype > B200FP8_OUT_F16) return cudaErrorInvalidValue;

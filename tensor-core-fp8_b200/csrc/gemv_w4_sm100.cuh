@@ -18,11 +18,12 @@
 // instructions above take 9 per eight (a shift, four masks, four subtractions) plus the tensor core's one.  So the
 // kernel is about bytes in flight and few instructions:
 //
-//   * a CTA owns 128 rows of weights, 16 for each of eight warps, and a part of K; every warp streams the codes of its rows
-//     by TMA through a ring of its own ([16 rows][128 bytes] boxes under the 128-byte swizzle) and refills a slot as soon as
+//   * a CTA owns 128 rows of weights, 16 for each of eight warps (256 and 32 where there are many CTAs), and a part of K;
+//     every warp streams the codes of its rows by TMA through a ring of its own (boxes of 16 or 32 rows of 128 bytes under
+//     the 128-byte swizzle, 8 KB in flight) and refills a slot as soon as
 //     it has read it: no producer warp and no waiting for other warps; two CTAs per SM;
 //   * its part of x lies in shared memory, in the order in which the lanes want it;
-//   * the parts of K of one 128-row tile form a thread-block cluster and add their FP32 sums through distributed shared
+//   * the parts of K of one tile of rows form a thread-block cluster and add their FP32 sums through distributed shared
 //     memory in the order of K: no scratch in HBM, no atomics, one launch.
 //
 // By expert: row r of y takes the weights of expert[r] and row r / (rows / tokens) of x.  A block finds its rows by itself
@@ -60,14 +61,11 @@ struct W4Args {
 
 constexpr int kW4MostRows = 4096;        // rows of y of one call by expert: their list is held in shared memory
 constexpr int kW4MostExperts = 4096;
-constexpr int kW4TileRows = 128;
 constexpr int kW4Warps = 8;
 constexpr int kW4Threads = 32 * kW4Warps;
 constexpr int kW4MostSplits = 8;         // portable cluster size
-constexpr int kW4Stages = 4;
 constexpr int kW4BoxBytes = 128;         // of codes per row and ring slot: 256 of K
 constexpr int kW4BoxK = 2 * kW4BoxBytes;
-constexpr int kW4SlotBytes = 16 * kW4BoxBytes;
 constexpr int kStatusW4Timeout = 106;
 
 // c = a b (FIRST) or c += a b
@@ -262,18 +260,22 @@ __device__ __forceinline__ uint32_t w4_zeros(const W4Args& args, const uint8_t* 
     return v;
 }
 
-template <int NT, bool INT>
+// NT: tiles of eight columns; RT: tiles of 16 rows per warp
+template <int NT, int RT, bool INT>
 struct W4Smem {
+    static constexpr int kTileRows = 16 * RT * kW4Warps;         // rows of the weights per CTA
+    static constexpr int kSlotBytes = 16 * RT * kW4BoxBytes;
+    static constexpr int kStages = 4 / RT;                       // 8 KB in flight per warp
     static constexpr int kVectors = INT ? 8 * NT / 3 : 8 * NT;   // of x that share a pass over the weights
     static constexpr int kXK = INT ? 2048 : 2048 / NT;           // of K whose x is staged at a time
     static constexpr int kXPitch = kXK * (INT ? 1 : 2) + 64;     // bytes; two columns' lanes meet different banks
-    static constexpr int kPartPitch = kW4TileRows + 4;           // floats
-    static constexpr int kXOff = kW4Warps * kW4Stages * kW4SlotBytes;
+    static constexpr int kPartPitch = kTileRows + 4;           // floats
+    static constexpr int kXOff = kW4Warps * kStages * kSlotBytes;
     static constexpr int kBackOff = kXOff + 8 * NT * kXPitch;     // powers of two [blocks][columns]
     static constexpr int kSumOff = kBackOff + kXK / kW4BoxK * 8 * NT * 4;               // INT: digits' sums [groups][columns]
     static constexpr int kPartOff = kSumOff + (INT ? kXK / 32 * 8 * NT * 4 : 0);
     static constexpr int kBarOff = kPartOff + 8 * NT * kPartPitch * 4;   // full[warp][stage], ready, done
-    static constexpr int kMiscOff = kBarOff + 8 * (kW4Warps * kW4Stages + 2);   // abort flag, vectors with numbers that are not finite
+    static constexpr int kMiscOff = kBarOff + 8 * (kW4Warps * kStages + 2);   // abort flag, vectors with numbers that are not finite
     static constexpr int kListOff = kMiscOff + 48;                       // by expert: rows of y (the call's row count)
     static constexpr int kFixedBytes = kListOff + 1024;                  // with the slack for 1024-byte alignment
 };
@@ -302,20 +304,21 @@ __device__ __forceinline__ int w4_find_rows(const W4Args& args, int slot, int* l
     return count > 0 ? e : -1;
 }
 
-template <bool BF16, int G, int NT, bool WIDE, bool INT>           // WIDE: FP32 scales
+template <bool BF16, int G, int NT, int RT, bool WIDE, bool INT>           // WIDE: FP32 scales
 __global__ void __launch_bounds__(kW4Threads, 2)
-gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)      // codes [experts][N][K/2], box 128 bytes x 16 rows
+gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)      // codes [experts][N][K/2], box 128 bytes x 16 RT rows
 {
-    using L = W4Smem<NT, INT>;
-    static_assert(!INT || NT == 1, "the integer form has one tile of columns");
+    using L = W4Smem<NT, RT, INT>;
+    constexpr int kStages = L::kStages;
+    static_assert((!INT && RT == 1) || NT == 1, "the integer form and the one with two row tiles have one tile of columns");
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_addr(smem_raw));
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
     const int lane = threadIdx.x & 31;
-    const uint32_t bar_full = smem_base + L::kBarOff + warp * 8 * kW4Stages;     // this warp's
-    const uint32_t bar_ready = smem_base + L::kBarOff + 8 * kW4Warps * kW4Stages, bar_done = bar_ready + 8;
-    const uint32_t ring = smem_base + warp * kW4Stages * kW4SlotBytes;
+    const uint32_t bar_full = smem_base + L::kBarOff + warp * 8 * kStages;     // this warp's
+    const uint32_t bar_ready = smem_base + L::kBarOff + 8 * kW4Warps * kStages, bar_done = bar_ready + 8;
+    const uint32_t ring = smem_base + warp * kStages * L::kSlotBytes;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + L::kMiscOff);
     volatile int* bad = reinterpret_cast<volatile int*>(smem_gen + L::kMiscOff + 8);   // [vector of the batch]
     int* list = reinterpret_cast<int*>(smem_gen + L::kListOff);
@@ -323,7 +326,7 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
-        for (int s = 0; s < kW4Warps * kW4Stages; ++s) ptx::mbar_init(smem_base + L::kBarOff + 8 * s, 1);
+        for (int s = 0; s < kW4Warps * kStages; ++s) ptx::mbar_init(smem_base + L::kBarOff + 8 * s, 1);
         ptx::mbar_init(bar_ready, args.splits);
         ptx::mbar_init(bar_done, args.splits);
         ptx::fence_mbar_init();
@@ -340,7 +343,7 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
         if (clustered) ptx::cluster_wait();
         return;
     }
-    const int n0 = blockIdx.y * kW4TileRows;
+    const int n0 = blockIdx.y * L::kTileRows;
     const int split = blockIdx.x;
     const int units = (args.k_blocks + args.k_unit - 1) / args.k_unit;
     const int kb0 = static_cast<int>(static_cast<long long>(units) * split / args.splits) * args.k_unit;
@@ -351,13 +354,13 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
     // one lane: the next block into slot s
     auto fill = [&](int s) {
         if (!(args.debug && warp == 0 && fill_kb == kb0 + 2) && ptx::elect_one()) {
-            ptx::mbar_arrive_expect_tx(bar_full + 8 * s, kW4SlotBytes);
-            ptx::tma_load_3d(ring + s * kW4SlotBytes, &tmap, fill_kb * kW4BoxBytes, n0 + warp * 16, e, bar_full + 8 * s);
+            ptx::mbar_arrive_expect_tx(bar_full + 8 * s, L::kSlotBytes);
+            ptx::tma_load_3d(ring + s * L::kSlotBytes, &tmap, fill_kb * kW4BoxBytes, n0 + warp * 16 * RT, e, bar_full + 8 * s);
         }
         --to_fill;
         if (++fill_kb == kb1) fill_kb = kb0;
     };
-    for (int s = 0; s < kW4Stages && to_fill > 0; ++s) fill(s);
+    for (int s = 0; s < kStages && to_fill > 0; ++s) fill(s);
 
     constexpr int kGroups = kW4BoxK / G;                         // groups per ring slot: 2, 4 or 8
     constexpr int kWords = 8 / kGroups;                          // 32-bit words of codes per lane, row and group
@@ -366,26 +369,40 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
     // bank conflicts: the rows that one pass of a shared-memory read takes (two of 64 bytes, four of 32, eight of 16)
     // differ in the bits of the swizzle that the bytes of one row do not.
     const int row_of = G == 128 ? (g >> 1) | ((g & 1) << 2) : G == 64 ? (2 * g) % 8 + g / 4 : g;
-    const int r_lo = warp * 16 + row_of, r_hi = r_lo + 8;        // this lane's two rows of the tile
-    // 16-byte chunk ^ row mod 8, the same for both rows: the bits that depend on the lane; the others are xor'ed in
+    const int groups = args.k / G;
+    // this lane's rows: two in each tile of 16, eight apart
+    auto row = [&](int h, int i) { return warp * 16 * RT + 16 * h + 8 * i + row_of; };
+    auto row_n = [&](int h, int i) { return static_cast<long long>(min(n0 + row(h, i), args.n - 1)); };
+    auto scale_at = [&](int h, int i) { return e * args.scale_stride + row_n(h, i) * args.scale_ld; };
+    auto zero_at = [&](int h, int i) { return args.zeros + e * args.zero_stride + row_n(h, i) * args.zero_ld; };
+    // 16-byte chunk ^ row mod 8, the same for all its rows: the bits that depend on the lane; the others are xor'ed in
     const uint32_t lane_at = row_of * kW4BoxBytes + ((G == 128 ? t ^ row_of : G == 64 ? (t >> 1) ^ row_of : row_of) << 4) + (G == 64 ? (t & 1) * 8 : G == 32 ? t * 4 : 0);
     const uint32_t x_lane = smem_base + L::kXOff + g * L::kXPitch + t * 16;
-    const int groups = args.k / G;
-    const long long n_lo = min(n0 + r_lo, args.n - 1), n_hi = min(n0 + r_hi, args.n - 1);
-    const long long s_lo = e * args.scale_stride + n_lo * args.scale_ld, s_hi = e * args.scale_stride + n_hi * args.scale_ld;
-    const uint8_t* z_lo = args.zeros ? args.zeros + e * args.zero_stride + n_lo * args.zero_ld : nullptr;
-    const uint8_t* z_hi = args.zeros ? args.zeros + e * args.zero_stride + n_hi * args.zero_ld : nullptr;
     // Scales and zero points: the four lanes of a row hold those of 16 groups in a row, four each (a whole sector of
     // 16-bit scales), fetched 16 groups ahead and handed round by shuffles.  Fetched one by one, just before their use,
     // they bound the kernel: every load missed to HBM and kept the load unit busy with eight rows' lines.
-    W4Scales<WIDE> s_now[2], s_next[2];
-    uint32_t z_now[2], z_next[2] = {0x08080808u, 0x08080808u};
+    W4Scales<WIDE> s_now[RT][2], s_next[RT][2];
+    uint32_t z_now[RT][2], z_next[RT][2];
     const int g_first = kb0 * kGroups;
+    long long s_row[RT][2];
+    const uint8_t* z_row[RT][2];
+#pragma unroll
+    for (int h = 0; h < RT; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            s_row[h][i] = scale_at(h, i);
+            z_row[h][i] = args.zeros ? zero_at(h, i) : nullptr;
+            z_next[h][i] = 0x08080808u;
+        }
     auto fetch = [&](int window) {
         const int at = g_first + 16 * window + 4 * t;
-        s_next[0].load(args, s_lo, at, groups);
-        s_next[1].load(args, s_hi, at, groups);
-        if (z_lo) { z_next[0] = w4_zeros(args, z_lo, at, groups) & 0x0F0F0F0Fu; z_next[1] = w4_zeros(args, z_hi, at, groups) & 0x0F0F0F0Fu; }
+#pragma unroll
+        for (int h = 0; h < RT; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                s_next[h][i].load(args, s_row[h][i], at, groups);
+                if (args.zeros) z_next[h][i] = w4_zeros(args, z_row[h][i], at, groups) & 0x0F0F0F0Fu;
+            }
     };
     int s = 0;
     uint32_t ph = 0, round = 0;
@@ -393,9 +410,11 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
     for (int b = 0; b < batches; ++b) {
         const int m0 = b * L::kVectors, cols = min(L::kVectors, have - m0);   // vectors of this batch
         if (INT && threadIdx.x < L::kVectors) bad[threadIdx.x] = 0;
-        float y[NT][4];
+        float y[RT][NT][4];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) y[j][0] = y[j][1] = y[j][2] = y[j][3] = 0.0f;
+        for (int h = 0; h < RT; ++h)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) y[h][j][0] = y[h][j][1] = y[h][j][2] = y[h][j][3] = 0.0f;
         fetch(0);
         for (int kc = kb0; kc < kb1; kc += L::kXK / kW4BoxK) {
             const int kend = min(kb1, kc + L::kXK / kW4BoxK);
@@ -475,8 +494,10 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
             for (int kb = kc; kb < kend; ++kb) {
                 const int rel = (kb - kb0) * kGroups & 15;        // first group of the slot within its 16
                 if (rel == 0) {
-                    s_now[0] = s_next[0]; s_now[1] = s_next[1];
-                    z_now[0] = z_next[0]; z_now[1] = z_next[1];
+#pragma unroll
+                    for (int h = 0; h < RT; ++h)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) { s_now[h][i] = s_next[h][i]; z_now[h][i] = z_next[h][i]; }
                     if (kb + 16 / kGroups < kb1) fetch(((kb - kb0) * kGroups >> 4) + 1);
                 }
                 if (ok && !wait_bounded(bar_full + 8 * s, ph, abort_flag, false)) {
@@ -484,26 +505,30 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
                     ok = false;
                 }
                 __syncwarp();
-                const uint32_t at = ring + s * kW4SlotBytes + lane_at;
-                uint32_t lo[8], hi[8];
-                if constexpr (G == 128) {
+                const uint32_t at = ring + s * L::kSlotBytes + lane_at;
+                uint32_t lo[RT][8], hi[RT][8];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint4 a = ptx::ld_shared_v4(at ^ (i << 6)), c = ptx::ld_shared_v4((at ^ (i << 6)) + 8 * kW4BoxBytes);
-                        lo[4 * i] = a.x; lo[4 * i + 1] = a.y; lo[4 * i + 2] = a.z; lo[4 * i + 3] = a.w;
-                        hi[4 * i] = c.x; hi[4 * i + 1] = c.y; hi[4 * i + 2] = c.z; hi[4 * i + 3] = c.w;
-                    }
-                } else if constexpr (G == 64) {
+                for (int h = 0; h < RT; ++h) {
+                    const uint32_t from = at + h * 16 * kW4BoxBytes;
+                    if constexpr (G == 128) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(lo[2 * i]), "=r"(lo[2 * i + 1]) : "r"(at ^ (i << 5)) : "memory");
-                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2+1024];" : "=r"(hi[2 * i]), "=r"(hi[2 * i + 1]) : "r"(at ^ (i << 5)) : "memory");
-                    }
-                } else {
+                        for (int i = 0; i < 2; ++i) {
+                            const uint4 a = ptx::ld_shared_v4(from ^ (i << 6)), c = ptx::ld_shared_v4((from ^ (i << 6)) + 8 * kW4BoxBytes);
+                            lo[h][4 * i] = a.x; lo[h][4 * i + 1] = a.y; lo[h][4 * i + 2] = a.z; lo[h][4 * i + 3] = a.w;
+                            hi[h][4 * i] = c.x; hi[h][4 * i + 1] = c.y; hi[h][4 * i + 2] = c.z; hi[h][4 * i + 3] = c.w;
+                        }
+                    } else if constexpr (G == 64) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        lo[i] = ptx::ld_shared_u32(at ^ (i << 4));
-                        hi[i] = ptx::ld_shared_u32((at ^ (i << 4)) + 8 * kW4BoxBytes);
+                        for (int i = 0; i < 4; ++i) {
+                            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(lo[h][2 * i]), "=r"(lo[h][2 * i + 1]) : "r"(from ^ (i << 5)) : "memory");
+                            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2+1024];" : "=r"(hi[h][2 * i]), "=r"(hi[h][2 * i + 1]) : "r"(from ^ (i << 5)) : "memory");
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            lo[h][i] = ptx::ld_shared_u32(from ^ (i << 4));
+                            hi[h][i] = ptx::ld_shared_u32((from ^ (i << 4)) + 8 * kW4BoxBytes);
+                        }
                     }
                 }
                 // The slot may be refilled once these reads are done.  The refill is a write of another proxy (TMA), and nothing
@@ -512,80 +537,95 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
                 __syncwarp();
                 if (ok && to_fill > 0) fill(s);
                 __syncwarp();
-                if (++s == kW4Stages) { s = 0; ph ^= 1u; }
+                if (++s == kStages) { s = 0; ph ^= 1u; }
                 const uint32_t x_at = x_lane + (kb - kc) * (INT ? 1 : 2) * kW4BoxK;
-                float2 two_lo, two_hi;
-                uint32_t zl = 0x08080808u, zh = 0x08080808u;
+                float2 two[RT][2];                                // scales of two groups
+                uint32_t zeros[RT][2];                            // zero points of four groups
                 uint4 digits[NT];
-                float ys[NT][4];                                  // this slot's sums, in the scaling of its x
+                float ys[RT][NT][4];                              // this slot's sums, in the scaling of its x
 #pragma unroll
-                for (int j = 0; j < NT; ++j) ys[j][0] = ys[j][1] = ys[j][2] = ys[j][3] = 0.0f;
+                for (int h = 0; h < RT; ++h) {
+                    zeros[h][0] = zeros[h][1] = 0x08080808u;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) ys[h][j][0] = ys[h][j][1] = ys[h][j][2] = ys[h][j][3] = 0.0f;
+                }
 #pragma unroll
                 for (int i = 0; i < kGroups; ++i) {
                     // group rel + i of the 16: lane (rel + i) / 4 of the row holds it, at place (rel + i) % 4
                     const int from = (lane & ~3) | ((rel + i) >> 2);
-                    if ((i & 1) == 0) {
-                        const int p = ((kGroups == 2 ? rel : i) >> 1) & 1;
-                        two_lo = s_now[0].pair(p, from, args.scale_dtype);
-                        two_hi = s_now[1].pair(p, from, args.scale_dtype);
-                    }
-                    const float cs_lo = i & 1 ? two_lo.y : two_lo.x, cs_hi = i & 1 ? two_hi.y : two_hi.x;
-                    if (z_lo && (i & 3) == 0) {                  // four groups' zero points of this lane's rows
-                        zl = __shfl_sync(0xffffffffu, z_now[0], from);
-                        zh = __shfl_sync(0xffffffffu, z_now[1], from);
-                    }
+#pragma unroll
+                    for (int h = 0; h < RT; ++h)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            if ((i & 1) == 0) two[h][u] = s_now[h][u].pair(((kGroups == 2 ? rel : i) >> 1) & 1, from, args.scale_dtype);
+                            if (args.zeros && (i & 3) == 0) zeros[h][u] = __shfl_sync(0xffffffffu, z_now[h][u], from);
+                        }
+                    auto scale = [&](int h, int u) { return i & 1 ? two[h][u].y : two[h][u].x; };
                     const uint32_t place = kGroups == 2 ? (rel + i) & 3 : i & 3;
                     if constexpr (INT) {
-                        int c[NT][4];
+                        int c[RT][NT][4];
 #pragma unroll
                         for (int w = i * kWords; w < (i + 1) * kWords; ++w) {
-                            const uint32_t le = lo[w] & 0x0F0F0F0Fu, lo4 = (lo[w] >> 4) & 0x0F0F0F0Fu;
-                            const uint32_t he = hi[w] & 0x0F0F0F0Fu, hi4 = (hi[w] >> 4) & 0x0F0F0F0Fu;
 #pragma unroll
-                            for (int j = 0; j < NT; ++j) {
+                            for (int j = 0; j < NT; ++j)
                                 if ((w & 1) == 0) digits[j] = ptx::ld_shared_v4(x_at + 8 * j * L::kXPitch + (w >> 1) * 64);   // two words'
-                                const uint32_t b0 = w & 1 ? digits[j].z : digits[j].x, b1 = w & 1 ? digits[j].w : digits[j].y;
-                                if (w == i * kWords) mma_16832<true>(c[j], le, he, lo4, hi4, b0, b1);
-                                else mma_16832<false>(c[j], le, he, lo4, hi4, b0, b1);
+#pragma unroll
+                            for (int h = 0; h < RT; ++h) {
+                                const uint32_t le = lo[h][w] & 0x0F0F0F0Fu, lo4 = (lo[h][w] >> 4) & 0x0F0F0F0Fu;
+                                const uint32_t he = hi[h][w] & 0x0F0F0F0Fu, hi4 = (hi[h][w] >> 4) & 0x0F0F0F0Fu;
+#pragma unroll
+                                for (int j = 0; j < NT; ++j) {
+                                    const uint32_t b0 = w & 1 ? digits[j].z : digits[j].x, b1 = w & 1 ? digits[j].w : digits[j].y;
+                                    if (w == i * kWords) mma_16832<true>(c[h][j], le, he, lo4, hi4, b0, b1);
+                                    else mma_16832<false>(c[h][j], le, he, lo4, hi4, b0, b1);
+                                }
                             }
                         }
-                        // z as a number: its byte below the bits of 2^23
-                        const float zf_lo = __uint_as_float(__byte_perm(zl, 0x4B000000u, 0x7540u | place)) - 8388608.0f;
-                        const float zf_hi = __uint_as_float(__byte_perm(zh, 0x4B000000u, 0x7540u | place)) - 8388608.0f;
                         const float* sums = reinterpret_cast<const float*>(smem_gen + L::kSumOff) + ((kb - kc) * kGroups + i) * 8 * NT + 2 * t;
 #pragma unroll
                         for (int j = 0; j < NT; ++j) {
                             const float2 d = *reinterpret_cast<const float2*>(sums + 8 * j);
-                            // exact: whole numbers below 2^24
-                            ys[j][0] = fmaf(cs_lo, fmaf(-zf_lo, d.x, __int_as_float(c[j][0])) - 12582912.0f, ys[j][0]);
-                            ys[j][1] = fmaf(cs_lo, fmaf(-zf_lo, d.y, __int_as_float(c[j][1])) - 12582912.0f, ys[j][1]);
-                            ys[j][2] = fmaf(cs_hi, fmaf(-zf_hi, d.x, __int_as_float(c[j][2])) - 12582912.0f, ys[j][2]);
-                            ys[j][3] = fmaf(cs_hi, fmaf(-zf_hi, d.y, __int_as_float(c[j][3])) - 12582912.0f, ys[j][3]);
+#pragma unroll
+                            for (int h = 0; h < RT; ++h)
+#pragma unroll
+                                for (int u = 0; u < 2; ++u) {
+                                    // z as a number: its byte below the bits of 2^23; all exact: whole numbers below 2^24
+                                    const float z = __uint_as_float(__byte_perm(zeros[h][u], 0x4B000000u, 0x7540u | place)) - 8388608.0f;
+                                    ys[h][j][2 * u] = fmaf(scale(h, u), fmaf(-z, d.x, __int_as_float(c[h][j][2 * u])) - 12582912.0f, ys[h][j][2 * u]);
+                                    ys[h][j][2 * u + 1] = fmaf(scale(h, u), fmaf(-z, d.y, __int_as_float(c[h][j][2 * u + 1])) - 12582912.0f, ys[h][j][2 * u + 1]);
+                                }
                         }
-                        continue;
-                    }
-                    const __half2 m_lo = w4_minus(zl, place), m_hi = w4_minus(zh, place);
-                    float c[NT][4];
+                    } else {
+                        float c[RT][NT][4];
+                        __half2 minus[RT][2];
 #pragma unroll
-                    for (int w = i * kWords; w < (i + 1) * kWords; ++w) {
-                        uint32_t a[4], b[4];
-                        w4_unpack(lo[w], m_lo, a);
-                        w4_unpack(hi[w], m_hi, b);
+                        for (int h = 0; h < RT; ++h) { minus[h][0] = w4_minus(zeros[h][0], place); minus[h][1] = w4_minus(zeros[h][1], place); }
 #pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            const uint4 v = ptx::ld_shared_v4(x_at + 8 * j * L::kXPitch + w * 64);
-                            if (w == i * kWords) mma_16816<true>(c[j], a[0], b[0], a[1], b[1], v.x, v.y);
-                            else mma_16816<false>(c[j], a[0], b[0], a[1], b[1], v.x, v.y);
-                            mma_16816<false>(c[j], a[2], b[2], a[3], b[3], v.z, v.w);
+                        for (int w = i * kWords; w < (i + 1) * kWords; ++w) {
+                            uint4 v[NT];
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) v[j] = ptx::ld_shared_v4(x_at + 8 * j * L::kXPitch + w * 64);
+#pragma unroll
+                            for (int h = 0; h < RT; ++h) {
+                                uint32_t a[4], b[4];
+                                w4_unpack(lo[h][w], minus[h][0], a);
+                                w4_unpack(hi[h][w], minus[h][1], b);
+#pragma unroll
+                                for (int j = 0; j < NT; ++j) {
+                                    if (w == i * kWords) mma_16816<true>(c[h][j], a[0], b[0], a[1], b[1], v[j].x, v[j].y);
+                                    else mma_16816<false>(c[h][j], a[0], b[0], a[1], b[1], v[j].x, v[j].y);
+                                    mma_16816<false>(c[h][j], a[2], b[2], a[3], b[3], v[j].z, v[j].w);
+                                }
+                            }
                         }
-                    }
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        float* sum = BF16 ? ys[j] : y[j];
-                        sum[0] = fmaf(cs_lo, c[j][0], sum[0]);
-                        sum[1] = fmaf(cs_lo, c[j][1], sum[1]);
-                        sum[2] = fmaf(cs_hi, c[j][2], sum[2]);
-                        sum[3] = fmaf(cs_hi, c[j][3], sum[3]);
+                        for (int h = 0; h < RT; ++h)
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) {
+                                float* sum = BF16 ? ys[h][j] : y[h][j];
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) sum[q] = fmaf(scale(h, q >> 1), c[h][j][q], sum[q]);
+                            }
                     }
                 }
                 if (BF16 || INT) {
@@ -593,34 +633,36 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         const float2 p = *reinterpret_cast<const float2*>(back + 8 * j);
-                        y[j][0] = fmaf(p.x, ys[j][0], y[j][0]);
-                        y[j][1] = fmaf(p.y, ys[j][1], y[j][1]);
-                        y[j][2] = fmaf(p.x, ys[j][2], y[j][2]);
-                        y[j][3] = fmaf(p.y, ys[j][3], y[j][3]);
+#pragma unroll
+                        for (int h = 0; h < RT; ++h)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) y[h][j][q] = fmaf(q & 1 ? p.y : p.x, ys[h][j][q], y[h][j][q]);
                     }
                 }
             }
         }
         if constexpr (INT) {                                      // rare: infinities and NaNs in these vectors
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int h = 0; h < RT; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int column = 8 * j + 2 * t + (i & 1), vector = column / 3;
+                    const int column = 2 * t + (i & 1), vector = column / 3, u = i >> 1;
                     if (vector < cols && column % 3 == 0 && bad[vector]) {
-                        const int row = args.expert ? list[m0 + vector] / args.rows_per_x : m0 + vector;
-                        y[j][i] += w4_special<BF16, G>(args.codes + e * args.code_stride + (i >> 1 ? n_hi : n_lo) * args.code_ld, args.scales,
-                                                       i >> 1 ? s_hi : s_lo, args.scale_dtype, i >> 1 ? z_hi : z_lo, args.x + row * args.ldx,
-                                                       kb0 * kW4BoxK, min(kb1 * kW4BoxK, args.k));
+                        const int from = args.expert ? list[m0 + vector] / args.rows_per_x : m0 + vector;
+                        y[h][0][i] += w4_special<BF16, G>(args.codes + e * args.code_stride + row_n(h, u) * args.code_ld, args.scales, s_row[h][u],
+                                                          args.scale_dtype, z_row[h][u], args.x + from * args.ldx, kb0 * kW4BoxK, min(kb1 * kW4BoxK, args.k));
                     }
                 }
         }
         // the parts of K meet: every CTA lays its sums out in its shared memory and adds a share of the rows
         float* part = reinterpret_cast<float*>(smem_gen + L::kPartOff);
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int h = 0; h < RT; ++h)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[(8 * j + 2 * t + (i & 1)) * L::kPartPitch + (i >> 1 ? r_hi : r_lo)] = INT ? y[j][i] : 1024.0f * y[j][i];   // see w4_unpack
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    part[(8 * j + 2 * t + (i & 1)) * L::kPartPitch + row(h, i >> 1)] = INT ? y[h][j][i] : 1024.0f * y[h][j][i];   // see w4_unpack
         if (clustered) {
             if (b == 0) ptx::cluster_wait();                     // every CTA of the cluster has its barriers
             __syncthreads();
@@ -629,7 +671,7 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
         } else {
             __syncthreads();
         }
-        const int share = kW4TileRows / args.splits;
+        const int share = L::kTileRows / args.splits;
         const uint32_t part_addr = smem_base + L::kPartOff;
         for (int i = threadIdx.x; i < cols * share && ok; i += 32 * kW4Warps) {
             const int c = i / share, r = split * share + i - c * share;
@@ -658,10 +700,10 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
         ++round;
     }
     if (!ok && lane == 0) {                                       // leave no copy in flight into this CTA's shared memory
-        for (int i = 0; i < kW4Stages; ++i) {
+        for (int i = 0; i < kStages; ++i) {
             const uint64_t t0 = ptx::globaltimer_ns();
             while (!ptx::mbar_try_wait(bar_full + 8 * s, ph) && ptx::globaltimer_ns() - t0 < kWaitLimitNs / 8) {}
-            if (++s == kW4Stages) { s = 0; ph ^= 1u; }
+            if (++s == kStages) { s = 0; ph ^= 1u; }
         }
     }
     __syncwarp();

@@ -650,6 +650,42 @@ def test_w4_by_expert(g, x_dtype, group, zeros, tokens, top_k, experts, n, block
             assert (y[r] == 5.0).all()
 
 
+@pytest.mark.parametrize("x_dtype,scale_dtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+@pytest.mark.parametrize("experts,n,k", [(64, 700, 1408), (64, 1000, 256), (160, 17, 640)])
+def test_w4_by_expert_with_more_blocks_than_fit(g, x_dtype, scale_dtype, group, zeros, experts, n, k):
+    """The form with 32 rows per warp: with K parted and whole, experts with more than eight rows, odd ends of N and K."""
+    tokens, top_k = 20, 8
+    rows = tokens * top_k
+    codes, scales, z = weights((experts,), n, k, group, scale_dtype, n, zeros)
+    x = torch.randn((tokens, k), generator=gen(9), device="cuda").to(x_dtype)
+    x[3, 7], x[4] = float("inf"), 0.0
+    expert = torch.randint(0, experts, (rows,), generator=gen(5), device="cuda", dtype=torch.int32)
+    expert[5::14], expert[2] = 3, -1                          # a dozen for one expert, and a padding row
+    y = torch.full((rows, n), 5.0, dtype=x_dtype, device="cuda")
+    g.gemv_w4_experts(codes, scales, x, y, expert, zeros=z)
+    done(g)
+    for r, e in enumerate(expert.tolist()):
+        if e < 0:
+            assert (y[r] == 5.0).all()
+        elif r // top_k == 3:                                 # infinity times a weight: its sign, or NaN for a weight of zero
+            assert torch.equal(torch.nan_to_num(y[r].double(), nan=9.0, posinf=1.0, neginf=-1.0),
+                               torch.nan_to_num(x[3, 7].double() * weights64(codes[e], scales[e], None if z is None else z[e])[:, 7], nan=9.0, posinf=1.0, neginf=-1.0))
+        else:
+            w4_close(y[r:r + 1], weights64(codes[e], scales[e], None if z is None else z[e]), x[r // top_k:r // top_k + 1], k, x_dtype)
+
+
+@pytest.mark.parametrize("m", [4, 8])
+def test_w4_of_many_outputs(g, m):
+    n, k, group = 40001, 320, 64
+    codes, scales, z = weights((), n, k, group, torch.bfloat16, 3, True)
+    x = torch.randn((m, k), generator=gen(9), device="cuda").half()
+    y = torch.empty((m, n), device="cuda")
+    g.gemv_w4(codes, scales, x, y, zeros=z)
+    done(g)
+    w4_close(y, weights64(codes, scales, z), x, k, torch.float32)
+
+
 @pytest.mark.parametrize("tokens", [1, 3, 20])
 def test_w4_by_expert_strides_and_repeats(g, tokens):
     """Experts' matrices inside wider buffers; a token that names one expert twice; the same bits on every run."""
