@@ -175,7 +175,9 @@ int choose_grouped(int sm_count, int mode, const GroupedCall& c) {
     // Rounds of tiles that each shape needs (whole ones while they are few) times what a round costs: a round of 256 x 256 pair
     // tiles takes about 1.3 times one of 128 x 128 tiles (one group of 256 rows, 8192 x 8192: 25.4 against 20.4 us in one round
     // each; 400 rows: 27.6 in one round against 32.3 in two), one of 64-row tiles, with more of the weights in flight, 0.88
-    // (100 rows: 17.0 against 19.2 us).  256-row tiles of one CTA were never ahead by more than 3 %.
+    // (100 rows: 17.0 against 19.2 us).  A short contraction leaves the epilogue to decide, and 256-row tiles of one CTA keep it
+    // busier than pairs do (8 groups of 1000 rows, 4096 columns: 22.4 / 25.9 / 37.6 / 63.5 us against 28.1 / 31.6 / 37.9 / 56.4
+    // for depths of 128 / 512 / 1024 / 2048).
     const double cols = mode == kGroupedForward ? c.n : c.k;
     auto cost = [&](int tile_rows, int tile_cols, int units, double per_round) {
         const double per_group = experts == 1 ? std::ceil(average / tile_rows) : 2 * average <= tile_rows ? 1.0 : average / tile_rows + 0.5;
@@ -183,7 +185,8 @@ int choose_grouped(int sm_count, int mode, const GroupedCall& c) {
         return per_round * (rounds < 4 ? std::ceil(rounds) : rounds);
     };
     const double low = cost(64, 128, sm_count, 0.88), mid = cost(128, 128, sm_count, 1.0), pair = cost(256, 256, sm_count / 2, 1.3);
-    if (pair <= mid && pair <= low) return B200FP8_KERNEL_PAIR_N256;
+    const int depth = mode == kGroupedForward ? c.k : c.n;
+    if (pair <= mid && pair <= low) return depth < 1024 ? B200FP8_KERNEL_CTA1_N256 : B200FP8_KERNEL_PAIR_N256;
     return mid <= low ? B200FP8_KERNEL_CTA1_N128 : B200FP8_KERNEL_CTA1_N64;
 }
 
