@@ -2,7 +2,7 @@
 //
 //     m_r  = max(2^-80, max over the finite |x[i_r][k]|)          i_r = index[r], or r without an index
 //     s_r  = m_r / top                                            top = 448 (E4M3), 57344 (E5M2)
-//     q[r][k] = RNE(x[i_r][k] / m_r * top)                        infinities saturate, a NaN stays a NaN
+//     q[r][k] = RNE(x[i_r][k] * top / m_r)                        infinities saturate, a NaN stays a NaN
 //
 // so that q * s is the row again.  The operands of the row-scaled products (a_row_scale / b_row_scale) are made by it;
 // i_r outside the source is a row of zeros (the padding of a fixed-capacity expert).  The floor 2^-80 keeps s_r and its
@@ -12,6 +12,10 @@
 // conversion, so it is read once: 32, 128, 256 or 512 threads hold it, four 16-byte pieces each, all loads in flight at
 // once (rows of up to 1024, 4096, 8192 and 16384 elements; a row of up to 1024 is one warp's, without a barrier).  Longer
 // rows and rows that are not 16-byte aligned take the two-pass form at the end.
+//
+// Measured: 8192 rows of 4096 gathered into 16384 (134 MB each way counted once: 67 read, 67 written) 25.2 us in a graph, 5.3 TB/s,
+// 0.81 of a plain copy's rate; the two-pass form 150 us.  What is left is issue slots: about eight instructions per element
+// in the first form of the quotient, five with packed ones.  One row of 8192: 1.6 us in a graph.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
