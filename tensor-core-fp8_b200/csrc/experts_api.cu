@@ -282,17 +282,31 @@ cudaError_t grouped(int mode, int experts, int rows, int k, int n, const int* en
     }
 }
 
+template <bool BF16, int Q, int THREADS, int PIECES>
+cudaError_t launch_quantize_form(const HostDevice& dev, const QuantizeArgs& args, cudaStream_t stream) {
+    constexpr unsigned kRows = THREADS == 32 ? 4 : 1;             // of a block
+    return launch(quantize_rows_kernel<BF16, Q, THREADS, PIECES>, dev.pdl, dim3((static_cast<unsigned>(args.rows) + kRows - 1) / kRows, 1, 1),
+                  kRows * THREADS, 0, 1, stream, args);
+}
+
 template <bool BF16, int Q>
 cudaError_t launch_quantize(const HostDevice& dev, const QuantizeArgs& args, cudaStream_t stream) {
-    const unsigned rows = static_cast<unsigned>(args.rows);
-    const bool pieces = args.k % 8 == 0 && args.ldx % 8 == 0 && args.ldq % 8 == 0 && aligned(args.x, 16) && aligned(args.q, 8);
-    if (!pieces || args.k > 8 * kQuantizePieces * kQuantizeMostThreads)
-        return launch(quantize_rows_any_kernel<BF16>, dev.pdl, dim3(rows, 1, 1), 256, 0, 1, stream, args);
-    const int threads = (args.k + 8 * kQuantizePieces - 1) / (8 * kQuantizePieces);
-    if (threads <= 32) return launch(quantize_rows_kernel<BF16, Q, 32>, dev.pdl, dim3((rows + 3) / 4, 1, 1), 128, 0, 1, stream, args);
-    if (threads <= 128) return launch(quantize_rows_kernel<BF16, Q, 128>, dev.pdl, dim3(rows, 1, 1), 128, 0, 1, stream, args);
-    if (threads <= 256) return launch(quantize_rows_kernel<BF16, Q, 256>, dev.pdl, dim3(rows, 1, 1), 256, 0, 1, stream, args);
-    return launch(quantize_rows_kernel<BF16, Q, 512>, dev.pdl, dim3(rows, 1, 1), 512, 0, 1, stream, args);
+    const bool whole = args.k % 8 == 0 && args.ldx % 8 == 0 && args.ldq % 8 == 0 && aligned(args.x, 16) && aligned(args.q, 8);
+    const int pieces = (args.k + 7) / 8;
+    if (!whole || pieces > kQuantizeMostPieces)
+        return launch(quantize_rows_any_kernel<BF16>, dev.pdl, dim3(static_cast<unsigned>(args.rows), 1, 1), 256, 0, 1, stream, args);
+    // Many rows: few blocks with much to do each, since the GPU starts about one block per nanosecond and every thread that has a
+    // piece too few still takes its instructions (67 million elements, a row of 1040 by 128 threads 67.8 us, by one warp 31.3; 2080
+    // 35.5 / 26.8; 10240 by 512 threads 32.5, by 256 with six pieces 27.0).  Few rows: more threads finish one earlier (1040 elements
+    // 1.2 against 1.4 us).
+    if (pieces <= 128) return launch_quantize_form<BF16, Q, 32, 4>(dev, args, stream);
+    if (args.rows > 8 * dev.sm_count && pieces <= 256) return launch_quantize_form<BF16, Q, 32, 8>(dev, args, stream);
+    if (args.rows > 8 * dev.sm_count && pieces <= 384) return launch_quantize_form<BF16, Q, 32, 12>(dev, args, stream);
+    if (pieces <= 512) return launch_quantize_form<BF16, Q, 128, 4>(dev, args, stream);
+    if (pieces <= 768) return launch_quantize_form<BF16, Q, 128, 6>(dev, args, stream);
+    if (pieces <= 1024) return launch_quantize_form<BF16, Q, 256, 4>(dev, args, stream);
+    if (pieces <= 1536) return launch_quantize_form<BF16, Q, 256, 6>(dev, args, stream);
+    return launch_quantize_form<BF16, Q, 512, 4>(dev, args, stream);
 }
 
 template <bool BF16, int G, int NT, int RT, bool WIDE, bool INT>

@@ -9,13 +9,13 @@
 // reciprocal normal numbers for rows of zeros.
 //
 // Bound by HBM: 2 bytes read and 1 written per element.  A row stays in registers between the maximum and the
-// conversion, so it is read once: 32, 128, 256 or 512 threads hold it, four 16-byte pieces each, all loads in flight at
-// once (rows of up to 1024, 4096, 8192 and 16384 elements; a row of up to 1024 is one warp's, without a barrier).  Longer
-// rows and rows that are not 16-byte aligned take the two-pass form at the end.
+// conversion, so it is read once: one warp (four rows to a block, no barrier) or a block of 128 to 512 threads holds it, 4 to 12
+// 16-byte pieces per thread, all loads in flight at once.  Rows of more than 16384 elements and rows that are not 16-byte aligned
+// take the two-pass form at the end.
 //
-// Measured: 8192 rows of 4096 gathered into 16384 (134 MB each way counted once: 67 read, 67 written) 25.2 us in a graph, 5.3 TB/s,
-// 0.81 of a plain copy's rate; the two-pass form 150 us.  What is left is issue slots: about eight instructions per element
-// in the first form of the quotient, five with packed ones.  One row of 8192: 1.6 us in a graph.
+// Measured: 8192 rows of 4096 gathered into 16384 (67 MB read, 67 MB written) 25.2 us in a graph, 5.3 TB/s, 0.81 of a plain
+// copy's rate; the two-pass form 150 us.  What is left is issue slots, about eight instructions per element.  One row of 8192:
+// 1.6 us in a graph.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -40,8 +40,7 @@ struct QuantizeArgs {
 
 constexpr float kQuantizeLeast = 8.271806125530277e-25f;    // 2^-80
 
-constexpr int kQuantizePieces = 4;       // of eight elements per thread
-constexpr int kQuantizeMostThreads = 512;
+constexpr int kQuantizeMostPieces = 2048;                   // of eight elements: the longest row that a block holds in registers
 
 template <bool BF16>
 __device__ __forceinline__ float2 unpack16(uint32_t w) {
@@ -125,8 +124,8 @@ __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
     }
 }
 
-// THREADS == 32: four rows to a block of four warps; else one row to a block.
-template <bool BF16, int Q, int THREADS>
+// THREADS == 32: four rows to a block of four warps; else one row to a block.  PIECES of 16 bytes per thread.
+template <bool BF16, int Q, int THREADS, int PIECES>
 __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) quantize_rows_kernel(const QuantizeArgs args) {
     __shared__ float shared[THREADS / 32];
     ptx::griddep_wait();
@@ -138,15 +137,15 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) quantize_rows_k
     const int src = args.index ? __ldg(args.index + r) : static_cast<int>(r);
     const bool have = src >= 0 && src < args.source_rows;
     const uint4* x = reinterpret_cast<const uint4*>(args.x + static_cast<long long>(have ? src : 0) * args.ldx);
-    uint4 v[kQuantizePieces];
+    uint4 v[PIECES];
 #pragma unroll
-    for (int i = 0; i < kQuantizePieces; ++i) {
+    for (int i = 0; i < PIECES; ++i) {
         v[i] = make_uint4(0u, 0u, 0u, 0u);
         if (have && t + i * THREADS < pieces) v[i] = __ldg(x + t + i * THREADS);
     }
     uint32_t both = 0u;
 #pragma unroll
-    for (int i = 0; i < kQuantizePieces; ++i)
+    for (int i = 0; i < PIECES; ++i)
         both = max_abs2<BF16>(max_abs2<BF16>(max_abs2<BF16>(max_abs2<BF16>(both, v[i].x), v[i].y), v[i].z), v[i].w);
     const float2 two = unpack16<BF16>(both);
     auto across = [&](float m) {
@@ -158,7 +157,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) quantize_rows_k
     if (infinite) {                                               // rare: the largest finite magnitude, one element at a time
         float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kQuantizePieces; ++i) {
+        for (int i = 0; i < PIECES; ++i) {
             const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(finite_abs<BF16>(static_cast<uint16_t>(w[j])), finite_abs<BF16>(static_cast<uint16_t>(w[j] >> 16))));
@@ -171,7 +170,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) quantize_rows_k
     uint2* q = reinterpret_cast<uint2*>(args.q + r * args.ldq);
     auto convert = [&](auto value) {
 #pragma unroll
-        for (int i = 0; i < kQuantizePieces; ++i) {
+        for (int i = 0; i < PIECES; ++i) {
             if (t + i * THREADS >= pieces) break;
             const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
             uint32_t b[4];

@@ -128,6 +128,21 @@ def test_quantize_rows_special_values_and_ties(g, dtype, source):
     check_quantized(g, rows, dtype)
 
 
+@pytest.mark.parametrize("dtype,source", [(E4, torch.bfloat16), (E5, torch.float16)])
+@pytest.mark.parametrize("rows,k", [(1301, 1024), (1301, 1032), (1301, 2048), (1301, 2056), (1301, 3064), (1301, 3080), (1100, 1032), (33, 2056), (33, 4104),
+                                    (33, 6144), (33, 6152), (33, 8200), (33, 12288), (33, 12296), (33, 16384)])
+def test_quantize_rows_every_form(g, dtype, source, rows, k):
+    """Row lengths at both ends of every form, with gathered and padding rows, infinities and NaNs in the first and last pieces."""
+    x = torch.randn((rows, k), generator=gen(k), device="cuda").to(source)
+    x[3, k - 1], x[4, 0], x[5, k - 8], x[6] = float("inf"), float("nan"), -float("inf"), float("inf")
+    check_quantized(g, x, dtype)
+    index = torch.randint(0, rows, (rows,), generator=gen(2), device="cuda", dtype=torch.int32)
+    index[0], index[-1], index[7:11] = -1, rows, torch.tensor([3, 4, 5, 6], device="cuda")
+    buf = torch.full((rows, k + 24), 0x33, dtype=torch.uint8, device="cuda").view(dtype)
+    check_quantized(g, x, dtype, index, buf[:, :k])
+    assert (bytes_of(buf[:, k:]) == 0x33).all()
+
+
 def test_quantize_rows_gathers_with_strides_and_padding(g):
     wide = torch.randn((40, 1000), generator=gen(3), device="cuda").to(torch.bfloat16)
     for lo, k in ((0, 512), (8, 512), (3, 512), (16, 333)):
