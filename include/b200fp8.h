@@ -213,7 +213,7 @@ int b200fp8_spmv_bell_f32(int m, int k, const void* ell_values, int a_dtype, lon
  * Requirements: A and B 16-byte aligned; K, lda, ldb, stride_b and, in dgrad and wgrad, N multiples of 16; D aligned to its
  * element (16-bit outputs: 16 bytes, and rows of a multiple of 16 bytes, for the fast store path).  options: max_ctas and
  * kernel, which here names the most rows of D per tile: PAIR_N256 (a CTA pair, 256 columns x 256 rows), CTA1_N256,
- * CTA1_N128 and, not in wgrad, CTA1_N64 (one CTA, 128 columns), or AUTO (by the average group); depth and split_k must be
+ * CTA1_N128 and, not in wgrad, CTA1_N64 (one CTA, 128 columns), or AUTO (by the average group and the depth); depth and split_k must be
  * 0.  The kernel is a matter of speed.  Outputs must not overlap inputs.  Nothing is allocated per call and no workspace
  * is shared between calls, so calls on several streams, and graphs that hold them, may run at once.
  */
@@ -231,7 +231,7 @@ int b200fp8_gemm_grouped_wgrad(int experts, int rows, int k, int n, const int* e
  * Rows of 16-bit floats (x_dtype B200FP8_OUT_BF16 or _F16) to rows of 8-bit floats with one FP32 scale each, the operands
  * of the row-scaled products (a_row_scale, b_row_scale):
  *
- *     m = max(2^-80, largest finite |x[i][k]|),  scale[r] = m / top,  q[r][k] = nearest(x[i][k] / m * top)
+ *     m = max(2^-80, largest finite |x[i][k]|),  scale[r] = m / top,  q[r][k] = nearest(x[i][k] * top / m)
  *
  * with i = index[r] (r itself for index = NULL) and top = 448 (E4M3) or 57344 (E5M2); nearest is round-to-nearest-even of
  * the exact quotient.  Infinities become +-top, a NaN stays a NaN.  index (DEVICE, int32) copies rows into the experts'
