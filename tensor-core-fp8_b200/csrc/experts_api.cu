@@ -226,7 +226,8 @@ cudaError_t grouped(int mode, int experts, int rows, int k, int n, const int* en
     if (d_dtype < B200FP8_OUT_F32 || d_dtype > B200FP8_OUT_E5M2) return cudaErrorInvalidValue;
     const bool wgrad = mode == kGroupedWgrad;
     if (ep && ep->bias && (ep->bias_dtype < B200FP8_OUT_F32 || ep->bias_dtype > B200FP8_OUT_F16 || !aligned(ep->bias, out_dtype_bytes(ep->bias_dtype)))) return cudaErrorInvalidValue;
-    if (ep && !aligned(ep->amax_d, 4)) return cudaErrorInvalidValue;
+    if (ep && (!aligned(ep->amax_d, 4) || !aligned(ep->a_scale, 4) || !aligned(ep->b_scale, 4) || !aligned(ep->d_scale, 4))) return cudaErrorInvalidValue;
+    if (extended && (!aligned(ep->a_row_scale, 4) || !aligned(ep->b_row_scale, 4))) return cudaErrorInvalidValue;
     // a bias, an activation or a scale of one row has no place in a sum over the rows
     if (wgrad && ep && (ep->bias || (extended && (ep->activation || ep->a_row_scale || ep->b_row_scale)))) return cudaErrorInvalidValue;
     const long long a_cols = mode == kGroupedForward ? k : n, d_cols = mode == kGroupedForward ? n : k;

@@ -134,6 +134,10 @@ def _grouped(what, a, b, d, ends, experts, rows, n, k, a_cols, cols, alpha, beta
     lda, ldb, ldd = _pitch("a", a, F8, a_cols), _pitch("b", b, F8, k), _pitch("d", d, OUT, cols)
     device = _device(d, a, b, ends, a_scale, b_scale, d_scale, amax_d, bias, a_row_scale, b_row_scale)
     if experts == 0 or n == 0 or k == 0:
+        if experts and rows and cols and what != "gemm_grouped_wgrad":
+            raise ValueError(f"{what}: the contraction has no extent, a is {list(a.shape)}")
+        if amax_d is not None:
+            amax_d.zero_()
         return d
     if what == "gemm_grouped_wgrad":
         _call(device, what, experts, rows, k, n, first_row, a.data_ptr(), F8[a.dtype], lda, b.data_ptr(), F8[b.dtype], ldb, d.data_ptr(),

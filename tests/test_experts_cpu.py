@@ -72,6 +72,13 @@ def test_grouped_products_refuse_what_only_one_of_them_refuses(pkg):
         assert lib.b200fp8_gemm_grouped_wgrad(4, 64, 128, 256, P, P, 0, 256, P, 0, 128, P, 0, 128, 256 * 128, ctypes.byref(ep), None, None) == INVALID
 
 
+@pytest.mark.parametrize("field", ["a_scale", "b_scale", "d_scale", "amax_d", "a_row_scale", "b_row_scale", "bias"])
+def test_grouped_products_refuse_misaligned_epilogue_vectors(pkg, field):
+    ep = pkg._cabi.EpilogueDesc(ctypes.sizeof(pkg._cabi.EpilogueDesc), 1.0, 0.0)
+    setattr(ep, field, 0x10002)
+    assert pkg._cabi.lib().b200fp8_gemm_grouped(4, 64, 128, 256, P, P, 0, 128, P, 0, 128, 256 * 128, P, 1, 256, ctypes.byref(ep), None, None) == INVALID
+
+
 @pytest.mark.parametrize("bad", [dict(source=-1), dict(rows=-1), dict(k=-1), dict(k=(1 << 30) + 1, ldx=1 << 31, ldq=1 << 31), dict(x_dtype=0), dict(x_dtype=3), dict(q_dtype=2), dict(ldx=63),
                                  dict(ldq=63), dict(rows=11), dict(scale=None), dict(scale=ODD), dict(x=None), dict(x=ODD), dict(q=None),
                                  dict(index=ODD)])

@@ -518,6 +518,26 @@ def test_grouped_gradients_against_differences(g, kind):
     done(g)
 
 
+def test_grouped_products_without_extent(g):
+    """An empty contraction is refused, not skipped; what has no output at all still sets the maximum to zero."""
+    ends = ends_of([4, 4])
+    e8 = lambda *shape: torch.empty(shape, dtype=torch.uint8, device="cuda").view(E4)
+    amax = torch.full((1,), 7.0, device="cuda")
+    with pytest.raises(ValueError):
+        g.gemm_grouped(e8(8, 0), e8(2, 16, 0), torch.empty((8, 16), device="cuda"), ends)
+    with pytest.raises(ValueError):
+        g.gemm_grouped_dgrad(e8(8, 0), e8(2, 0, 16), torch.empty((8, 16), device="cuda"), ends)
+    g.gemm_grouped(e8(8, 16), e8(2, 0, 16), torch.empty((8, 0), device="cuda"), ends, amax_d=amax)
+    assert amax.item() == 0.0
+    amax.fill_(7.0)
+    g.gemm_grouped(e8(0, 16), e8(2, 16, 16), torch.empty((0, 16), device="cuda"), ends_of([0, 0]), amax_d=amax)
+    assert amax.item() == 0.0
+    d = torch.full((2, 16, 16), 3.0, device="cuda")
+    g.gemm_grouped_wgrad(e8(0, 16), e8(0, 16), d, ends_of([0, 0]), beta=2.0)
+    done(g)
+    assert (d == 6.0).all()
+
+
 # ---- 4-bit weights ---------------------------------------------------------------------------------------------------
 
 
