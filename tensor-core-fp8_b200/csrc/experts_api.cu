@@ -128,7 +128,8 @@ cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStre
     args.status = dev.status;
     args.debug = dev.debug;
     args.epi = c.epi;
-    args.wide_store = OB == 2 && args.cols % 8 == 0 && c.ldd % 8 == 0 && (!wgrad || c.stride_d % 8 == 0) && aligned(c.d, 16);
+    constexpr int kWide = OB == 2 ? 8 : 4;                        // columns per store
+    args.wide_store = OB != 4 && args.cols % kWide == 0 && c.ldd % kWide == 0 && (!wgrad || c.stride_d % kWide == 0) && aligned(c.d, kWide * OB);
 
     GroupedMaps maps;
     const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;

@@ -27,7 +27,8 @@
 //     bias) are a few registers.  FP32 rows go out as they are, 128 bytes per instruction.  16-bit ones are read from TMEM
 //     in the matrix-fragment distribution, packed in pairs along the rows and transposed on the way through shared memory
 //     by stmatrix, then stored 16 bytes per lane (swapping columns between neighbouring lanes instead took four times the
-//     instructions, and the epilogue bounds products with a short contraction).  Rows behind a group's end are simply not
+//     instructions, and the epilogue bounds products with a short contraction).  8-bit ones are packed four rows to a word
+//     and transposed 4 x 4 between four lanes, then stored 4 bytes per lane.  Rows behind a group's end are simply not
 //     stored, and D needs no TMA.
 //
 // Rows behind a group's end inside a tile belong to the next group.  Forward and dgrad may load and multiply them (each
@@ -67,7 +68,7 @@ struct GroupedArgs {
     int col_tiles;
     int group_rows;       // tiles are walked down this many row tiles before the next column tile
     uint32_t idesc;       // without N
-    int wide_store;       // 16-bit D: eight neighbouring columns can be stored as 16 bytes
+    int wide_store;       // 16-bit D: eight neighbouring columns can be stored as 16 bytes; 8-bit D: four as 4
     void* d;
     long long ldd, stride_d;
     const uint8_t* w;     // wgrad: base pointers of the ragged rows' ordinary loads
@@ -183,6 +184,17 @@ __device__ __forceinline__ void grouped_gelu_tanh(uint32_t& t0, uint32_t& t1) {
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e1));
     t0 = __float_as_uint(__uint_as_float(t0) * e0);
     t1 = __float_as_uint(__uint_as_float(t1) * e1);
+}
+
+// 32 numbers to bytes, four to a word
+template <__nv_fp8_interpretation_t TYPE>
+__device__ __forceinline__ void grouped_pack8(const uint32_t (&v)[32], uint32_t (&b)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])), __NV_SATFINITE, TYPE);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])), __NV_SATFINITE, TYPE);
+        b[j] = lo | hi << 16;
+    }
 }
 
 // ROWS: rows of D per tile (of the pair), the largest N of the MMA
@@ -606,6 +618,21 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
                         const uint4 two = ptx::ld_shared_v4(turn + r * 64 + ((chunk ^ ((r >> 1) & 3)) << 4));
                         if (in && r < rows) *reinterpret_cast<uint4*>(to) = two;
                         to += 16 * args.ldd;                      // eight rows, in bytes
+                    }
+                } else if (OB == 1 && args.wide_store) {
+                    // four rows of this lane's column to a word, 4 x 4 bytes transposed between four lanes: row 4 j + lane % 4, four columns
+                    uint32_t b[8];
+                    if (out_dtype == 3) grouped_pack8<__NV_E4M3>(v, b);
+                    else grouped_pack8<__NV_E5M2>(v, b);
+                    const uint32_t first = lane & 1 ? 0x3715u : 0x6240u, second = lane & 2 ? 0x3276u : 0x5410u;
+                    const bool in = col_base + (lane & ~3) < args.cols;
+                    uint8_t* to = static_cast<uint8_t*>(args.d) + at + (lane & 3) * args.ldd + col_base + (lane & ~3);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        b[j] = __byte_perm(b[j], __shfl_xor_sync(0xffffffffu, b[j], 1), first);
+                        b[j] = __byte_perm(b[j], __shfl_xor_sync(0xffffffffu, b[j], 2), second);
+                        if (in && 4 * j + (lane & 3) < rows) *reinterpret_cast<uint32_t*>(to) = b[j];
+                        to += 4 * args.ldd;
                     }
                 } else if (OB == 4 && rows == 32) {
                     if (col_base + lane < args.cols) {

@@ -469,6 +469,30 @@ def test_grouped_bias_types_and_one_vector_at_a_time(g, bias_dtype, out):
             close(d, want, tol, out)
 
 
+@pytest.mark.parametrize("kind", ["forward", "dgrad", "wgrad"])
+@pytest.mark.parametrize("out", [E4, E5])
+def test_grouped_8_bit_outputs_are_the_rounded_wide_ones(g, kind, out):
+    """Every alignment of an 8-bit output: the bytes are those of the FP32 output rounded, and nothing beside them is written."""
+    sizes, n, k = [37, 0, 64, 101], 80, 144
+    a, b, shape = operands(kind, sizes, 3, n, k, E5 if kind != "forward" else E4, E4, 5)
+    widths = {"forward": (n, n - 4, n - 1, n - 6), "dgrad": (k,), "wgrad": (k,)}[kind]
+    for cols in widths:
+        w = b[:, :cols].contiguous() if cols != b.shape[1] and kind == "forward" else b
+        wide = torch.zeros((*shape[:-1], cols), device="cuda")
+        call(g, kind)(a, w, wide, ends_of(sizes), alpha=2.0 ** -4)
+        for pitch, at in ((cols, 0), (cols + 8, 4), (cols + 4, 1), (cols + 5, 0)):
+            buf = torch.full((*shape[:-1], pitch), 0x33, dtype=torch.uint8, device="cuda")
+            d = buf.view(out)[..., at:at + cols]
+            call(g, kind)(a, w, d, ends_of(sizes), alpha=2.0 ** -4)
+            done(g)
+            want = torch.full_like(buf, 0x33)
+            rounded = bytes_of(nearest8(wide.double(), out).float().to(out))
+            if kind != "wgrad":
+                rounded[sum(sizes):] = 0x33
+            want[..., at:at + cols] = rounded
+            assert torch.equal(buf & 0x7F, want & 0x7F) and torch.equal(buf.view(out).float(), want.view(out).float())
+
+
 @pytest.mark.parametrize("out", [E4, E5])
 def test_wgrad_to_fp8(g, out):
     sizes, n, k = [33, 0, 200], 48, 112
