@@ -102,11 +102,11 @@ struct GroupedCall {
     Epilogue epi;
 };
 
-template <int MODE, int ROWS, int CTAS, int OB>
-cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStream_t stream) {
+template <int MODE, int ROWS, int CTAS, int OB, bool BETA>
+cudaError_t launch_grouped_form(const HostDevice& dev, const GroupedCall& c, cudaStream_t stream) {
     using L = GroupedSmem<ROWS, CTAS>;
     constexpr bool wgrad = MODE == kGroupedWgrad;
-    cudaError_t e = allow_smem<gemm_fp8_grouped_kernel<MODE, ROWS, CTAS, OB>>(L::kDynamicBytes);
+    cudaError_t e = allow_smem<gemm_fp8_grouped_kernel<MODE, ROWS, CTAS, OB, BETA>>(L::kDynamicBytes);
     if (e != cudaSuccess) return e;
     GroupedArgs args{};
     args.experts = c.experts;
@@ -159,8 +159,13 @@ cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStre
     int units = dev.sm_count / CTAS;
     if (c.max_ctas > 0) units = std::max(1, std::min(units, c.max_ctas / CTAS));
     units = static_cast<int>(std::min<long long>(units, tiles));
-    return launch(gemm_fp8_grouped_kernel<MODE, ROWS, CTAS, OB>, dev.pdl, dim3(static_cast<unsigned>(units * CTAS), 1, 1), kGemmThreads, L::kDynamicBytes,
+    return launch(gemm_fp8_grouped_kernel<MODE, ROWS, CTAS, OB, BETA>, dev.pdl, dim3(static_cast<unsigned>(units * CTAS), 1, 1), kGemmThreads, L::kDynamicBytes,
                   CTAS, stream, maps, args);
+}
+
+template <int MODE, int ROWS, int CTAS, int OB>
+cudaError_t launch_grouped(const HostDevice& dev, const GroupedCall& c, cudaStream_t stream) {
+    return c.epi.beta != 0.0f ? launch_grouped_form<MODE, ROWS, CTAS, OB, true>(dev, c, stream) : launch_grouped_form<MODE, ROWS, CTAS, OB, false>(dev, c, stream);
 }
 
 // The automatic choice.  The sizes of the groups are known on the device only, so it goes by their average.

@@ -186,6 +186,11 @@ __device__ __forceinline__ void grouped_gelu_tanh(uint32_t& t0, uint32_t& t1) {
     t1 = __float_as_uint(__uint_as_float(t1) * e1);
 }
 
+// the low half of a word as BF16 (out_dtype 1) or FP16
+__device__ __forceinline__ float wide16(uint32_t bits, int out_dtype) {
+    return out_dtype == 1 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+}
+
 // 32 numbers to bytes, four to a word
 template <__nv_fp8_interpretation_t TYPE>
 __device__ __forceinline__ void grouped_pack8(const uint32_t (&v)[32], uint32_t (&b)[8]) {
@@ -236,7 +241,8 @@ __device__ __forceinline__ void grouped_load_ragged(uint32_t dst, const uint8_t*
     }
 }
 
-template <int MODE, int ROWS, int CTAS, int OB>               // OB: bytes of an element of D
+// OB: bytes of an element of D.  BETA: D is read too (a kernel of its own: its registers and code cost the others 8 %).
+template <int MODE, int ROWS, int CTAS, int OB, bool BETA>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedArgs args)
 {
@@ -454,7 +460,7 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
         if (args.epi.b_scale) alpha0 *= *args.epi.b_scale;
         if (args.epi.d_scale) dscale = *args.epi.d_scale;
         // what few calls ask for sits behind one branch
-        const bool more = args.epi.beta != 0.0f || args.epi.activation != 0 || args.epi.amax != nullptr || args.epi.d_scale != nullptr;
+        const bool more = BETA || args.epi.activation != 0 || args.epi.amax != nullptr || args.epi.d_scale != nullptr;
         // This lane's columns of a tile: one, or four for 16-bit outputs.
         constexpr int kCols = OB == 2 ? 4 : 1;
         auto col_of = [&](const GroupedTile& w, int m) {
@@ -479,6 +485,9 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
             for (int i = 0; i < ROWS / 64; ++i) {                 // this warp's chunks: grp, grp + 2, ...
                 const int r = (2 * i + grp) * 32 + lane;
                 next_row[i] = args.epi.a_row_scale != nullptr && r < w.rows ? __ldg(args.epi.a_row_scale + w.row0 + r) : 0.0f;
+                if (BETA && r < w.rows && w.col0 + static_cast<int>(rank) * 128 + q * 32 < args.cols)
+                    ptx::prefetch_l2(static_cast<const char*>(args.d) + OB * ((MODE == kGroupedWgrad ? w.e * args.stride_d : 0) +
+                                     (static_cast<long long>(w.row0) + r) * args.ldd + w.col0 + static_cast<int>(rank) * 128 + q * 32));
             }
         };
         int it = 0;
@@ -529,6 +538,33 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
 #pragma unroll 1
             for (int c = grp; c < chunks; c += 2) {
                 const int rows = min(32, w.rows - c * 32);
+                const long long at = d_base + static_cast<long long>(c) * 32 * args.ldd;
+                // What D holds, for beta: all loads in flight at once (one by one they took ten times as long as the rest of wgrad),
+                // from L2, where they were asked for a tile ahead.  16-bit rows come 16 bytes per lane, as they go.
+                [[maybe_unused]] uint32_t old[32];
+                if constexpr (BETA) {
+                    if (OB == 2 && args.wide_store) {
+                        const bool in = col_base + 8 * (lane & 3) < args.cols;
+                        const uint16_t* from = static_cast<const uint16_t*>(args.d) + at + (lane >> 2) * args.ldd + col_base + 8 * (lane & 3);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint4 four = make_uint4(0u, 0u, 0u, 0u);
+                            if (in && 8 * i + (lane >> 2) < rows) four = __ldcg(reinterpret_cast<const uint4*>(from + 8 * i * args.ldd));
+                            old[4 * i] = four.x; old[4 * i + 1] = four.y; old[4 * i + 2] = four.z; old[4 * i + 3] = four.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const long long from = at + row_of(i) * args.ldd + col(block_of(i));
+                            old[i] = 0u;
+                            if (row_of(i) < rows && col(block_of(i)) < args.cols) {
+                                if constexpr (OB == 4) old[i] = __ldcg(static_cast<const unsigned int*>(args.d) + from);
+                                else if constexpr (OB == 2) old[i] = __ldcg(static_cast<const unsigned short*>(args.d) + from);
+                                else old[i] = __ldcg(static_cast<const unsigned char*>(args.d) + from);
+                            }
+                        }
+                    }
+                }
                 if (empty) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = 0u;
@@ -541,7 +577,6 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
                     }
                     ptx::tmem_ld_wait();
                 }
-                const long long at = d_base + static_cast<long long>(c) * 32 * args.ldd;
                 if (args.epi.a_row_scale != nullptr) {
                     const float* ra = row_scales + (c >> 1) * 32;
                     if constexpr (OB == 2) {
@@ -569,11 +604,40 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(fmaf(factor[block_of(i)], __uint_as_float(v[i]), bias[block_of(i)]));
                 if (more) {
-                    if (args.epi.beta != 0.0f) {
+                    if constexpr (BETA) {
+                        auto add = [&](uint32_t& sum, float d) { sum = __float_as_uint(fmaf(args.epi.beta, d, __uint_as_float(sum))); };
+                        if (OB == 2 && args.wide_store) {
+                            __syncwarp();                         // the chunk before has been read
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (row_of(i) < rows && col(block_of(i)) < args.cols)
-                                v[i] = __float_as_uint(fmaf(args.epi.beta, load_out(args.d, at + row_of(i) * args.ldd + col(block_of(i)), out_dtype), __uint_as_float(v[i])));
+                            for (int i = 0; i < 4; ++i) {
+                                const int r = 8 * i + (lane >> 2);
+                                ptx::st_shared_v4(turn + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4), old[4 * i], old[4 * i + 1], old[4 * i + 2], old[4 * i + 3]);
+                            }
+                            __syncwarp();
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                uint32_t p[4];
+                                ptx::ldmatrix_x4_trans(turn + 512 * j + (lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4), p);
+#pragma unroll
+                                for (int m = 0; m < 4; ++m) {
+                                    uint32_t* s = v + 16 * (m >> 1) + 4 * j + 2 * (m & 1);
+                                    add(s[0], wide16(p[m], out_dtype));
+                                    add(s[1], wide16(p[m] >> 16, out_dtype));
+                                }
+                            }
+                        } else if constexpr (OB == 4) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) add(v[i], __uint_as_float(old[i]));
+                        } else if constexpr (OB == 2) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) add(v[i], wide16(old[i], out_dtype));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(old[i]), out_dtype == 3 ? __NV_E4M3 : __NV_E5M2);
+                                add(v[i], __half2float(__half(h)));
+                            }
+                        }
                     }
                     if (args.epi.activation == 1) {
 #pragma unroll

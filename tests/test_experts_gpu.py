@@ -542,6 +542,35 @@ def test_grouped_gradients_against_differences(g, kind):
     done(g)
 
 
+@pytest.mark.parametrize("kind", ["forward", "dgrad", "wgrad"])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16, torch.float16, E4, E5])
+def test_grouped_accumulation_at_every_alignment(g, kind, out):
+    """beta * D with rows at any place of a wider buffer: what D held counts once, and nothing beside it changes."""
+    sizes, n, k = [37, 0, 64, 101], 144, 160
+    a, b, shape = operands(kind, sizes, 3, n, k, E5 if kind != "forward" else E4, E4, 5)
+    cols = shape[-1]
+    old = torch.randint(-8, 9, shape, generator=gen(7), device="cuda").float().to(out)
+    t, s = product64(kind, a, b, sizes, shape)
+    want, tol = t / 64 + 0.5 * old.double(), 1.2 * s / 64 * steps(max(n, k)) + 2.0 ** -22 * (s / 64 + old.double().abs())
+    if kind != "wgrad":
+        want[sum(sizes):] = old[sum(sizes):].double()
+    first = None
+    for pitch, at in ((cols, 0), (cols + 16, 8), (cols + 5, 3), (cols + 3, 0)):
+        buf = torch.full((*shape[:-1], pitch), 3.0, device="cuda").to(out)
+        d = buf[..., at:at + cols]
+        d.copy_(old)
+        call(g, kind)(a, b, d, ends_of(sizes), alpha=1 / 64, beta=0.5)
+        done(g)
+        if out in TOP:
+            lo, hi = (nearest8(want + sign * tol, out) for sign in (-1, 1))
+            assert ((d.double() >= lo) & (d.double() <= hi)).all()
+        else:
+            close(d, want, tol, out)
+        first = d.clone() if first is None else first
+        assert torch.equal(bytes_of(d), bytes_of(first))
+        assert (buf[..., :at].float() == 3.0).all() and (buf[..., at + cols:].float() == 3.0).all()
+
+
 def test_grouped_products_without_extent(g):
     """An empty contraction is refused, not skipped; what has no output at all still sets the maximum to zero."""
     ends = ends_of([4, 4])
