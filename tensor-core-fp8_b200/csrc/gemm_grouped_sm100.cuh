@@ -26,7 +26,7 @@
 //     16 to 128 rows, that covers them).  In the epilogue a lane owns columns, so the vectors per column (b_row_scale,
 //     bias) are a few registers.  FP32 rows go out as they are, 128 bytes per instruction.  16-bit ones are read from TMEM
 //     in the matrix-fragment distribution, packed in pairs along the rows and transposed on the way through shared memory
-//     by stmatrix, then stored 16 bytes per lane (swapping columns between neighbouring lanes instead took four times the
+//     by stmatrix, then stored 16 bytes per lane, or a row's 64 bytes from 32 lanes where the alignment allows no more (swapping columns between neighbouring lanes instead took four times the
 //     instructions, and the epilogue bounds products with a short contraction).  8-bit ones are packed four rows to a word
 //     and transposed 4 x 4 between four lanes, then stored 4 bytes per lane.  Rows behind a group's end are simply not
 //     stored, and D needs no TMA.
@@ -659,7 +659,7 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
                         for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(dscale * __uint_as_float(v[i]));
                     }
                 }
-                if (OB == 2 && args.wide_store) {
+                if constexpr (OB == 2) {
                     // rows of 64 bytes, 16-byte chunk ^ (row / 2) mod 4: neither side has bank conflicts
                     __syncwarp();                                 // the chunk before has been read
 #pragma unroll
@@ -673,15 +673,25 @@ gemm_fp8_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedA
                         ptx::stmatrix_x4_trans(turn + 512 * j + (lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4), p[0], p[1], p[2], p[3]);
                     }
                     __syncwarp();
-                    const int chunk = lane & 3;                   // eight columns
-                    const bool in = col_base + 8 * chunk < args.cols;
-                    char* to = reinterpret_cast<char*>(static_cast<uint16_t*>(args.d) + at + (lane >> 2) * args.ldd + col_base + 8 * chunk);
+                    if (args.wide_store) {
+                        const int chunk = lane & 3;                   // eight columns
+                        const bool in = col_base + 8 * chunk < args.cols;
+                        char* to = reinterpret_cast<char*>(static_cast<uint16_t*>(args.d) + at + (lane >> 2) * args.ldd + col_base + 8 * chunk);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = 8 * i + (lane >> 2);
-                        const uint4 two = ptx::ld_shared_v4(turn + r * 64 + ((chunk ^ ((r >> 1) & 3)) << 4));
-                        if (in && r < rows) *reinterpret_cast<uint4*>(to) = two;
-                        to += 16 * args.ldd;                      // eight rows, in bytes
+                        for (int i = 0; i < 4; ++i) {
+                            const int r = 8 * i + (lane >> 2);
+                            const uint4 two = ptx::ld_shared_v4(turn + r * 64 + ((chunk ^ ((r >> 1) & 3)) << 4));
+                            if (in && r < rows) *reinterpret_cast<uint4*>(to) = two;
+                            to += 16 * args.ldd;                      // eight rows, in bytes
+                        }
+                    } else {                                      // a row's 64 bytes from 32 lanes
+                        const bool in = col_base + lane < args.cols;
+                        uint16_t* to = static_cast<uint16_t*>(args.d) + at + col_base + lane;
+#pragma unroll 8
+                        for (int r = 0; r < rows; ++r, to += args.ldd) {
+                            const uint16_t one = ptx::ld_shared_u16(turn + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + 2 * (lane & 7));
+                            if (in) *to = one;
+                        }
                     }
                 } else if (OB == 1 && args.wide_store) {
                     // four rows of this lane's column to a word, 4 x 4 bytes transposed between four lanes: row 4 j + lane % 4, four columns
