@@ -571,6 +571,23 @@ def test_grouped_accumulation_at_every_alignment(g, kind, out):
         assert (buf[..., :at].float() == 3.0).all() and (buf[..., at + cols:].float() == 3.0).all()
 
 
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 17, 33, 129, 250, 515])
+def test_grouped_products_of_any_number_of_columns(g, out, n):
+    sizes, k = [65, 0, 300, 31, 1], 208
+    a, b, shape = operands("forward", sizes, 2, n, k, E4, E4, n)
+    buf = torch.full((shape[0] + 1, n), 3.0, device="cuda").to(out)
+    d, bias = buf[:-1], torch.randn((5, n), generator=gen(3), device="cuda")
+    g.gemm_grouped(a, b, d, ends_of(sizes), alpha=1 / 64, bias=bias)
+    done(g)
+    t, s = product64("forward", a, b, sizes, shape)
+    used = sum(sizes)
+    of = torch.cat([torch.full((hi - lo,), e, device="cuda") for e, lo, hi in spans(sizes)]).long()
+    want = t[:used] / 64 + bias.double()[of]
+    close(d[:used], want, steps(k) * s[:used] / 64 + 2.0 ** -23 * (s[:used] / 64 + bias.double()[of].abs()), out)
+    assert (buf[used:].float() == 3.0).all()
+
+
 def test_grouped_products_without_extent(g):
     """An empty contraction is refused, not skipped; what has no output at all still sets the maximum to zero."""
     ends = ends_of([4, 4])
