@@ -30,6 +30,11 @@
 // in one pass over `expert`: with fewer rows than experts block z stands for row z and works if that row is the
 // first of its expert, else block z stands for expert z.  Each expert's weights are read once per eight of its rows.
 //
+// Measured: one vector, 8192 x 8192, groups of 128: 12.0 us (2.9 TB/s; starting and joining the parts of K is about 5 of them); eight
+// vectors, 28672 x 8192, groups of 64 with zero points: 45.5 us (2.8 TB/s, 0.43 of a plain copy's rate); 16 tokens with 8 of 64
+// experts each, 2048 x 4096, groups of 128: 44.7 us.  Issue slots are half used: what bounds it is a warp's chain from a slot's
+// arrival over unpacking to the sums, about 380 instructions per 16 x 256 codes at 16 warps per SM (a third CTA per SM spills: 64 us).
+//
 // Waits on mbarriers are bounded as in the other kernels: a wait that runs out sets the status word and ends the kernel.
 #pragma once
 #include <cuda_bf16.h>
