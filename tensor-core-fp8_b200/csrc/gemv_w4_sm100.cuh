@@ -5,11 +5,11 @@
 // c: codes 0..15, two to a byte, the even k in the low half; one scale (and, optionally, one zero point; 8 without) per row
 // and group of 32, 64 or 128 k.  x is BF16 or FP16; y has its type or FP32.
 //
-// The arithmetic is exact up to the FP32 sums: c - z is a whole number of at most 15 and so exact in FP16 (over 1024), the tensor core
-// (m16n8k16) multiplies exactly and adds in FP32, and the scale multiplies a group's FP32 sum, not the rounded weight.
-// BF16 vectors are brought to FP16 by a power of two per vector and 256 of K, so that the largest of these lies in
-// [2^14, 2^15): eight significant bits fit eleven, and what falls below FP16's smallest step is less than 2^-39 of the
-// largest, far below the FP32 sums' rounding.  (FP16 takes one shift per eight codes where BF16 takes three.)
+// The arithmetic is exact up to the FP32 sums: c - z is a whole number of at most 15 and so exact in x's type (over 1024 in
+// FP16, over 64 in BF16), the tensor core (m16n8k16) multiplies exactly and adds in FP32, and the scale multiplies a group's
+// FP32 sum, not the rounded weight.  x is taken as it is, whatever stands beside it: bringing BF16 vectors to FP16 by a power
+// of two per 256 of K, as this kernel once did, lost what was 2^-32 of the largest among them, which shows where that
+// one's weight is zero, and took a sum and a factor per slot more (eight vectors, 28672 x 8192: 49.6 -> 45.4 us).
 // Rows of the weights are the M index of the instruction and the vectors its N index, so up to eight vectors cost what
 // one costs; the order of k inside an instruction is free, and is chosen so that a lane's eight codes are one aligned
 // 32-bit word: (k, k + 4) share a 16-bit pair, which is what a mask takes out of the word.
@@ -41,6 +41,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
+#include <type_traits>
 #include "gemm_sm100.cuh"
 
 namespace b200fp8 {
@@ -73,70 +74,57 @@ constexpr int kW4BoxBytes = 128;         // of codes per row and ring slot: 256 
 constexpr int kW4BoxK = 2 * kW4BoxBytes;
 constexpr int kStatusW4Timeout = 106;
 
-// c = a b (FIRST) or c += a b
-template <bool FIRST>
+// c = a b (FIRST) or c += a b, in BF16 or FP16
+#define B200FP8_W4_MMA(TYPE)                                                                                                                    \
+    if constexpr (FIRST)                                                                                                                        \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"  \
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));               \
+    else                                                                                                                                        \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"      \
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
+template <bool BF16, bool FIRST>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (FIRST)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// A row's zero point z as what its codes lose: -z / 1024 in both halves (FP16).  `zeros` holds four zero points, one to a byte.
-__device__ __forceinline__ __half2 w4_minus(uint32_t zeros, uint32_t place) {
-    const uint32_t z = __byte_perm(zeros, 0u, 0x4040u + place * 0x0101u);     // z * 2^-24: a subnormal number's bits count upwards
-    return __hmul2(*reinterpret_cast<const __half2*>(&z), __half2half2(__ushort_as_half(0xF400)));   // * -2^14
-}
-// The eight codes of a word as four pairs (j, j + 4) of FP16 numbers (c - z) / 1024, exactly.  A code in the four lowest bits
-// of a half is the subnormal number c * 2^-24, one in the next four bits c * 2^-20, so that a mask alone makes it a
-// number and one fused multiply-add scales it and takes the zero point off.
-__device__ __forceinline__ void w4_unpack(uint32_t word, __half2 minus, uint32_t (&a)[4]) {
-    const uint32_t next = word >> 8;
-    const uint32_t v[4] = {word & 0x000F000Fu, word & 0x00F000F0u, next & 0x000F000Fu, next & 0x00F000F0u};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&v[i]), __half2half2(__ushort_as_half(i & 1 ? 0x6400 : 0x7400)), minus);
-        a[i] = *reinterpret_cast<const uint32_t*>(&r);
+    if constexpr (BF16) {
+        B200FP8_W4_MMA("bf16");
+    } else {
+        B200FP8_W4_MMA("f16");
     }
 }
+#undef B200FP8_W4_MMA
 
-// Eight consecutive x of one vector as FP16 pairs (0, 4), (1, 5), (2, 6), (3, 7).  BF16: a whole warp calls it with the
-// pieces of 256 consecutive k and gets the power of two `back` that undoes the scaling.
+// Codes become numbers of x's type without a conversion: a code in the four lowest bits of a half is the subnormal number
+// c * 2^-24 of FP16 or c * 2^-133 of BF16, one in the next four bits 16 times that, so that a mask alone makes it a number
+// and one fused multiply-add brings it to c * kUnit and takes the zero point off.  kUnit is the largest power of two that
+// the factors of both places allow; (c - z) * kUnit has four significant bits and is exact.
 template <bool BF16>
-__device__ __forceinline__ uint4 w4_vector_piece(uint4 v, float& back) {
-    if constexpr (!BF16) {
-        back = 1.0f;
-        return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-    } else {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        uint32_t most = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) most = max(most, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
-        most = __reduce_max_sync(0xffffffffu, most);
-        if (most >= 0x7F80u) {                                   // an infinity or a NaN: the largest finite number counts
-            most = 0u;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t a = w[i] & 0x7FFFu, b = (w[i] >> 16) & 0x7FFFu;
-                most = max(most, max(a < 0x7F80u ? a : 0u, b < 0x7F80u ? b : 0u));
-            }
-            most = __reduce_max_sync(0xffffffffu, most);
-        }
-        const int up = min(126, 141 - static_cast<int>(most >> 7));          // 14 - (exponent - 127)
-        const float forth = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-        back = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
-        uint32_t r[4];
+struct W4Number {
+    using Pair = typename std::conditional<BF16, __nv_bfloat162, __half2>::type;
+    static constexpr float kBack = BF16 ? 64.0f : 1024.0f;              // 1 / kUnit
+    static __device__ __forceinline__ Pair twice(uint32_t bits) {
+        const uint32_t w = bits | bits << 16;
+        return *reinterpret_cast<const Pair*>(&w);
+    }
+    // A row's zero point as what its codes lose, -z * kUnit.  `zeros` holds four zero points, one to a byte.
+    static __device__ __forceinline__ Pair minus(uint32_t zeros, uint32_t place) {
+        const uint32_t z = __byte_perm(zeros, 0u, 0x4040u + place * 0x0101u);
+        return __hmul2(*reinterpret_cast<const Pair*>(&z), twice(BF16 ? 0xFF00u : 0xF400u));                        // -2^127, -2^14
+    }
+    // The eight codes of a word as four pairs (j, j + 4).
+    static __device__ __forceinline__ void unpack(uint32_t word, Pair minus, uint32_t (&a)[4]) {
+        const uint32_t next = word >> 8;
+        const uint32_t v[4] = {word & 0x000F000Fu, word & 0x00F000F0u, next & 0x000F000Fu, next & 0x00F000F0u};
+        const Pair low = twice(BF16 ? 0x7F00u : 0x7400u), high = twice(BF16 ? 0x7D00u : 0x6400u);                   // 2^127, 2^14; 2^123, 2^10
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t lo = w[i >> 1], hi = w[2 + (i >> 1)];             // numbers i and i + 4
-            const float a = __uint_as_float(i & 1 ? lo & 0xFFFF0000u : lo << 16), b = __uint_as_float(i & 1 ? hi & 0xFFFF0000u : hi << 16);
-            const __half2 h = __floats2half2_rn(a * forth, b * forth);
-            r[i] = *reinterpret_cast<const uint32_t*>(&h);
+            const Pair r = __hfma2(*reinterpret_cast<const Pair*>(&v[i]), i & 1 ? high : low, minus);
+            a[i] = *reinterpret_cast<const uint32_t*>(&r);
         }
-        return make_uint4(r[0], r[1], r[2], r[3]);
     }
+};
+
+// Eight consecutive x of one vector as pairs (0, 4), (1, 5), (2, 6), (3, 7).
+__device__ __forceinline__ uint4 w4_vector_piece(uint4 v) {
+    return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
 }
 
 // ---- the integer form --------------------------------------------------------------------------------------------------
@@ -488,10 +476,8 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if (c0 + i >= limit) break;
-                        float back;
-                        const uint4 h = w4_vector_piece<BF16>(v[i], back);
+                        const uint4 h = w4_vector_piece(v[i]);
                         ptx::st_shared_v4(to + (c0 + i) * L::kXPitch, h.x, h.y, h.z, h.w);
-                        if (BF16 && lane == 0) reinterpret_cast<float*>(smem_gen + L::kBackOff)[block * 8 * NT + c0 + i] = back;
                     }
                 }
             }
@@ -602,9 +588,10 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
                         }
                     } else {
                         float c[RT][NT][4];
-                        __half2 minus[RT][2];
+                        using Number = W4Number<BF16>;
+                        typename Number::Pair minus[RT][2];
 #pragma unroll
-                        for (int h = 0; h < RT; ++h) { minus[h][0] = w4_minus(zeros[h][0], place); minus[h][1] = w4_minus(zeros[h][1], place); }
+                        for (int h = 0; h < RT; ++h) { minus[h][0] = Number::minus(zeros[h][0], place); minus[h][1] = Number::minus(zeros[h][1], place); }
 #pragma unroll
                         for (int w = i * kWords; w < (i + 1) * kWords; ++w) {
                             uint4 v[NT];
@@ -613,13 +600,13 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
 #pragma unroll
                             for (int h = 0; h < RT; ++h) {
                                 uint32_t a[4], b[4];
-                                w4_unpack(lo[h][w], minus[h][0], a);
-                                w4_unpack(hi[h][w], minus[h][1], b);
+                                Number::unpack(lo[h][w], minus[h][0], a);
+                                Number::unpack(hi[h][w], minus[h][1], b);
 #pragma unroll
                                 for (int j = 0; j < NT; ++j) {
-                                    if (w == i * kWords) mma_16816<true>(c[h][j], a[0], b[0], a[1], b[1], v[j].x, v[j].y);
-                                    else mma_16816<false>(c[h][j], a[0], b[0], a[1], b[1], v[j].x, v[j].y);
-                                    mma_16816<false>(c[h][j], a[2], b[2], a[3], b[3], v[j].z, v[j].w);
+                                    if (w == i * kWords) mma_16816<BF16, true>(c[h][j], a[0], b[0], a[1], b[1], v[j].x, v[j].y);
+                                    else mma_16816<BF16, false>(c[h][j], a[0], b[0], a[1], b[1], v[j].x, v[j].y);
+                                    mma_16816<BF16, false>(c[h][j], a[2], b[2], a[3], b[3], v[j].z, v[j].w);
                                 }
                             }
                         }
@@ -627,13 +614,12 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
                         for (int h = 0; h < RT; ++h)
 #pragma unroll
                             for (int j = 0; j < NT; ++j) {
-                                float* sum = BF16 ? ys[h][j] : y[h][j];
 #pragma unroll
-                                for (int q = 0; q < 4; ++q) sum[q] = fmaf(scale(h, q >> 1), c[h][j][q], sum[q]);
+                                for (int q = 0; q < 4; ++q) y[h][j][q] = fmaf(scale(h, q >> 1), c[h][j][q], y[h][j][q]);
                             }
                     }
                 }
-                if (BF16 || INT) {
+                if (INT) {
                     const float* back = reinterpret_cast<const float*>(smem_gen + L::kBackOff) + (kb - kc) * 8 * NT + 2 * t;
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
@@ -667,7 +653,7 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    part[(8 * j + 2 * t + (i & 1)) * L::kPartPitch + row(h, i >> 1)] = INT ? y[h][j][i] : 1024.0f * y[h][j][i];   // see w4_unpack
+                    part[(8 * j + 2 * t + (i & 1)) * L::kPartPitch + row(h, i >> 1)] = (INT ? 1.0f : W4Number<BF16>::kBack) * y[h][j][i];
         if (clustered) {
             if (b == 0) ptx::cluster_wait();                     // every CTA of the cluster has its barriers
             __syncthreads();

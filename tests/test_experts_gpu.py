@@ -734,6 +734,34 @@ def test_w4_vectors_of_any_size(g, x_dtype, m):
     close(y, v @ w.T, tol, torch.float32)
 
 
+@pytest.mark.parametrize("x_dtype,outliers", [(torch.float16, (1e3, 6e4)), (torch.bfloat16, (1e3, 6e4, 2.0 ** 20, 2.0 ** 60, 2.0 ** 120))])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+@pytest.mark.parametrize("m", [3, 8, 16])
+def test_w4_small_numbers_beside_a_large_one(g, x_dtype, outliers, group, zeros, m):
+    """One large element among small ones, with a weight of zero in every second row: the row's sum is that of the small ones."""
+    n, k = 64, 4096
+    codes, scales, z = weights((), n, k, group, torch.float32, 1, zeros)
+    x = torch.randn((m, k), generator=gen(9), device="cuda") * 0.01
+    for i, size in enumerate(outliers):
+        at = 700 * i + 37
+        x[:, at] = size
+        none = 8 if z is None else z[::2, at // group]
+        codes[::2, at // 2] = codes[::2, at // 2] & 15 | none << 4            # odd places: the high half
+    x = x.to(x_dtype)
+    w = weights64(codes, scales, z)
+    y = torch.full((m, n), float("nan"), device="cuda")
+    g.gemv_w4(codes, scales, x, y, zeros=z)
+    done(g)
+    w4_close(y, w, x, k, torch.float32)
+    # by expert, every token with two of four
+    ids = torch.tensor([(3 * t + j) % 4 for t in range(m) for j in range(2)], dtype=torch.int32, device="cuda")
+    four = lambda t: None if t is None else torch.stack([t] * 4)
+    y2 = torch.full((2 * m, n), float("nan"), device="cuda")
+    g.gemv_w4_experts(four(codes), four(scales), x, y2, ids, zeros=four(z))
+    done(g)
+    w4_close(y2, w, x.repeat_interleave(2, 0), k, torch.float32)
+
+
 @pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
 @pytest.mark.parametrize("tokens,top_k,experts,n,blocks", [(1, 1, 1, 16, 1), (1, 4, 64, 1000, 4), (16, 8, 64, 130, 3), (5, 2, 3, 515, 2), (33, 2, 2, 64, 2),
