@@ -351,13 +351,16 @@ cudaError_t launch_w4(const HostDevice& dev, W4Args args, cudaStream_t stream) {
 
 template <bool BF16, int G, bool WIDE>
 cudaError_t launch_w4_form(const HostDevice& dev, const W4Args& args, cudaStream_t stream) {
-    // One or two vectors (a token's experts are different ones, so two tokens give an expert two rows at most) take the
-    // integer form: 8192 x 8192 with groups of 128 12.4 us against 14.4, 16384 x 16384 31.8 against 39.4; with groups of 32
-    // its work per group outweighs that for a short K (four experts of 1000 x 2048: 8.2 against 7.5 us).  Filling two tiles of
-    // columns with five vectors' digits lost to the FP16 form everywhere.
+    // One or two vectors (a token's experts are usually different ones, so two tokens give an expert two rows) of weights beyond
+    // 2^25 take the integer form.  Groups of 128: 8192 x 8192 12.8 us against 14.2, 28672 x 8192 32.2 against 39.0, but 4096 x 4096
+    // 9.0 against 8.3 and 16384 x 2048 10.8 against 10.8 for two vectors; groups of 64: 28672 x 8192 37.6 against 41.8, 4096 x 4096
+    // 9.6 against 8.4.  With groups of 32 its work per group outweighs the rest (8192 x 8192 18.2 against 17.9, 4096 x 4096 9.5
+    // against 8.5).  Filling two tiles of columns with the digits of more vectors lost to the other form everywhere.
     const int vectors = args.expert ? args.m / args.rows_per_x : args.m;
-    if (vectors <= 2 && (G > 32 || args.k >= 4096)) return launch_w4<BF16, G, 1, 1, WIDE, true>(dev, args, stream);
-    // The FP16 form takes eight vectors to a pass, or sixteen.  By expert the number of rows that share an expert is known on
+    const long long matrices = args.expert ? std::min(args.experts, args.m) : 1;
+    if constexpr (G > 32)
+        if (vectors <= 2 && matrices * args.n * args.k > (1LL << 25)) return launch_w4<BF16, G, 1, 1, WIDE, true>(dev, args, stream);
+    // The form in x's type takes eight vectors to a pass, or sixteen.  By expert the number of rows that share an expert is known on
     // the device only: their average.
     const long long shared = args.expert ? args.experts : 1;
     if (args.m <= 8 * shared) {

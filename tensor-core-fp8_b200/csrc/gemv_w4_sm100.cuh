@@ -28,10 +28,11 @@
 //
 // By expert: row r of y takes the weights of expert[r] and row r / (rows / tokens) of x.  A block finds its rows by itself
 // in one pass over `expert`: with fewer rows than experts block z stands for row z and works if that row is the
-// first of its expert, else block z stands for expert z.  Each expert's weights are read once per eight of its rows.
+// first of its expert, else block z stands for expert z.  Each expert's weights are read once per eight of its rows (two in the
+// integer form, which calls of one or two tokens take).
 //
-// Measured: one vector, 8192 x 8192, groups of 128: 12.0 us (2.9 TB/s; starting and joining the parts of K is about 5 of them); eight
-// vectors, 28672 x 8192, groups of 64 with zero points: 45.5 us (2.8 TB/s, 0.43 of a plain copy's rate); 16 tokens with 8 of 64
+// Measured: one vector, 8192 x 8192, groups of 128: 12.8 us (2.7 TB/s; starting and joining the parts of K is about 5 of them); eight
+// vectors, 28672 x 8192, groups of 64 with zero points: 45.4 us (2.8 TB/s, 0.43 of a plain copy's rate); 16 tokens with 8 of 64
 // experts each, 2048 x 4096, groups of 128: 44.7 us.  Issue slots are half used: what bounds it is a warp's chain from a slot's
 // arrival over unpacking to the sums, about 380 instructions per 16 x 256 codes at 16 warps per SM (a third CTA per SM spills: 64 us).
 //
@@ -128,12 +129,14 @@ __device__ __forceinline__ uint4 w4_vector_piece(uint4 v) {
 }
 
 // ---- the integer form --------------------------------------------------------------------------------------------------
-// A few vectors leave most of the instruction's eight columns empty, and unpacking codes to FP16 is what bounds the form
-// above.  Here an x becomes a whole number of 23 bits and a sign (scaled by a power of two per vector and 256 of K so that
-// the largest lies in [2^21, 2^22): what is rounded off is below FP32's rounding of a sum with that element), cut into three
-// signed bytes that take a column each.  The codes then go into m16n8k32 as bytes, two masks and a shift per eight, the
-// sums are exact integers (at most 128 * 15 * 128 in magnitude), z enters as z times the digits' sum over the group, and the
-// columns meet with weights 1, 256, 65536.  Two vectors fill a tile of eight columns.
+// A few vectors leave most of the instruction's eight columns empty, and unpacking codes to floats is what bounds the form
+// above.  Here an x becomes a whole number of 30 bits and a sign (scaled by a power of two per vector and 256 of K so that
+// the largest lies in [2^29, 2^30)), cut into four signed bytes that take a column each: two vectors fill a tile of eight
+// columns.  The codes then go into m16n8k32 as bytes, two masks and a shift per eight, the sums are exact integers (at most
+// 128 * 15 * 128 in magnitude), z enters as z times the digits' sum over the group, and the columns meet with weights 1, 256,
+// 65536, 2^24.  A block of 256 of K whose numbers do not all fit (an element more than 2^22 below the largest in BF16, 2^19
+// in FP16 where the largest is 64 or more, an infinity or a NaN) is multiplied as the form above does it, with one column per
+// vector, so that no block loses anything: an element far below the largest is all that counts where that one's weight is zero.
 constexpr int kW4Magic = 0x4B400000;     // the FP32 number 3 * 2^22: adding a small integer to its bits adds it to its value
 
 template <bool FIRST>
@@ -146,66 +149,40 @@ __device__ __forceinline__ void mma_16832(int (&c)[4], uint32_t a0, uint32_t a1,
             : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Eight consecutive x of one vector as digits d[0..2]: .x the even k's, .y the odd ones.  A whole warp calls it with 256
-// consecutive k; `back` undoes the scaling.  Numbers that are not finite count as zeros here (true is returned: see w4_special).
+// Eight consecutive x of one vector as digits d[0..3]: .x the even k's, .y the odd ones.  A whole warp calls it with 256
+// consecutive k; `back` undoes the scaling.  True where this lane's numbers are not exactly these digits.
 template <bool BF16>
-__device__ __forceinline__ bool w4_digits(uint4 v, float& back, uint2 (&d)[3]) {
-    constexpr uint32_t kInfinite = BF16 ? 0x7F80u : 0x7C00u;
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ bool w4_digits(uint4 v, float& back, uint2 (&d)[4]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     uint32_t most = 0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) most = max(most, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
     most = __reduce_max_sync(0xffffffffu, most);
-    const bool bad = most >= kInfinite;
-    if (bad) {
-        most = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if ((w[i] & 0x7FFFu) >= kInfinite) w[i] &= 0xFFFF0000u;
-            if (((w[i] >> 16) & 0x7FFFu) >= kInfinite) w[i] &= 0xFFFFu;
-            most = max(most, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
-        }
-        most = __reduce_max_sync(0xffffffffu, most);
-    }
     // exponent of the largest: |x| < 2^(e + 1); a subnormal FP16 number counts as the smallest exponent
     const int e = BF16 ? static_cast<int>(most >> 7) - 127 : max(static_cast<int>(most >> 10), 1) - 15;
-    const int up = min(126, 21 - e);
+    const int up = min(126, 29 - e);
     const float forth = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
     back = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+    bool lost = false;
     uint32_t u[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float2 f;
         if constexpr (BF16) f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
         else f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        // the integer nearest to x * forth, plus 0x808080: its bytes are the balanced digits plus 128
-        u[2 * i] = __float_as_uint(fmaf(f.x, forth, 12582912.0f)) + (0x00808080u - kW4Magic);
-        u[2 * i + 1] = __float_as_uint(fmaf(f.y, forth, 12582912.0f)) + (0x00808080u - kW4Magic);
+        const float a = f.x * forth, b = f.y * forth;
+        const int n = __float2int_rn(a), o = __float2int_rn(b);              // a NaN becomes 0, infinities the ends of int: not equal either
+        lost = lost || __int2float_rn(n) != a || __int2float_rn(o) != b;
+        u[2 * i] = static_cast<uint32_t>(n) + 0x80808080u;                   // its bytes are the balanced digits plus 128
+        u[2 * i + 1] = static_cast<uint32_t>(o) + 0x80808080u;
     }
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const uint32_t pick = i | (4 + i) << 4;
         d[i].x = __byte_perm(__byte_perm(u[0], u[2], pick), __byte_perm(u[4], u[6], pick), 0x5410) ^ 0x80808080u;
         d[i].y = __byte_perm(__byte_perm(u[1], u[3], pick), __byte_perm(u[5], u[7], pick), 0x5410) ^ 0x80808080u;
     }
-    return bad;
-}
-
-// What the infinities and NaNs of x[k0 .. k1) add to the product with one row of the weights (the other elements are skipped).
-template <bool BF16, int G>
-__device__ __noinline__ float w4_special(const uint8_t* codes, const void* scales, long long scale_at, int scale_dtype, const uint8_t* zeros,
-                                         const uint16_t* x, int k0, int k1) {
-    float sum = 0.0f;
-    for (int k = k0; k < k1; ++k) {
-        const uint32_t bits = x[k];
-        if ((bits & 0x7FFFu) < (BF16 ? 0x7F80u : 0x7C00u)) continue;
-        const uint32_t two = codes[k / 2];
-        const int c = k & 1 ? two >> 4 : two & 15u;
-        const int z = zeros ? zeros[k / G] & 15 : 8;
-        sum += static_cast<float>(c - z) * load_out(scales, scale_at + k / G, scale_dtype) *
-               (BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(bits))));
-    }
-    return sum;
+    return lost;
 }
 
 // Four scales in a row from group `at` on (a multiple of four) as they are stored: FP32, or 16-bit ones two to a word.
@@ -259,7 +236,7 @@ struct W4Smem {
     static constexpr int kTileRows = 16 * RT * kW4Warps;         // rows of the weights per CTA
     static constexpr int kSlotBytes = 16 * RT * kW4BoxBytes;
     static constexpr int kStages = 4 / RT;                       // 8 KB in flight per warp
-    static constexpr int kVectors = INT ? 8 * NT / 3 : 8 * NT;   // of x that share a pass over the weights
+    static constexpr int kVectors = INT ? 2 * NT : 8 * NT;        // of x that share a pass over the weights
     static constexpr int kXK = INT ? 2048 : 2048 / NT;           // of K whose x is staged at a time
     static constexpr int kXPitch = kXK * (INT ? 1 : 2) + 64;     // bytes; two columns' lanes meet different banks
     static constexpr int kPartPitch = kTileRows + 4;           // floats
@@ -268,7 +245,7 @@ struct W4Smem {
     static constexpr int kSumOff = kBackOff + kXK / kW4BoxK * 8 * NT * 4;               // INT: digits' sums [groups][columns]
     static constexpr int kPartOff = kSumOff + (INT ? kXK / 32 * 8 * NT * 4 : 0);
     static constexpr int kBarOff = kPartOff + 8 * NT * kPartPitch * 4;   // full[warp][stage], ready, done
-    static constexpr int kMiscOff = kBarOff + 8 * (kW4Warps * kStages + 2);   // abort flag, vectors with numbers that are not finite
+    static constexpr int kMiscOff = kBarOff + 8 * (kW4Warps * kStages + 2);   // abort flag, INT: blocks of the chunk that go as floats
     static constexpr int kListOff = kMiscOff + 48;                       // by expert: rows of y (the call's row count)
     static constexpr int kFixedBytes = kListOff + 1024;                  // with the slack for 1024-byte alignment
 };
@@ -313,7 +290,7 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
     const uint32_t bar_ready = smem_base + L::kBarOff + 8 * kW4Warps * kStages, bar_done = bar_ready + 8;
     const uint32_t ring = smem_base + warp * kStages * L::kSlotBytes;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + L::kMiscOff);
-    volatile int* bad = reinterpret_cast<volatile int*>(smem_gen + L::kMiscOff + 8);   // [vector of the batch]
+    int* as_floats = reinterpret_cast<int*>(smem_gen + L::kMiscOff + 8);               // INT: [block of the chunk]
     int* list = reinterpret_cast<int*>(smem_gen + L::kListOff);
     const bool clustered = args.splits > 1;
 
@@ -402,7 +379,6 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
     bool ok = true;                                              // after a wait that ran out: no more waits, no more copies, and on to the end
     for (int b = 0; b < batches; ++b) {
         const int m0 = b * L::kVectors, cols = min(L::kVectors, have - m0);   // vectors of this batch
-        if (INT && threadIdx.x < L::kVectors) bad[threadIdx.x] = 0;
         float y[RT][NT][4];
 #pragma unroll
         for (int h = 0; h < RT; ++h)
@@ -434,28 +410,38 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
                         v[i] = __ldg(reinterpret_cast<const uint4*>(args.x + row * args.ldx + k));
                     }
                 }
+                bool lost = false;
 #pragma unroll
                 for (int i = 0; i < L::kVectors; ++i) {
-                    if (i >= cols && kc != kb0) break;
+                    if (i >= cols && kc != kb0) break;            // columns of a vector that is not there: zeros, written once per batch
                     float back;
-                    uint2 d[3];
-                    if (w4_digits<BF16>(v[i], back, d)) bad[i] = 1;
+                    uint2 d[4];
+                    lost = w4_digits<BF16>(v[i], back, d) || lost;
 #pragma unroll
-                    for (int q = 0; q < 3; ++q) {
-                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + (3 * i + q) * L::kXPitch), "r"(d[q].x), "r"(d[q].y) : "memory");
-                        int sum = __dp4a(static_cast<int>(d[q].x), 0x01010101, __dp4a(static_cast<int>(d[q].y), 0x01010101, 0));
+                    for (int q = 0; q < 4; q += 2) {              // two digits' sums in one word: at most 2^14 in magnitude each
+                        int two = 0;
 #pragma unroll
-                        for (int o = 1; o < 4 * kWords; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                        if (rest == 0) sums[3 * i + q] = static_cast<float>(sum);
-                        if (lane == 0) backs[3 * i + q] = back * (q == 0 ? 1.0f : q == 1 ? 256.0f : 65536.0f);
+                        for (int u = q; u < q + 2; ++u) {
+                            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + (4 * i + u) * L::kXPitch), "r"(d[u].x), "r"(d[u].y) : "memory");
+                            two += __dp4a(static_cast<int>(d[u].x), 0x01010101, __dp4a(static_cast<int>(d[u].y), 0x01010101, 0)) * (u == q ? 1 : 65536);
+                        }
+#pragma unroll
+                        for (int o = 1; o < 4 * kWords; o <<= 1) two += __shfl_xor_sync(0xffffffffu, two, o);
+                        const int low = static_cast<short>(two);
+                        if (rest == 0) *reinterpret_cast<float2*>(sums + 4 * i + q) = make_float2(static_cast<float>(low), static_cast<float>((two - low) >> 16));
                     }
+                    if (lane == 0) *reinterpret_cast<float4*>(backs + 4 * i) = make_float4(back, 256.0f * back, 65536.0f * back, 16777216.0f * back);
                 }
-                if (kc == kb0) {
+                lost = __any_sync(0xffffffffu, lost);
+                if (lane == 0) as_floats[block] = lost;
+                if (lost) {                                       // as floats: 512 bytes per vector, in the place of its first two columns
+                    const int piece = lane - rest + rest % kWords * 4 + rest / kWords;
+                    const uint32_t to_floats = smem_base + L::kXOff + (piece >> 4) * L::kXPitch + block * kW4BoxK + (piece & 15) * 16;
+                    __syncwarp();                                 // behind the other lanes' digits
 #pragma unroll
-                    for (int i = 3 * L::kVectors; i < 8 * NT; ++i) {      // columns that no vector has
-                        asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(to + i * L::kXPitch), "r"(0u) : "memory");
-                        if (rest == 0) sums[i] = 0.0f;
-                        if (lane == 0) backs[i] = 0.0f;
+                    for (int i = 0; i < L::kVectors; ++i) {
+                        const uint4 h = w4_vector_piece(v[i]);
+                        ptx::st_shared_v4(to_floats + 4 * i * L::kXPitch, h.x, h.y, h.z, h.w);
                     }
                 }
             }
@@ -482,168 +468,175 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
                 }
             }
             __syncthreads();
-            for (int kb = kc; kb < kend; ++kb) {
-                const int rel = (kb - kb0) * kGroups & 15;        // first group of the slot within its 16
-                if (rel == 0) {
+            const uint32_t floats = INT ? __ballot_sync(0xffffffffu, lane < kend - kc && as_floats[lane % kBlocks] != 0) : 0u;   // a bit per block
+            // The slots of the chunk; `mixed`: some of the integer form's blocks are floats.  Two copies of the loop, since the
+            // choice inside it cost every call of the integer form 2 to 4 % (16384 x 16384: 36.3 -> 34.8 us).
+            auto slots = [&](auto mixed) {
+                for (int kb = kc; kb < kend; ++kb) {
+                    const int rel = (kb - kb0) * kGroups & 15;        // first group of the slot within its 16
+                    if (rel == 0) {
 #pragma unroll
-                    for (int h = 0; h < RT; ++h)
+                        for (int h = 0; h < RT; ++h)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) { s_now[h][i] = s_next[h][i]; z_now[h][i] = z_next[h][i]; }
-                    if (kb + 16 / kGroups < kb1) fetch(((kb - kb0) * kGroups >> 4) + 1);
-                }
-                if (ok && !wait_bounded(bar_full + 8 * s, ph, abort_flag, false)) {
-                    record_failure(args.status, abort_flag, kStatusW4Timeout);
-                    ok = false;
-                }
-                __syncwarp();
-                const uint32_t at = ring + s * L::kSlotBytes + lane_at;
-                uint32_t lo[RT][8], hi[RT][8];
-#pragma unroll
-                for (int h = 0; h < RT; ++h) {
-                    const uint32_t from = at + h * 16 * kW4BoxBytes;
-                    if constexpr (G == 128) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint4 a = ptx::ld_shared_v4(from ^ (i << 6)), c = ptx::ld_shared_v4((from ^ (i << 6)) + 8 * kW4BoxBytes);
-                            lo[h][4 * i] = a.x; lo[h][4 * i + 1] = a.y; lo[h][4 * i + 2] = a.z; lo[h][4 * i + 3] = a.w;
-                            hi[h][4 * i] = c.x; hi[h][4 * i + 1] = c.y; hi[h][4 * i + 2] = c.z; hi[h][4 * i + 3] = c.w;
-                        }
-                    } else if constexpr (G == 64) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(lo[h][2 * i]), "=r"(lo[h][2 * i + 1]) : "r"(from ^ (i << 5)) : "memory");
-                            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2+1024];" : "=r"(hi[h][2 * i]), "=r"(hi[h][2 * i + 1]) : "r"(from ^ (i << 5)) : "memory");
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            lo[h][i] = ptx::ld_shared_u32(from ^ (i << 4));
-                            hi[h][i] = ptx::ld_shared_u32((from ^ (i << 4)) + 8 * kW4BoxBytes);
-                        }
+                            for (int i = 0; i < 2; ++i) { s_now[h][i] = s_next[h][i]; z_now[h][i] = z_next[h][i]; }
+                        if (kb + 16 / kGroups < kb1) fetch(((kb - kb0) * kGroups >> 4) + 1);
                     }
-                }
-                // The slot may be refilled once these reads are done.  The refill is a write of another proxy (TMA), and nothing
-                // but a proxy fence orders it behind them: without it a warp read codes of the ring's next turn.
-                ptx::fence_proxy_async_smem();
-                __syncwarp();
-                if (ok && to_fill > 0) fill(s);
-                __syncwarp();
-                if (++s == kStages) { s = 0; ph ^= 1u; }
-                const uint32_t x_at = x_lane + (kb - kc) * (INT ? 1 : 2) * kW4BoxK;
-                float2 two[RT][2];                                // scales of two groups
-                uint32_t zeros[RT][2];                            // zero points of four groups
-                uint4 digits[NT];
-                float ys[RT][NT][4];                              // this slot's sums, in the scaling of its x
+                    if (ok && !wait_bounded(bar_full + 8 * s, ph, abort_flag, false)) {
+                        record_failure(args.status, abort_flag, kStatusW4Timeout);
+                        ok = false;
+                    }
+                    __syncwarp();
+                    const uint32_t at = ring + s * L::kSlotBytes + lane_at;
+                    uint32_t lo[RT][8], hi[RT][8];
 #pragma unroll
-                for (int h = 0; h < RT; ++h) {
-                    zeros[h][0] = zeros[h][1] = 0x08080808u;
+                    for (int h = 0; h < RT; ++h) {
+                        const uint32_t from = at + h * 16 * kW4BoxBytes;
+                        if constexpr (G == 128) {
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) ys[h][j][0] = ys[h][j][1] = ys[h][j][2] = ys[h][j][3] = 0.0f;
-                }
+                            for (int i = 0; i < 2; ++i) {
+                                const uint4 a = ptx::ld_shared_v4(from ^ (i << 6)), c = ptx::ld_shared_v4((from ^ (i << 6)) + 8 * kW4BoxBytes);
+                                lo[h][4 * i] = a.x; lo[h][4 * i + 1] = a.y; lo[h][4 * i + 2] = a.z; lo[h][4 * i + 3] = a.w;
+                                hi[h][4 * i] = c.x; hi[h][4 * i + 1] = c.y; hi[h][4 * i + 2] = c.z; hi[h][4 * i + 3] = c.w;
+                            }
+                        } else if constexpr (G == 64) {
 #pragma unroll
-                for (int i = 0; i < kGroups; ++i) {
-                    // group rel + i of the 16: lane (rel + i) / 4 of the row holds it, at place (rel + i) % 4
-                    const int from = (lane & ~3) | ((rel + i) >> 2);
+                            for (int i = 0; i < 4; ++i) {
+                                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(lo[h][2 * i]), "=r"(lo[h][2 * i + 1]) : "r"(from ^ (i << 5)) : "memory");
+                                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2+1024];" : "=r"(hi[h][2 * i]), "=r"(hi[h][2 * i + 1]) : "r"(from ^ (i << 5)) : "memory");
+                            }
+                        } else {
 #pragma unroll
-                    for (int h = 0; h < RT; ++h)
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            if ((i & 1) == 0) two[h][u] = s_now[h][u].pair(((kGroups == 2 ? rel : i) >> 1) & 1, from, args.scale_dtype);
-                            if (args.zeros && (i & 3) == 0) zeros[h][u] = __shfl_sync(0xffffffffu, z_now[h][u], from);
-                        }
-                    auto scale = [&](int h, int u) { return i & 1 ? two[h][u].y : two[h][u].x; };
-                    const uint32_t place = kGroups == 2 ? (rel + i) & 3 : i & 3;
-                    if constexpr (INT) {
-                        int c[RT][NT][4];
-#pragma unroll
-                        for (int w = i * kWords; w < (i + 1) * kWords; ++w) {
-#pragma unroll
-                            for (int j = 0; j < NT; ++j)
-                                if ((w & 1) == 0) digits[j] = ptx::ld_shared_v4(x_at + 8 * j * L::kXPitch + (w >> 1) * 64);   // two words'
-#pragma unroll
-                            for (int h = 0; h < RT; ++h) {
-                                const uint32_t le = lo[h][w] & 0x0F0F0F0Fu, lo4 = (lo[h][w] >> 4) & 0x0F0F0F0Fu;
-                                const uint32_t he = hi[h][w] & 0x0F0F0F0Fu, hi4 = (hi[h][w] >> 4) & 0x0F0F0F0Fu;
-#pragma unroll
-                                for (int j = 0; j < NT; ++j) {
-                                    const uint32_t b0 = w & 1 ? digits[j].z : digits[j].x, b1 = w & 1 ? digits[j].w : digits[j].y;
-                                    if (w == i * kWords) mma_16832<true>(c[h][j], le, he, lo4, hi4, b0, b1);
-                                    else mma_16832<false>(c[h][j], le, he, lo4, hi4, b0, b1);
-                                }
+                            for (int i = 0; i < 8; ++i) {
+                                lo[h][i] = ptx::ld_shared_u32(from ^ (i << 4));
+                                hi[h][i] = ptx::ld_shared_u32((from ^ (i << 4)) + 8 * kW4BoxBytes);
                             }
                         }
-                        const float* sums = reinterpret_cast<const float*>(smem_gen + L::kSumOff) + ((kb - kc) * kGroups + i) * 8 * NT + 2 * t;
+                    }
+                    // The slot may be refilled once these reads are done.  The refill is a write of another proxy (TMA), and nothing
+                    // but a proxy fence orders it behind them: without it a warp read codes of the ring's next turn.
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (ok && to_fill > 0) fill(s);
+                    __syncwarp();
+                    if (++s == kStages) { s = 0; ph ^= 1u; }
+                    const uint32_t x_at = x_lane + (kb - kc) * (INT ? 1 : 2) * kW4BoxK;
+                    // The slot's products, by group; `ints`: in the integer form.
+                    auto multiply = [&](auto ints) {
+                        constexpr bool kInts = decltype(ints)::value;
+                        float2 two[RT][2];                            // scales of two groups
+                        uint32_t zeros[RT][2];                        // zero points of four groups
+                        uint4 digits[NT];
+                        float ys[RT][NT][4];                          // kInts: this slot's sums, in the scaling of its x
 #pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            const float2 d = *reinterpret_cast<const float2*>(sums + 8 * j);
+                        for (int h = 0; h < RT; ++h) {
+                            zeros[h][0] = zeros[h][1] = 0x08080808u;
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) ys[h][j][0] = ys[h][j][1] = ys[h][j][2] = ys[h][j][3] = 0.0f;
+                        }
+#pragma unroll
+                        for (int i = 0; i < kGroups; ++i) {
+                            // group rel + i of the 16: lane (rel + i) / 4 of the row holds it, at place (rel + i) % 4
+                            const int from = (lane & ~3) | ((rel + i) >> 2);
 #pragma unroll
                             for (int h = 0; h < RT; ++h)
 #pragma unroll
                                 for (int u = 0; u < 2; ++u) {
-                                    // z as a number: its byte below the bits of 2^23; all exact: whole numbers below 2^24
-                                    const float z = __uint_as_float(__byte_perm(zeros[h][u], 0x4B000000u, 0x7540u | place)) - 8388608.0f;
-                                    ys[h][j][2 * u] = fmaf(scale(h, u), fmaf(-z, d.x, __int_as_float(c[h][j][2 * u])) - 12582912.0f, ys[h][j][2 * u]);
-                                    ys[h][j][2 * u + 1] = fmaf(scale(h, u), fmaf(-z, d.y, __int_as_float(c[h][j][2 * u + 1])) - 12582912.0f, ys[h][j][2 * u + 1]);
+                                    if ((i & 1) == 0) two[h][u] = s_now[h][u].pair(((kGroups == 2 ? rel : i) >> 1) & 1, from, args.scale_dtype);
+                                    if (args.zeros && (i & 3) == 0) zeros[h][u] = __shfl_sync(0xffffffffu, z_now[h][u], from);
                                 }
-                        }
-                    } else {
-                        float c[RT][NT][4];
-                        using Number = W4Number<BF16>;
-                        typename Number::Pair minus[RT][2];
+                            auto scale = [&](int h, int u) { return i & 1 ? two[h][u].y : two[h][u].x; };
+                            const uint32_t place = kGroups == 2 ? (rel + i) & 3 : i & 3;
+                            if constexpr (kInts) {
+                                int c[RT][NT][4];
 #pragma unroll
-                        for (int h = 0; h < RT; ++h) { minus[h][0] = Number::minus(zeros[h][0], place); minus[h][1] = Number::minus(zeros[h][1], place); }
+                                for (int w = i * kWords; w < (i + 1) * kWords; ++w) {
 #pragma unroll
-                        for (int w = i * kWords; w < (i + 1) * kWords; ++w) {
-                            uint4 v[NT];
+                                    for (int j = 0; j < NT; ++j)
+                                        if ((w & 1) == 0) digits[j] = ptx::ld_shared_v4(x_at + 8 * j * L::kXPitch + (w >> 1) * 64);   // two words'
 #pragma unroll
-                            for (int j = 0; j < NT; ++j) v[j] = ptx::ld_shared_v4(x_at + 8 * j * L::kXPitch + w * 64);
+                                    for (int h = 0; h < RT; ++h) {
+                                        const uint32_t le = lo[h][w] & 0x0F0F0F0Fu, lo4 = (lo[h][w] >> 4) & 0x0F0F0F0Fu;
+                                        const uint32_t he = hi[h][w] & 0x0F0F0F0Fu, hi4 = (hi[h][w] >> 4) & 0x0F0F0F0Fu;
 #pragma unroll
-                            for (int h = 0; h < RT; ++h) {
-                                uint32_t a[4], b[4];
-                                Number::unpack(lo[h][w], minus[h][0], a);
-                                Number::unpack(hi[h][w], minus[h][1], b);
+                                        for (int j = 0; j < NT; ++j) {
+                                            const uint32_t b0 = w & 1 ? digits[j].z : digits[j].x, b1 = w & 1 ? digits[j].w : digits[j].y;
+                                            if (w == i * kWords) mma_16832<true>(c[h][j], le, he, lo4, hi4, b0, b1);
+                                            else mma_16832<false>(c[h][j], le, he, lo4, hi4, b0, b1);
+                                        }
+                                    }
+                                }
+                                const float* sums = reinterpret_cast<const float*>(smem_gen + L::kSumOff) + ((kb - kc) * kGroups + i) * 8 * NT + 2 * t;
 #pragma unroll
                                 for (int j = 0; j < NT; ++j) {
-                                    if (w == i * kWords) mma_16816<BF16, true>(c[h][j], a[0], b[0], a[1], b[1], v[j].x, v[j].y);
-                                    else mma_16816<BF16, false>(c[h][j], a[0], b[0], a[1], b[1], v[j].x, v[j].y);
-                                    mma_16816<BF16, false>(c[h][j], a[2], b[2], a[3], b[3], v[j].z, v[j].w);
+                                    const float2 d = *reinterpret_cast<const float2*>(sums + 8 * j);
+#pragma unroll
+                                    for (int h = 0; h < RT; ++h)
+#pragma unroll
+                                        for (int u = 0; u < 2; ++u) {
+                                            // z as a number: its byte below the bits of 2^23; all exact: whole numbers below 2^24
+                                            const float z = __uint_as_float(__byte_perm(zeros[h][u], 0x4B000000u, 0x7540u | place)) - 8388608.0f;
+                                            ys[h][j][2 * u] = fmaf(scale(h, u), fmaf(-z, d.x, __int_as_float(c[h][j][2 * u])) - 12582912.0f, ys[h][j][2 * u]);
+                                            ys[h][j][2 * u + 1] = fmaf(scale(h, u), fmaf(-z, d.y, __int_as_float(c[h][j][2 * u + 1])) - 12582912.0f, ys[h][j][2 * u + 1]);
+                                        }
                                 }
+                            } else {
+                                float c[RT][NT][4];
+                                using Number = W4Number<BF16>;
+                                typename Number::Pair minus[RT][2];
+#pragma unroll
+                                for (int h = 0; h < RT; ++h) { minus[h][0] = Number::minus(zeros[h][0], place); minus[h][1] = Number::minus(zeros[h][1], place); }
+#pragma unroll
+                                for (int w = i * kWords; w < (i + 1) * kWords; ++w) {
+                                    uint4 v[NT];
+                                    if constexpr (INT) {              // a vector's first column has all of it
+                                        v[0] = make_uint4(0u, 0u, 0u, 0u);
+                                        if ((g & 3) == 0) v[0] = ptx::ld_shared_v4(x_at + (w >> 2) * L::kXPitch + (w & 3) * 64);
+                                    } else {
+#pragma unroll
+                                        for (int j = 0; j < NT; ++j) v[j] = ptx::ld_shared_v4(x_at + 8 * j * L::kXPitch + w * 64);
+                                    }
+#pragma unroll
+                                    for (int h = 0; h < RT; ++h) {
+                                        uint32_t a[4], b[4];
+                                        Number::unpack(lo[h][w], minus[h][0], a);
+                                        Number::unpack(hi[h][w], minus[h][1], b);
+#pragma unroll
+                                        for (int j = 0; j < NT; ++j) {
+                                            if (w == i * kWords) mma_16816<BF16, true>(c[h][j], a[0], b[0], a[1], b[1], v[j].x, v[j].y);
+                                            else mma_16816<BF16, false>(c[h][j], a[0], b[0], a[1], b[1], v[j].x, v[j].y);
+                                            mma_16816<BF16, false>(c[h][j], a[2], b[2], a[3], b[3], v[j].z, v[j].w);
+                                        }
+                                    }
+                                }
+#pragma unroll
+                                for (int h = 0; h < RT; ++h)
+#pragma unroll
+                                    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                                        for (int q = 0; q < 4; ++q) y[h][j][q] = fmaf(scale(h, q >> 1), (INT ? Number::kBack : 1.0f) * c[h][j][q], y[h][j][q]);
+                                    }
                             }
                         }
-#pragma unroll
-                        for (int h = 0; h < RT; ++h)
+                        if constexpr (kInts) {
+                            const float* back = reinterpret_cast<const float*>(smem_gen + L::kBackOff) + (kb - kc) * 8 * NT + 2 * t;
 #pragma unroll
                             for (int j = 0; j < NT; ++j) {
+                                const float2 p = *reinterpret_cast<const float2*>(back + 8 * j);
 #pragma unroll
-                                for (int q = 0; q < 4; ++q) y[h][j][q] = fmaf(scale(h, q >> 1), c[h][j][q], y[h][j][q]);
+                                for (int h = 0; h < RT; ++h)
+#pragma unroll
+                                    for (int q = 0; q < 4; ++q) y[h][j][q] = fmaf(q & 1 ? p.y : p.x, ys[h][j][q], y[h][j][q]);
                             }
-                    }
+                        }
+                    };
+                    if constexpr (!INT) multiply(std::false_type{});
+                    else if constexpr (!decltype(mixed)::value) multiply(std::true_type{});
+                    else if (floats >> (kb - kc) & 1) multiply(std::false_type{});
+                    else multiply(std::true_type{});
                 }
-                if (INT) {
-                    const float* back = reinterpret_cast<const float*>(smem_gen + L::kBackOff) + (kb - kc) * 8 * NT + 2 * t;
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const float2 p = *reinterpret_cast<const float2*>(back + 8 * j);
-#pragma unroll
-                        for (int h = 0; h < RT; ++h)
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) y[h][j][q] = fmaf(q & 1 ? p.y : p.x, ys[h][j][q], y[h][j][q]);
-                    }
-                }
-            }
-        }
-        if constexpr (INT) {                                      // rare: infinities and NaNs in these vectors
-#pragma unroll
-            for (int h = 0; h < RT; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int column = 2 * t + (i & 1), vector = column / 3, u = i >> 1;
-                    if (vector < cols && column % 3 == 0 && bad[vector]) {
-                        const int from = args.expert ? list[m0 + vector] / args.rows_per_x : m0 + vector;
-                        y[h][0][i] += w4_special<BF16, G>(args.codes + e * args.code_stride + row_n(h, u) * args.code_ld, args.scales, s_row[h][u],
-                                                          args.scale_dtype, z_row[h][u], args.x + from * args.ldx, kb0 * kW4BoxK, min(kb1 * kW4BoxK, args.k));
-                    }
-                }
+            };
+            if (INT && floats != 0) slots(std::true_type{});
+            else slots(std::false_type{});
         }
         // the parts of K meet: every CTA lays its sums out in its shared memory and adds a share of the rows
         float* part = reinterpret_cast<float*>(smem_gen + L::kPartOff);
@@ -668,8 +661,8 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
             const int c = i / share, r = split * share + i - c * share;
             float sum = 0.0f;
 #pragma unroll
-            for (int q = 0; q < (INT ? 3 : 1); ++q) {
-                const int column = (INT ? 3 : 1) * c + q;
+            for (int q = 0; q < (INT ? 4 : 1); ++q) {
+                const int column = (INT ? 4 : 1) * c + q;
                 if (clustered) {
                     const uint32_t at = part_addr + (column * L::kPartPitch + r) * 4;
                     float v[kW4MostSplits];                       // all loads in flight, then added in the order of K

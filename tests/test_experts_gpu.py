@@ -736,15 +736,14 @@ def test_w4_vectors_of_any_size(g, x_dtype, m):
 
 @pytest.mark.parametrize("x_dtype,outliers", [(torch.float16, (1e3, 6e4)), (torch.bfloat16, (1e3, 6e4, 2.0 ** 20, 2.0 ** 60, 2.0 ** 120))])
 @pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
-@pytest.mark.parametrize("m", [3, 8, 16])
-def test_w4_small_numbers_beside_a_large_one(g, x_dtype, outliers, group, zeros, m):
+@pytest.mark.parametrize("m,n,k", [(1, 64, 4096), (2, 64, 4096), (3, 64, 4096), (8, 64, 4096), (16, 64, 4096), (1, 20001, 8320), (2, 20001, 8320)])
+def test_w4_small_numbers_beside_a_large_one(g, x_dtype, outliers, group, zeros, m, n, k):
     """One large element among small ones, with a weight of zero in every second row: the row's sum is that of the small ones."""
-    n, k = 64, 4096
     codes, scales, z = weights((), n, k, group, torch.float32, 1, zeros)
     x = torch.randn((m, k), generator=gen(9), device="cuda") * 0.01
     for i, size in enumerate(outliers):
         at = 700 * i + 37
-        x[:, at] = size
+        x[i % min(m, 2)::2, at] = size                                        # every second vector
         none = 8 if z is None else z[::2, at // group]
         codes[::2, at // 2] = codes[::2, at // 2] & 15 | none << 4            # odd places: the high half
     x = x.to(x_dtype)
@@ -753,6 +752,8 @@ def test_w4_small_numbers_beside_a_large_one(g, x_dtype, outliers, group, zeros,
     g.gemv_w4(codes, scales, x, y, zeros=z)
     done(g)
     w4_close(y, w, x, k, torch.float32)
+    if n > 64:
+        return
     # by expert, every token with two of four
     ids = torch.tensor([(3 * t + j) % 4 for t in range(m) for j in range(2)], dtype=torch.int32, device="cuda")
     four = lambda t: None if t is None else torch.stack([t] * 4)
@@ -760,6 +761,62 @@ def test_w4_small_numbers_beside_a_large_one(g, x_dtype, outliers, group, zeros,
     g.gemv_w4_experts(four(codes), four(scales), x, y2, ids, zeros=four(z))
     done(g)
     w4_close(y2, w, x.repeat_interleave(2, 0), k, torch.float32)
+
+
+@pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("scale_dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group,zeros", [(32, False), (64, True), (128, False), (128, True)])
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("n,k", [(4100, 8320), (515, 65664), (40001, 896)])
+def test_w4_one_or_two_vectors_of_large_weights(g, x_dtype, scale_dtype, group, zeros, m, n, k):
+    """Sizes beyond the border to the integer form, with odd ends of N and K and every spread of x: blocks of whole numbers, of wide
+    range, of zeros, of subnormal numbers, beside an infinity and a NaN in rows of their own further down."""
+    codes, scales, z = weights((), n, k, group, scale_dtype, 2, zeros)
+    x = torch.randn((m, k), generator=gen(9), device="cuda")
+    x[:, 256:300] *= 1e-7                                                     # more than FP16 or 30 bits hold
+    x[:, 300:330] = 0
+    x[-1, 512:768] = 0
+    x[0, 800:1024 if k > 900 else 896] *= 2.0 ** (-24 if x_dtype == torch.float16 else -133)
+    x = x.to(x_dtype)
+    w = weights64(codes, scales, z)
+    for y_dtype in (x_dtype, torch.float32):
+        y = torch.full((m, n), float("nan"), dtype=y_dtype, device="cuda")
+        g.gemv_w4(codes, scales, x, y, zeros=z)
+        done(g)
+        w4_close(y, w, x, k, y_dtype)
+    first = y.clone()
+    g.gemv_w4(codes, scales, x, y, zeros=z)
+    assert torch.equal(y, first)
+    x[0, 5], x[0, k - 1], x[m - 1, 520] = float("inf"), float("inf"), -float("inf") if m == 1 else float("nan")
+    g.gemv_w4(codes, scales, x, y, zeros=z)
+    done(g)
+    want = torch.stack([(row * w[:, [5, 520, k - 1]]).sum(-1) for row in x.double()[:, [5, 520, k - 1]]])
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.isinf(y), torch.isinf(want))
+    assert torch.equal(torch.sign(y[torch.isinf(y)]).double(), torch.sign(want[torch.isinf(want)]))
+
+
+@pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group,zeros", [(64, True), (128, False)])
+@pytest.mark.parametrize("tokens,top_k,experts,n,k", [(1, 8, 9, 1000, 8320), (2, 4, 40, 515, 8320), (2, 12, 3, 700, 32896)])
+def test_w4_by_expert_of_large_weights(g, x_dtype, group, zeros, tokens, top_k, experts, n, k):
+    """One or two tokens beyond the border to the integer form: several rows of one expert, padding rows, strided weights."""
+    rows = tokens * top_k
+    codes, scales, z = weights((experts,), n, k, group, torch.float16, n, zeros)
+    wide = torch.full((experts, n + 1, k // 2 + 16), 255, dtype=torch.uint8, device="cuda")
+    wide[:, :n, :k // 2] = codes
+    x = torch.randn((tokens, k), generator=gen(9), device="cuda")
+    x[0, 300] = 3e4                                                           # a block as floats
+    x = x.to(x_dtype)
+    expert = torch.randint(0, experts, (rows,), generator=gen(5), device="cuda", dtype=torch.int32)
+    expert[1], expert[3], expert[4] = -1, expert[2], expert[2]
+    buf = torch.full((rows, n + 3), 5.0, device="cuda")
+    y = buf[:, :n]
+    g.gemv_w4_experts(wide[:, :n, :k // 2], scales, x, y, expert, zeros=z)
+    done(g)
+    assert (buf[:, n:] == 5.0).all() and (buf[1] == 5.0).all()
+    for r, e in enumerate(expert.tolist()):
+        if e >= 0:
+            w4_close(y[r:r + 1], weights64(codes[e], scales[e], None if z is None else z[e]), x[r // top_k:r // top_k + 1], k, torch.float32)
 
 
 @pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float16])
