@@ -53,18 +53,20 @@ __device__ __forceinline__ float2 unpack16(uint32_t w) {
 // and any error below that is harmless; a quotient that IS such a border (a tie) has to come out exactly.  One
 // residual step after the multiplication by the reciprocal does that: the residual of a product that should have been
 // exact is computed without error by the fused multiply-add, and adding it lands on the representable quotient.
-// x carries 2^-20 so that 1 / m is a normal number for every finite m; top = 0.875 * 2^9 or 0.875 * 2^16.
+// x carries 2^-3, so that 1 / m is a normal number for every finite m while the residual of E5M2's smallest tie in a row of
+// the least m, 2^-148, is still a number (with 2^-20 ties were lost for m of 2^-80 to 2^-76); top = 0.875 * 2^9 or 0.875 * 2^16.
 struct Quotient {
+    static constexpr float kUp = 0.125f;
     float m, back, inverse;
     __device__ __forceinline__ Quotient(float most, float two_power) : m(most) {
-        const float a = most * 9.5367431640625e-07f;             // 2^-20
+        const float a = most * kUp;
         back = a / two_power;
         inverse = two_power * __frcp_rn(a);
     }
     // an infinity as the largest finite magnitude, which becomes +-top; a NaN passes
     __device__ __forceinline__ float finite(float x) const { return fabsf(x) > m ? copysignf(m, x) : x; }
     __device__ __forceinline__ float operator()(float x) const {
-        const float u = x * (0.875f * 9.5367431640625e-07f);     // exact: three more bits
+        const float u = x * (0.875f * kUp);                      // exact: three more bits
         const float z = u * inverse;
         return fmaf(fmaf(-z, back, u), inverse, z);
     }
@@ -80,7 +82,7 @@ struct Quotient2 {
         return r;
     }
     __device__ __forceinline__ explicit Quotient2(const Quotient& q)
-        : unit(twice(0.875f * 9.5367431640625e-07f)), minus_back(twice(-q.back)), inverse(twice(q.inverse)) {}
+        : unit(twice(0.875f * Quotient::kUp)), minus_back(twice(-q.back)), inverse(twice(q.inverse)) {}
     __device__ __forceinline__ float2 operator()(float2 x) const {
         uint64_t u, z, r;
         asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(u) : "l"(pack(x)), "l"(unit));

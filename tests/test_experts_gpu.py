@@ -128,6 +128,18 @@ def test_quantize_rows_special_values_and_ties(g, dtype, source):
     check_quantized(g, rows, dtype)
 
 
+@pytest.mark.parametrize("dtype", [E4, E5])
+@pytest.mark.parametrize("pad", [0, 7])
+@pytest.mark.parametrize("exponent", [-80, -79, -76, -70, -30, -1, 0, 1, 100])
+def test_quantize_rows_ties_of_small_and_large_rows(g, dtype, pad, exponent):
+    """Every BF16 maximum of one exponent with every number down to 2^-34 of it, both ways of reading a row."""
+    below = torch.arange((exponent + 127 - 34) << 7, (exponent + 128) << 7, dtype=torch.int32, device="cuda")
+    top = below[-128:]
+    x = torch.where(below[None] <= top[:, None], below[None], 0).to(torch.int16).view(torch.bfloat16)
+    x[:, ::3] = -x[:, ::3]
+    check_quantized(g, torch.nn.functional.pad(x, (0, pad)), dtype)
+
+
 @pytest.mark.parametrize("dtype,source", [(E4, torch.bfloat16), (E5, torch.float16)])
 @pytest.mark.parametrize("rows,k", [(1301, 1024), (1301, 1032), (1301, 2048), (1301, 2056), (1301, 3064), (1301, 3080), (1100, 1032), (33, 2056), (33, 4104),
                                     (33, 6144), (33, 6152), (33, 8200), (33, 12288), (33, 12296), (33, 16384)])
