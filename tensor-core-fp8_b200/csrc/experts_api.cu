@@ -21,6 +21,8 @@ constexpr int kMaxRows = 1 << 30;        // and columns: index arithmetic in 32 
 constexpr int kMaxExperts = 1 << 16;
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// elements from the first to behind the last of a matrix; in floating point, where no pitch overflows
+double span(int rows, long long pitch, int columns) { return (rows - 1.0) * static_cast<double>(pitch) + columns; }
 bool fp8(int d) { return d == B200FP8_E4M3 || d == B200FP8_E5M2; }
 
 // dynamic shared memory above the default has to be asked for once per kernel and device
@@ -242,8 +244,10 @@ cudaError_t grouped(int mode, int experts, int rows, int k, int n, const int* en
     if (lda < a_cols || ldb < k || ldd < d_cols) return cudaErrorInvalidValue;
     constexpr long long kMostStride = 1LL << 39;                  // a tensor map's strides are below 2^40 bytes
     if (lda > kMostStride || ldb > kMostStride || ldd > kMostStride / 4) return cudaErrorInvalidValue;
-    if (!wgrad && (stride_b % 16 || (experts > 1 && stride_b < static_cast<long long>(n - 1) * ldb + k) || stride_b > kMostStride)) return cudaErrorInvalidValue;
-    if (wgrad && ((experts > 1 && stride_d < static_cast<long long>(n - 1) * ldd + k) || stride_d > kMostStride / 4)) return cudaErrorInvalidValue;
+    if (experts > 1) {                                            // one expert's matrix has no next one
+        if (!wgrad && (stride_b % 16 || stride_b < span(n, ldb, k) || stride_b > kMostStride)) return cudaErrorInvalidValue;
+        if (wgrad && (stride_d < span(n, ldd, k) || stride_d > kMostStride / 4)) return cudaErrorInvalidValue;
+    }
     const int out_bytes = out_dtype_bytes(d_dtype);
     const bool nothing = experts == 0 || (rows == 0 && !wgrad);
     if (!nothing) {
@@ -391,7 +395,8 @@ cudaError_t launch_w4_type(const HostDevice& dev, const W4Args& args, cudaStream
 }
 
 cudaError_t w4(const W4Args& args, int x_dtype, cudaStream_t stream) {
-    if (args.n < 0 || args.k <= 0 || args.m < 0 || args.n > 65535 * 128 || args.k > kMaxRows || args.m > kMaxRows || args.code_ld > (1LL << 39) || args.code_stride > (1LL << 39)) return cudaErrorInvalidValue;
+    if (args.n < 0 || args.k <= 0 || args.m < 0 || args.n > 65535 * 128 || args.k > kMaxRows || args.m > kMaxRows || args.code_ld > (1LL << 39))
+        return cudaErrorInvalidValue;
     if (x_dtype != B200FP8_OUT_BF16 && x_dtype != B200FP8_OUT_F16) return cudaErrorInvalidValue;
     if (args.y_dtype != x_dtype && args.y_dtype != B200FP8_OUT_F32) return cudaErrorInvalidValue;
     if (args.scale_dtype < B200FP8_OUT_F32 || args.scale_dtype > B200FP8_OUT_F16) return cudaErrorInvalidValue;
@@ -476,9 +481,10 @@ int b200fp8_gemv_w4_experts(int tokens, int rows, int experts, int k, int n, int
     if (tokens < 0 || rows < 0 || experts < 0 || rows > kW4MostRows || experts > kW4MostExperts) return cudaErrorInvalidValue;
     if (rows > 0 && (tokens == 0 || rows % tokens || !expert || !aligned(expert, 4))) return cudaErrorInvalidValue;
     if (experts > 1 && k > 0 && n > 0 &&
-        (code_stride % 16 || code_stride < (n - 1) * code_ld + k / 2 || scale_stride < (n - 1) * scale_ld + k / std::max(group, 1) ||
-         (zeros && zero_stride < (n - 1) * zero_ld + k / std::max(group, 1))))
+        (code_stride % 16 || code_stride > (1LL << 39) || code_stride < span(n, code_ld, k / 2) ||
+         scale_stride < span(n, scale_ld, k / std::max(group, 1)) || (zeros && zero_stride < span(n, zero_ld, k / std::max(group, 1)))))
         return cudaErrorInvalidValue;
+    if (experts == 1) code_stride = scale_stride = zero_stride = 0;             // not read
     W4Args args{};
     args.codes = static_cast<const uint8_t*>(codes); args.code_ld = code_ld; args.code_stride = code_stride;
     args.scales = scales; args.scale_dtype = scale_dtype; args.scale_ld = scale_ld; args.scale_stride = scale_stride;

@@ -116,6 +116,19 @@ def test_w4_by_expert_refuses(pkg, change):
     assert pkg._cabi.lib().b200fp8_gemv_w4_experts(*args) == INVALID
 
 
+def test_one_experts_stride_is_not_read(pkg):
+    """The pitch from one expert's matrix to the next says nothing where there is one expert (calls without rows: nothing is launched)."""
+    lib = pkg._cabi.lib()
+    for stride in (7, -16, 1 << 60):
+        assert lib.b200fp8_gemm_grouped(1, 0, 128, 256, P, P, 0, 128, P, 0, 128, stride, P, 1, 256, None, None, None) != INVALID
+        assert lib.b200fp8_gemm_grouped_dgrad(1, 0, 128, 256, P, P, 0, 256, P, 0, 128, stride, P, 1, 128, None, None, None) != INVALID
+        assert lib.b200fp8_gemv_w4_experts(0, 0, 1, 64, 64, 64, P, 32, stride, P, 1, 1, stride, P, 1, stride, None, P, 1, 64, P, 1, 64, None) == 0
+    # with two it does, and a pitch between rows that overflows does not slip through
+    assert lib.b200fp8_gemm_grouped(2, 0, 128, 256, P, P, 0, 128, P, 0, 128, 7, P, 1, 256, None, None, None) == INVALID
+    assert lib.b200fp8_gemm_grouped(2, 0, 128, 1 << 30, P, P, 0, 128, P, 0, 1 << 38, 1 << 38, P, 1, 1 << 30, None, None, None) == INVALID
+    assert lib.b200fp8_gemv_w4_experts(0, 0, 2, 64, 65, 64, P, 32, 2080, P, 1, 1 << 58, 64, P, 1, 65, None, P, 1, 64, P, 1, 65, None) == INVALID
+
+
 def test_empty_calls_do_nothing(pkg):
     lib = pkg._cabi.lib()
     assert lib.b200fp8_quantize_rows(0, 0, 64, None, 1, 64, None, None, 0, 64, None, None) == 0

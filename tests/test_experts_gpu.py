@@ -620,6 +620,29 @@ def test_grouped_products_without_extent(g):
     assert (d == 6.0).all()
 
 
+@pytest.mark.parametrize("stride", [7, -16, 1 << 60])
+def test_one_experts_stride_is_not_read(g, stride):
+    n, k, rows = 48, 64, 70
+    lib, stream = g._cabi.lib(), torch.cuda.current_stream().cuda_stream
+    a, b, dy = fp8((rows, k), E4, 1), fp8((1, n, k), E4, 2), fp8((rows, n), E5, 3)
+    ends = ends_of([rows])
+    y, dx, dw = torch.empty((rows, n), device="cuda"), torch.empty((rows, k), device="cuda"), torch.empty((1, n, k), device="cuda")
+    at = lambda t: t.data_ptr()
+    assert lib.b200fp8_gemm_grouped(1, rows, k, n, at(ends), at(a), 0, k, at(b), 0, k, stride, at(y), 0, n, None, None, stream) == 0
+    assert lib.b200fp8_gemm_grouped_dgrad(1, rows, k, n, at(ends), at(dy), 1, n, at(b), 0, k, stride, at(dx), 0, k, None, None, stream) == 0
+    assert lib.b200fp8_gemm_grouped_wgrad(1, rows, k, n, at(ends), at(dy), 1, n, at(a), 0, k, at(dw), 0, k, stride, None, None, stream) == 0
+    done(g)
+    assert torch.equal(y, g.gemm_grouped(a, b, torch.empty_like(y), ends)) and torch.equal(dx, g.gemm_grouped_dgrad(dy, b, torch.empty_like(dx), ends))
+    assert torch.equal(dw, g.gemm_grouped_wgrad(dy, a, torch.empty_like(dw), ends))
+    codes, scales, z = weights((1,), n, k, 64, torch.float16, 4, True)
+    x = torch.randn((2, k), generator=gen(9), device="cuda").half()
+    expert, out = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.empty((2, n), device="cuda")
+    assert lib.b200fp8_gemv_w4_experts(2, 2, 1, k, n, 64, at(codes), k // 2, stride, at(scales), 2, 1, stride, at(z), 1, stride, at(expert), at(x), 2, k,
+                                       at(out), 0, n, stream) == 0
+    done(g)
+    assert torch.equal(out, g.gemv_w4_experts(codes, scales, x, torch.empty_like(out), expert, zeros=z))
+
+
 # ---- 4-bit weights ---------------------------------------------------------------------------------------------------
 
 
