@@ -208,6 +208,8 @@ int b200fp8_spmv_bell_f32(int m, int k, const void* ell_values, int a_dtype, lon
  * ep is the epilogue of b200fp8_gemm_rowcol_epilogue (NULL: D = convert(sum)), with b_row_scale and bias holding one value
  * per expert and column of D ([experts][columns of D]) and a_row_scale one per row; amax_d is taken over the rows of groups.
  * wgrad sums over the rows: it takes alpha, beta, a_scale, b_scale, d_scale and amax_d only (operands with one scale each).
+ * Scales that the forward pass had along the index that a gradient sums over -- its b_row_scale in dgrad, its a_row_scale in
+ * wgrad -- cannot be applied to the sum: multiply them into the gradient of the output before it is quantised.
  *
  * ld*: row pitches; stride_b / stride_d: pitch from one expert's matrix to the next (elements; not read for one expert).
  * Requirements: A and B 16-byte aligned; K, lda, ldb, stride_b and, in dgrad and wgrad, N multiples of 16; D aligned to its

@@ -178,6 +178,7 @@ def gemm_grouped_dgrad(a: torch.Tensor, b: torch.Tensor, d: torch.Tensor, ends: 
                        activation: str | int = 0, kernel: int = KERNEL_AUTO, max_ctas: int = 0):
     """The gradient of ``gemm_grouped`` by its rows: d[r] = ep(b[e]^T a[r]), with a [rows][N] the gradient of the output, the
     weights b [experts][N][K] as the forward pass has them, and d [rows][K].  Epilogue as there, vectors of [experts][K].
+    The forward pass's ``b_row_scale`` lies along the sum over N: multiply it into the gradient before that is quantised.
     N and K must be multiples of 16."""
     if a.dim() != 2 or b.dim() != 3 or d.dim() != 2 or ends.dim() != 1:
         _shapes(a, b, d, ends, "a [rows][N], b [experts][N][K], d [rows][K]")
@@ -193,7 +194,9 @@ def gemm_grouped_wgrad(a: torch.Tensor, b: torch.Tensor, d: torch.Tensor, ends: 
                        a_scale=None, b_scale=None, d_scale=None, amax_d=None, kernel: int = KERNEL_AUTO, max_ctas: int = 0):
     """The gradient of ``gemm_grouped`` by its weights: d[e] = alpha * a_scale * b_scale * sum over the rows r of group e of
     a[r]^T b[r], plus beta * d[e]; a [rows][N] is the gradient of the output, b [rows][K] the forward pass's input, d
-    [experts][N][K].  An empty group gives beta * d[e] (zeros for beta = 0).  N and K must be multiples of 16."""
+    [experts][N][K].  An empty group gives beta * d[e] (zeros for beta = 0).  The operands have one scale each: the forward
+    pass's ``a_row_scale`` lies along the sum over the rows, multiply it into the gradient before that is quantised.  N and K must be
+    multiples of 16."""
     if a.dim() != 2 or b.dim() != 2 or d.dim() != 3 or ends.dim() != 1:
         _shapes(a, b, d, ends, "a [rows][N], b [rows][K], d [experts][N][K]")
     experts, n, k = d.shape

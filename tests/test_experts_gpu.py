@@ -1041,6 +1041,40 @@ def test_training_step_of_a_layer(g):
         close(got, t * f + old, (steps(max(hidden, inner, max(sizes))) + 2.0 ** -21) * s * f + 2.0 ** -22, torch.float32)
 
 
+def test_documented_training_step_with_scales_of_rows_and_columns(g):
+    """The lines that the integration guide gives, run as they stand: gradients of the product with a scale per row and per
+    output channel.  dq * dq_scale is within half an E5M2 step (2^-3 of the value, at least 2^-17 of the scale) and a BF16
+    rounding (2^-8, here 2^-7 with the products of both) of dh * w1_scale; dr without the latter; the sums add FP32's roundings."""
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")).read()
+    lines = text[text.index("# a layer of experts"):text.index("# few tokens")]
+    hidden, inner, experts, tokens = 256, 320, 5, 300
+    source_row, ends, expert_of_row, _, _ = route(tokens, 2, experts, 6)
+    rows, expert_of_row = 2 * tokens, expert_of_row.long()
+    power = lambda shape, seed: torch.exp2(torch.randint(-4, 5, shape, generator=gen(seed), device="cuda").float())
+    x = (torch.randn((tokens, hidden), generator=gen(1), device="cuda") * power((tokens, 1), 2)).to(torch.bfloat16)
+    w1, w1_scale = fp8((experts, inner, hidden), E4, 3), power((experts, inner), 4) * (1 / 48 + torch.rand((experts, inner), generator=gen(5), device="cuda") / 48)
+    b1 = torch.zeros((experts, inner), device="cuda")
+    q, row_scale = torch.empty((rows, hidden), dtype=torch.uint8, device="cuda").view(E4), torch.empty(rows, device="cuda")
+    h, dh = torch.empty((rows, inner), dtype=torch.bfloat16, device="cuda"), torch.randn((rows, inner), generator=gen(7), device="cuda").to(torch.bfloat16)
+    dq, dq_scale = torch.empty((rows, inner), dtype=torch.uint8, device="cuda").view(E5), torch.empty(rows, device="cuda")
+    dx, dw1 = torch.empty((rows, hidden), device="cuda"), torch.empty((experts, inner, hidden), device="cuda")
+    names = dict(locals(), torch=torch)
+    exec(lines, names)
+    done(g)
+    real_w = w1.double() * w1_scale.double()[..., None]
+    real_x = q.double() * row_scale.double()[:, None]
+    for e, lo, hi in spans(torch.diff(ends, prepend=ends.new_zeros(1)).tolist()):
+        grad = dh[lo:hi].double()
+        folded = grad * w1_scale[e].double()
+        off = (2.0 ** -3 + 2.0 ** -7) * folded.abs() + 2.0 ** -17 * dq_scale[lo:hi, None].double()
+        want, s = grad @ real_w[e], folded.abs() @ w1[e].double().abs()
+        assert ((dx[lo:hi].double() - want).abs() <= off @ w1[e].double().abs() + 2 * (steps(inner) + 2.0 ** -21) * s).all()
+        folded = grad * row_scale[lo:hi, None].double()
+        off = (2.0 ** -3 + 2.0 ** -20) * folded.abs() + 2.0 ** -17 * names["dr_scale"].double()
+        want, s = grad.T @ real_x[lo:hi], folded.abs().T @ q[lo:hi].double().abs()
+        assert ((dw1[e].double() - want).abs() <= off.T @ q[lo:hi].double().abs() + 2 * (steps(hi - lo) + 2.0 ** -21) * s).all()
+
+
 @pytest.mark.parametrize("tokens", [1, 6])
 def test_decode_step_with_four_bit_experts(g, tokens):
     hidden, inner, experts, top_k = 512, 640, 16, 4
