@@ -15,12 +15,16 @@ A step is one operator call on operands resident in HBM.  `value` is whole-job T
 GPUs from the max-over-ranks device time; `e2e` is the same quantity through the host-pointer
 entry point (pinned host buffers, uploads and the download of C inside the timed region).
 
-Beside the headline the default run reports, in the same line:
+The line is one that a reader of a log's last few thousand characters gets whole: what goes beyond it (the largest of the
+keys below first, named in `in_details`) is written by `--details FILE`, a JSON object with every key.
+
+Beside the headline the default run measures:
     parity      the C buffer that was timed, checked after the timed region (FP64 oracle on sampled rows, columns and
                 points over the full K; a randomised product check of every element on the device)
     configs     (N = 1) every other benchmark configuration -- 1024^3, 4096^3 x 4 dtype pairs x ring depths, 8192^3,
                 the FFN shapes, the decode shapes -- each timed as CUDA graphs over rotating buffers, alternating with
                 cuBLASLt on the same buffers, with the parity of its own timed buffer
+                (`configs_summary` keeps the worst parity and the least and median ratio to cuBLASLt in the line)
     side        (N = 1) the reference's own kernels where they build for sm_100 (time only)
     sustained, allgather, fused_allgather   (N > 1) a one-second steady-state leg per GPU, the NCCL all-gather of the C
                 blocks, and the GEMM with the all-gather fused into its epilogue, each with its own parity
@@ -452,6 +456,26 @@ def measure_config(torch, g, cmp, dev, name, M, K, N, fa, fb, depth, kernel, pea
     return row
 
 
+LINE_LIMIT = 2600                # characters
+LINE_KEYS = ("metric", "value", "unit", "n_gpus", "steps", "warmup", "ms_per_step", "higher_is_better", "scaling", "vs_baseline", "dtype", "data",
+             "config", "roofline", "gpu_launches", "clocks", "e2e", "cpu_baseline")
+
+
+def emit(fd, line, details=None):
+    """Writes the result line to `fd`, without its largest extra keys where it would be too long, and all of it to `details`."""
+    if details:
+        with open(details, "w") as f:
+            json.dump(line, f, indent=1)
+    short, left_out = dict(line), []
+    for key in sorted((k for k in line if k not in LINE_KEYS), key=lambda k: -len(json.dumps(line[k]))):
+        if len(json.dumps(short)) <= LINE_LIMIT:
+            break
+        del short[key]
+        left_out.append(key)
+        short["in_details"] = left_out
+    os.write(fd, (json.dumps(short) + "\n").encode())
+
+
 def run_configs(torch, g, cmp, dev, peaks, budget_s=150.0):
     """Every benchmark configuration other than the headline.  Short ones first: after the power-capped long runs the
     clocks need a while to recover."""
@@ -477,8 +501,10 @@ def run_configs(torch, g, cmp, dev, peaks, budget_s=150.0):
             continue
         out[name] = measure_config(torch, g, cmp, dev, name, M, K, N, fa, fb, depth, kernel, peaks, seed=2 * idx)
     worst = [r["parity"]["worst"] for r in out.values() if "parity" in r]
+    ratios = sorted(round(r["vs_cublaslt"], 3) for r in out.values() if r.get("vs_cublaslt"))
     summary = {"rows": len(out), "measured": len(worst), "parity_worst": max(worst) if worst else None,
-               "all_within_tolerance": bool(worst) and max(worst) <= 1.0, "seconds": round(time.perf_counter() - t0, 1)}
+               "all_within_tolerance": bool(worst) and max(worst) <= 1.0,
+               "vs_cublaslt_least_median": [ratios[0], ratios[len(ratios) // 2]] if ratios else None, "seconds": round(time.perf_counter() - t0, 1)}
     return out, summary
 
 
@@ -784,6 +810,7 @@ def main() -> int:
     ap.add_argument("--no-e2e", action="store_true")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-extras", action="store_true", help="skip the configs / reference-kernel / collective legs")
+    ap.add_argument("--details", default=None, metavar="FILE", help="every key of the result as JSON, also those too large for the line")
     ap.add_argument("--no-parity", action="store_true", help="skip the check of the timed C buffer")
     ap.add_argument("--multimem", action="store_true", help="fused all-gather through NVSwitch multicast only (multimem stores)")
     ap.add_argument("--phase-timeline", action="store_true", help="kernel time stamps of one launch (diagnostics build)")
@@ -1151,7 +1178,7 @@ def main() -> int:
 
     if rank == 0:
         sys.stdout.flush()
-        os.write(json_fd, (json.dumps(line) + "\n").encode())
+        emit(json_fd, line, args.details)
     if world > 1:
         dist.barrier()
         dist.destroy_process_group()
