@@ -237,8 +237,9 @@ int b200fp8_gemm_grouped_wgrad(int experts, int rows, int k, int n, const int* e
  *
  * with i = index[r] (r itself for index = NULL) and top = 448 (E4M3) or 57344 (E5M2); nearest is round-to-nearest-even of
  * the exact quotient.  Infinities become +-top, a NaN stays a NaN.  index (DEVICE, int32) copies rows into the experts'
- * order on the way; an index outside [0, source_rows) makes a row of zeros.  Any K and any pitch; 16-byte aligned rows
- * of x and 8-byte aligned rows of q take the fast path.  q and scale must not overlap x.
+ * order on the way; an index outside [0, source_rows) makes a row of zeros.  Any K and any pitch; K a multiple of 8 up to
+ * 16384 with 16-byte aligned rows of x and 8-byte aligned rows of q takes the fast path, which reads a row once (the other
+ * takes about six times as long where rows are many).  q and scale must not overlap x.
  */
 int b200fp8_quantize_rows(int source_rows, int rows, int k, const void* x, int x_dtype, long long ldx, const int* index,
                           void* q, int q_dtype, long long ldq, float* scale, void* stream);
@@ -249,15 +250,17 @@ int b200fp8_quantize_rows(int source_rows, int rows, int k, const void* x, int x
  *     y[m][n] = sum over groups g of scales[n][g] * sum_{k in g} (codes[n][k] - zeros[n][g]) * x[m][k]
  *
  * codes: N rows of K/2 bytes, two codes 0..15 to a byte, the even k in the low half; code_ld is the row pitch in BYTES, a
- * multiple of 16.  scales: N rows of K/group values of scale_dtype (B200FP8_OUT_F32, _BF16 or _F16); zeros: N rows of
- * K/group bytes (their low four bits), or NULL for 8 throughout.  group is 32, 64 or 128 and divides K.  x: BF16 or FP16,
- * 16-byte aligned, ldx a multiple of 8; y: x's type or FP32.  Sums are FP32, the products before them exact.  Made for
- * few vectors: weights are read once per sixteen of them.  An infinity or NaN in x counts as it does in the formula.
+ * multiple of 16.  scales: N rows of K/group values of scale_dtype (B200FP8_OUT_F32, _BF16 or _F16), finite and below
+ * 2^100 in magnitude; zeros: N rows of K/group bytes (their low four bits), or NULL for 8 throughout.  group is 32, 64 or
+ * 128 and divides K.  x: BF16 or FP16, 16-byte aligned, ldx a multiple of 8; y: x's type or FP32.  Sums are FP32, the
+ * products before them exact, whatever the spread of x.  Made for few vectors: weights are read once per eight of them, or
+ * sixteen where there are more than eight.  An infinity or NaN in x counts as it does in the formula.
  *
  * b200fp8_gemv_w4_experts: row r of y takes the weights of expert[r] (DEVICE, int32) and row r / (rows / tokens) of x --
  * `rows` is a multiple of `tokens`, at most 4096; experts at most 4096.  A row whose expert lies outside [0, experts) is
  * left as it was.  Strides from one expert's matrix to the next: code_stride in bytes (a multiple of 16), scale_stride
- * and zero_stride in elements.  Each expert that occurs is read once per eight of its rows.
+ * and zero_stride in elements (none is read for one expert).  Each expert that occurs is read once per two of its rows in
+ * calls of one or two tokens on large weights, else once per eight, or per sixteen where an expert has more than eight on average.
  */
 int b200fp8_gemv_w4(int m, int k, int n, int group, const void* codes, long long code_ld, const void* scales, int scale_dtype,
                     long long scale_ld, const unsigned char* zeros, long long zero_ld, const void* x, int x_dtype, long long ldx,
@@ -380,7 +383,9 @@ int b200fp8_fill_normal(void* dst, long long count, int dtype, float sigma, unsi
 /*
  * Device status word of the current device: 0 when every kernel of this
  * library ran its pipeline to completion, otherwise the first recorded code
- * (a bounded wait inside a kernel ran out).  Synchronises the device.  `reset`
+ * (a bounded wait inside a kernel ran out: 101 producer, 102 matrix unit,
+ * 103 epilogue of the tiled and grouped products, 104 skinny products, 106
+ * 4-bit products).  Synchronises the device.  `reset`
  * non-zero clears the word after reading.  The reference has no counterpart:
  * its kernels cannot report anything (GEMM/src/gemm.cu:276 returns only the
  * launch status).

@@ -230,10 +230,12 @@ cudaError_t grouped(int mode, int experts, int rows, int k, int n, const int* en
     if (ep && ep->struct_bytes != static_cast<int>(sizeof(b200fp8_epilogue)) && ep->struct_bytes != B200FP8_EPILOGUE_V1_BYTES) return cudaErrorInvalidValue;
     const bool extended = ep && ep->struct_bytes == static_cast<int>(sizeof(b200fp8_epilogue));
     if (extended && (ep->activation < B200FP8_ACT_NONE || ep->activation > B200FP8_ACT_GELU_TANH)) return cudaErrorInvalidValue;
-    if (experts < 0 || rows < 0 || k <= 0 || n <= 0 || experts > kMaxExperts || rows > kMaxRows || k > kMaxRows || n > kMaxRows || !fp8(a_dtype) || !fp8(b_dtype)) return cudaErrorInvalidValue;
+    if (experts < 0 || rows < 0 || k <= 0 || n <= 0 || experts > kMaxExperts || rows > kMaxRows || k > kMaxRows || n > kMaxRows) return cudaErrorInvalidValue;
+    if (!fp8(a_dtype) || !fp8(b_dtype)) return cudaErrorInvalidValue;
     if (d_dtype < B200FP8_OUT_F32 || d_dtype > B200FP8_OUT_E5M2) return cudaErrorInvalidValue;
     const bool wgrad = mode == kGroupedWgrad;
-    if (ep && ep->bias && (ep->bias_dtype < B200FP8_OUT_F32 || ep->bias_dtype > B200FP8_OUT_F16 || !aligned(ep->bias, out_dtype_bytes(ep->bias_dtype)))) return cudaErrorInvalidValue;
+    if (ep && ep->bias && (ep->bias_dtype < B200FP8_OUT_F32 || ep->bias_dtype > B200FP8_OUT_F16)) return cudaErrorInvalidValue;
+    if (ep && ep->bias && !aligned(ep->bias, out_dtype_bytes(ep->bias_dtype))) return cudaErrorInvalidValue;
     if (ep && (!aligned(ep->amax_d, 4) || !aligned(ep->a_scale, 4) || !aligned(ep->b_scale, 4) || !aligned(ep->d_scale, 4))) return cudaErrorInvalidValue;
     if (extended && (!aligned(ep->a_row_scale, 4) || !aligned(ep->b_row_scale, 4))) return cudaErrorInvalidValue;
     // a bias, an activation or a scale of one row has no place in a sum over the rows
@@ -254,7 +256,8 @@ cudaError_t grouped(int mode, int experts, int rows, int k, int n, const int* en
         if (!ends || !aligned(ends, 4) || !d || !aligned(d, out_bytes)) return cudaErrorInvalidValue;
         if ((rows > 0 && !a) || ((!wgrad || rows > 0) && !b) || !aligned(a, 16) || !aligned(b, 16)) return cudaErrorInvalidValue;
         // a matrix of all rows has to be addressable as one tensor map
-        if (static_cast<double>(rows) * static_cast<double>(lda) > 5e11 || static_cast<double>(rows) * static_cast<double>(wgrad ? ldb : ldd) * out_bytes > 1e12) return cudaErrorInvalidValue;
+        const double height = rows;
+        if (height * static_cast<double>(lda) > 5e11 || height * static_cast<double>(wgrad ? ldb : ldd) * out_bytes > 1e12) return cudaErrorInvalidValue;
     }
     const int kernel = options ? options->kernel : B200FP8_KERNEL_AUTO;
     if (kernel != B200FP8_KERNEL_AUTO && kernel != B200FP8_KERNEL_PAIR_N256 && kernel != B200FP8_KERNEL_CTA1_N256 &&
@@ -349,8 +352,8 @@ cudaError_t launch_w4(const HostDevice& dev, W4Args args, cudaStream_t stream) {
                        experts > 1 ? args.code_stride : args.code_ld * static_cast<long long>(args.n), kW4BoxBytes, 16 * RT,
                        CU_TENSOR_MAP_SWIZZLE_128B)) != cudaSuccess)
         return e;
-    return launch(gemv_w4_kernel<BF16, G, NT, RT, WIDE, INT>, dev.pdl, dim3(splits, static_cast<unsigned>(tiles), static_cast<unsigned>(slots)), kW4Threads, bytes, splits,
-                  stream, map, args);
+    const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(tiles), static_cast<unsigned>(slots));
+    return launch(gemv_w4_kernel<BF16, G, NT, RT, WIDE, INT>, dev.pdl, grid, kW4Threads, bytes, splits, stream, map, args);
 }
 
 template <bool BF16, int G, bool WIDE>
@@ -447,7 +450,8 @@ int b200fp8_gemm_grouped_wgrad(int experts, int rows, int k, int n, const int* e
 
 int b200fp8_quantize_rows(int source_rows, int rows, int k, const void* x, int x_dtype, long long ldx, const int* index, void* q, int q_dtype,
                           long long ldq, float* scale, void* stream) {
-    if (source_rows < 0 || rows < 0 || k < 0 || k > kMaxRows || !fp8(q_dtype) || (x_dtype != B200FP8_OUT_BF16 && x_dtype != B200FP8_OUT_F16)) return cudaErrorInvalidValue;
+    if (source_rows < 0 || rows < 0 || k < 0 || k > kMaxRows) return cudaErrorInvalidValue;
+    if (!fp8(q_dtype) || (x_dtype != B200FP8_OUT_BF16 && x_dtype != B200FP8_OUT_F16)) return cudaErrorInvalidValue;
     if (ldx < k || ldq < k || (!index && rows > source_rows)) return cudaErrorInvalidValue;
     if (rows == 0) return cudaSuccess;
     if (!scale || !aligned(scale, 4) || !aligned(index, 4) || !aligned(x, 2)) return cudaErrorInvalidValue;

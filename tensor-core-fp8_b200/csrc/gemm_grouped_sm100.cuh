@@ -26,10 +26,10 @@
 //     16 to 128 rows, that covers them).  In the epilogue a lane owns columns, so the vectors per column (b_row_scale,
 //     bias) are a few registers.  FP32 rows go out as they are, 128 bytes per instruction.  16-bit ones are read from TMEM
 //     in the matrix-fragment distribution, packed in pairs along the rows and transposed on the way through shared memory
-//     by stmatrix, then stored 16 bytes per lane, or a row's 64 bytes from 32 lanes where the alignment allows no more (swapping columns between neighbouring lanes instead took four times the
-//     instructions, and the epilogue bounds products with a short contraction).  8-bit ones are packed four rows to a word
-//     and transposed 4 x 4 between four lanes, then stored 4 bytes per lane.  Rows behind a group's end are simply not
-//     stored, and D needs no TMA.
+//     by stmatrix, then stored 16 bytes per lane, or a row's 64 bytes from 32 lanes where the alignment allows no more
+//     (swapping columns between neighbouring lanes instead took four times the instructions, and the epilogue bounds
+//     products with a short contraction).  8-bit ones are packed four rows to a word and transposed 4 x 4 between four
+//     lanes, then stored 4 bytes per lane.  Rows behind a group's end are simply not stored, and D needs no TMA.
 //
 // Rows behind a group's end inside a tile belong to the next group.  Forward and dgrad may load and multiply them (each
 // row of a product depends on its own row of A only) and do not store them.  wgrad contracts over the rows, so the block
@@ -38,10 +38,10 @@
 // may hold infinities or NaN).  The MMA issues only as many K = 32 steps as there are rows.  A group without rows stores
 // zeros (or beta * D).
 //
-// Measured (per call, BF16 outputs): 32 rows over 16 experts of 4096 x 4096, 12 hit: 33.4 us, 6.0 TB/s of weights.  16384 rows, 16
-// experts of 8192 x 4096, bias and GELU: 420-530 us, 2.0-2.5 PFLOP/s, the power limit deciding.  dgrad of 8192 rows, 8 experts of
-// 8192 x 4096: 250 us, 2.2 PFLOP/s (the dense product of that size under the same load: 212).  wgrad of 8192 rows, 8 experts of
-// 4096 x 4096: 138-163 us; its store alone, 268 MB, takes 62.
+// Measured (per call, BF16 outputs; one launch - a long run, which the power limit slows): 32 rows over 16 experts of 4096 x
+// 4096, 12 hit: 33.4 us, 6.0 TB/s of weights.  16384 rows, 16 experts of 8192 x 4096, bias and GELU: 412 - 526 us (1.04 GHz),
+// 2.6 - 2.0 PFLOP/s, tensor pipe 81 % in the former.  dgrad of 8192 rows, 8 experts of 8192 x 4096: 202 - 262 us (1.09 GHz), 2.7 -
+// 2.1 PFLOP/s, tensor pipe 79 %.  wgrad of 8192 rows, 8 experts of 4096 x 4096: 138 - 166 us (1.43 GHz), tensor pipe 52 %.
 //
 // Every wait on an mbarrier is bounded, as in the dense kernel.
 #pragma once

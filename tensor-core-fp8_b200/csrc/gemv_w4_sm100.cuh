@@ -14,7 +14,7 @@
 // one costs; the order of k inside an instruction is free, and is chosen so that a lane's eight codes are one aligned
 // 32-bit word: (k, k + 4) share a 16-bit pair, which is what a mask takes out of the word.
 //
-// Bound by the weights' bytes from HBM: 13 weights per nanosecond at the measured rate, 47 per SM and clock, of which the
+// Bound by the weights' bytes from HBM: 13 weights per picosecond at the measured rate, 47 per SM and clock, of which the
 // instructions above take 9 per eight (a shift, four masks, four subtractions) plus the tensor core's one.  So the
 // kernel is about bytes in flight and few instructions:
 //
@@ -31,9 +31,9 @@
 // first of its expert, else block z stands for expert z.  Each expert's weights are read once per eight of its rows (two in the
 // integer form, which calls of one or two tokens take).
 //
-// Measured: one vector, 8192 x 8192, groups of 128: 12.8 us (2.7 TB/s; starting and joining the parts of K is about 5 of them); eight
+// Measured: one vector, 8192 x 8192, groups of 128: 12.4 us (2.8 TB/s; starting and joining the parts of K is about 5 of them); eight
 // vectors, 28672 x 8192, groups of 64 with zero points: 45.4 us (2.8 TB/s, 0.43 of a plain copy's rate); 16 tokens with 8 of 64
-// experts each, 2048 x 4096, groups of 128: 44.7 us.  Issue slots are half used: what bounds it is a warp's chain from a slot's
+// experts each, 2048 x 4096, groups of 128: 42.0 us.  Issue slots are half used: what bounds it is a warp's chain from a slot's
 // arrival over unpacking to the sums, about 380 instructions per 16 x 256 codes at 16 warps per SM (a third CTA per SM spills: 64 us).
 //
 // Waits on mbarriers are bounded as in the other kernels: a wait that runs out sets the status word and ends the kernel.
@@ -575,8 +575,10 @@ gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args args)     
                                         for (int u = 0; u < 2; ++u) {
                                             // z as a number: its byte below the bits of 2^23; all exact: whole numbers below 2^24
                                             const float z = __uint_as_float(__byte_perm(zeros[h][u], 0x4B000000u, 0x7540u | place)) - 8388608.0f;
-                                            ys[h][j][2 * u] = fmaf(scale(h, u), fmaf(-z, d.x, __int_as_float(c[h][j][2 * u])) - 12582912.0f, ys[h][j][2 * u]);
-                                            ys[h][j][2 * u + 1] = fmaf(scale(h, u), fmaf(-z, d.y, __int_as_float(c[h][j][2 * u + 1])) - 12582912.0f, ys[h][j][2 * u + 1]);
+                                            const float even = fmaf(-z, d.x, __int_as_float(c[h][j][2 * u])) - 12582912.0f;
+                                            const float odd = fmaf(-z, d.y, __int_as_float(c[h][j][2 * u + 1])) - 12582912.0f;
+                                            ys[h][j][2 * u] = fmaf(scale(h, u), even, ys[h][j][2 * u]);
+                                            ys[h][j][2 * u + 1] = fmaf(scale(h, u), odd, ys[h][j][2 * u + 1]);
                                         }
                                 }
                             } else {
