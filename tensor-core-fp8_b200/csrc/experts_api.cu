@@ -360,7 +360,7 @@ template <bool BF16, int G, bool WIDE>
 cudaError_t launch_w4_form(const HostDevice& dev, const W4Args& args, cudaStream_t stream) {
     // One or two vectors (a token's experts are usually different ones, so two tokens give an expert two rows) of weights beyond
     // 2^25 take the integer form.  Groups of 128: 8192 x 8192 12.8 us against 14.2, 28672 x 8192 32.2 against 39.0, but 4096 x 4096
-    // 9.0 against 8.3 and 16384 x 2048 10.8 against 10.8 for two vectors; groups of 64: 28672 x 8192 37.6 against 41.8, 4096 x 4096
+    // 9.0 against 8.3 and, at the border, 16384 x 2048 10.5 against 10.7; groups of 64: 28672 x 8192 37.6 against 41.8, 4096 x 4096
     // 9.6 against 8.4.  With groups of 32 its work per group outweighs the rest (8192 x 8192 18.2 against 17.9, 4096 x 4096 9.5
     // against 8.5).  Filling two tiles of columns with the digits of more vectors lost to the other form everywhere.
     const int vectors = args.expert ? args.m / args.rows_per_x : args.m;

@@ -219,8 +219,9 @@ def gemv_w4(codes: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, y: torch
     """y[m] = W x[m] for a matrix of 4-bit weights W[n][k] = scales[n][k // group] * (codes[n][k] - zeros[n][k // group]).
 
     codes is uint8 [N][K/2], two codes to a byte with the even k in the low half; scales [N][K/group] is float32, bfloat16 or
-    float16 and says the group size (32, 64 or 128); zeros is uint8 of the same shape, or None for 8.  x [M][K] is bfloat16 or
-    float16, y [M][N] has its type or float32.  Made for a few vectors.  Returns y.
+    float16, finite and below 2^100, and says the group size (32, 64 or 128); zeros is uint8 of the same shape, or None for 8.
+    x [M][K] is bfloat16 or float16, y [M][N] has its type or float32.  Products are exact and sums float32, whatever the spread of
+    x.  Made for a few vectors.  Returns y.
     """
     if codes.dim() != 2 or scales.dim() != 2 or x.dim() != 2 or y.dim() != 2:
         raise ValueError("codes [N][K/2], scales [N][K/group], x [M][K], y [M][N]")
