@@ -830,6 +830,39 @@ def test_w4_one_or_two_vectors_of_large_weights(g, x_dtype, scale_dtype, group, 
     assert torch.equal(torch.sign(y[torch.isinf(y)]).double(), torch.sign(want[torch.isinf(want)]))
 
 
+def test_w4_of_large_weights_replayed_on_two_streams(g):
+    """Two captured calls at once, replayed with other vectors than the captured ones: narrow, wide in some blocks, infinite."""
+    n, k, group = 4100, 8320, 64
+    graphs, streams, states = [], [torch.cuda.Stream() for _ in range(2)], []
+    for i, stream in enumerate(streams):
+        codes, scales, z = weights((), n, k, group, torch.float16, 5 + i, True)
+        x, y = torch.ones((1 + i, k), dtype=torch.bfloat16, device="cuda"), torch.empty((1 + i, n), device="cuda")
+        g.gemv_w4(codes, scales, x, y, zeros=z)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            for _ in range(20):
+                g.gemv_w4(codes, scales, x, y, zeros=z)
+        graphs.append(graph)
+        states.append((codes, scales, z, x, y))
+    for at, value in ((0, 0.0), (300, 1e6), (5000, 1e30), (77, float("inf"))):
+        for i, (codes, scales, z, x, y) in enumerate(states):
+            x.copy_(torch.randn(x.shape, generator=gen(at + i), device="cuda"))
+            x[-1, at] = value
+            y.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        done(g)
+        for codes, scales, z, x, y in states:
+            w = weights64(codes, scales, z)
+            if math.isinf(value):
+                assert not torch.isfinite(y[-1]).any()
+                x, y = x[:-1], y[:-1]
+            w4_close(y, w, x, k, torch.float32)
+
+
 @pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("group,zeros", [(64, True), (128, False)])
 @pytest.mark.parametrize("tokens,top_k,experts,n,k", [(1, 8, 9, 1000, 8320), (2, 4, 40, 515, 8320), (2, 12, 3, 700, 32896)])
